@@ -235,6 +235,150 @@ int shk_cuda_kv_attend_batch(shk_kv *kv, uint32_t layer0, uint32_t n_seq, const 
 void shk_cuda_kv_clear(shk_kv *kv);
 uint32_t shk_cuda_kv_seq_len(shk_kv *kv, uint32_t layer);
 
+/* ---- paged K/V pools in 8 bits, shared by the requests of a batch.  No
+ *      counterpart in the reference, which decodes one sequence from one cache
+ *      (engine/include/kv_cache.h:5-37).  A pool is cut into blocks of
+ *      block_tokens positions; a request holds the blocks that its block table
+ *      lists, so requests of different lengths share one pool without gaps.
+ *      Values are held in 8 bits with one fp32 scale per block and head (K and
+ *      V apart): value = scale * byte.  Buffers belong to the caller; one
+ *      struct shk_pages describes one layer's.
+ *
+ *      A step of a batch: shk_cuda_pages_release (blocks of the requests that
+ *      ended), shk_cuda_pages_assign (blocks, slots, positions of the new
+ *      tokens), per layer shk_cuda_pages_append and shk_cuda_pages_attend, then
+ *      shk_cuda_sample on the logits.  All of it is stream-ordered and reads
+ *      lengths on the device only, so a captured step can be replayed.
+ *
+ *      Lengths, slots, positions and block ids are int32.  A bad one (a block
+ *      id outside the pool, a position outside the table, a slot outside the
+ *      pool) is left out and recorded: shk_cuda_check returns SHK_EDEVICE. ---- */
+#define SHK_PAGES_I8 0u   /* signed integers -127..127 */
+#define SHK_PAGES_E4M3 1u /* 8-bit floating point: 4 exponent, 3 mantissa bits, largest value 448 */
+#define SHK_PAGES_MAX_SEQ 16384u
+#define SHK_PAGES_MAX_ROWS 65535u
+/* types of activations (ggml's codes) */
+#define SHK_DTYPE_F32 0u
+#define SHK_DTYPE_F16 1u
+#define SHK_DTYPE_BF16 30u
+struct shk_pages {
+    void *k_dev, *v_dev;              /* [n_blocks][n_kv_heads][block_tokens][head_dim] bytes, 16-byte aligned */
+    float *k_scale_dev, *v_scale_dev; /* [n_blocks][n_kv_heads] */
+    uint32_t type;                    /* SHK_PAGES_* */
+    uint32_t n_blocks;                /* n_blocks * block_tokens < 2^31 */
+    uint32_t n_kv_heads;              /* at most 1024 */
+    uint32_t head_dim;                /* 64 or 128 */
+    uint32_t block_tokens;            /* 16, 32, 64, 128 or 256 */
+};
+/* Block tables and slots from lengths.  Request r holds have[r] tokens in the
+ * blocks table[r][0 ..] and gets add[r] more.  Requests are served in order:
+ * their rows (one per new token) are laid out one request after the other, and
+ * a new block of theirs is taken from the top of the free stack
+ * free_dev[0 .. *n_free_dev).  Row i: slots[i] = block * block_tokens + place in
+ * the block, pos[i] = position in the request, seq[i] = request.  Rows that no
+ * token takes get -1 in all three.  A request is refused whole -- lens[r] =
+ * have[r], its rows -1, no block taken -- when its tokens outgrow table_stride
+ * blocks, its rows outgrow n_rows, or its blocks and those asked for by the
+ * requests before it outgrow the free stack; rows are counted as if every
+ * request before it had been served.  lens_dev may be have_dev, and counts_dev
+ * may be n_free_dev.  One launch; async on stream. */
+struct shk_pages_assign {
+    uint32_t n_seq;        /* request slots: 1 .. SHK_PAGES_MAX_SEQ */
+    uint32_t block_tokens; /* 16 .. 256, a power of two */
+    uint32_t n_blocks;     /* blocks in the pool */
+    uint32_t table_stride; /* block ids per table row */
+    uint32_t n_rows;       /* rows laid out, at most 2^30 - 1 */
+    const int32_t *have_dev, *add_dev; /* [n_seq] */
+    int32_t *table_dev;                /* [n_seq][table_stride]: read for the blocks held, new ones written */
+    const int32_t *free_dev;           /* [n_blocks], the stack; not changed */
+    const int32_t *n_free_dev;         /* [1] its height */
+    int32_t *lens_dev;                 /* [n_seq] out: tokens after the step */
+    int32_t *counts_dev;               /* [3] out: free blocks left, rows taken, requests refused */
+    int32_t *slots_dev, *pos_dev, *seq_dev; /* [n_rows] out */
+    int32_t *last_dev;                 /* [n_seq] out: the request's last row (its next token's logits), or -1 */
+};
+int shk_cuda_pages_assign(shk_ctx *ctx, const struct shk_pages_assign *a, void *stream);
+/* Gives the blocks of the requests with done[r] != 0 back: pushed on the free
+ * stack in request and table order, lens[r] = 0 (have[r] for the others), the
+ * new height to n_free_out_dev.  lens_dev may be have_dev, n_free_out_dev may be
+ * n_free_dev.  Where the stack would outgrow n_blocks (a block given back
+ * twice) nothing is given back and shk_cuda_check returns SHK_EDEVICE. */
+int shk_cuda_pages_release(shk_ctx *ctx, uint32_t n_seq, uint32_t block_tokens, uint32_t n_blocks,
+                           uint32_t table_stride, const int32_t *table_dev, const int32_t *done_dev,
+                           const int32_t *have_dev, int32_t *lens_dev, int32_t *free_dev,
+                           const int32_t *n_free_dev, int32_t *n_free_out_dev, void *stream);
+/* Quantise-and-store n_tokens rows of K and V (dtype F32, F16 or BF16; row i at
+ * i * row_stride elements, 0 = n_kv_heads * head_dim) at slots_dev[i]; a
+ * negative slot is a padding row and is skipped.  Per block and head the scale
+ * is max|x| / 127 (E4M3: / 448) over the tokens it has taken since its first
+ * place was last written: a token that raises it has the block's earlier
+ * places rounded again to the new scale.  Quotients are formed in fp32 and
+ * rounded half to even; NaN counts for nothing and is stored as 0; an infinity
+ * makes the scale infinite (the block then reads as NaN).  The rows of one
+ * block must be consecutive in the call and rising by one, as
+ * shk_cuda_pages_assign lays them out: a block's second run in one call is not
+ * stored, and shk_cuda_check returns SHK_EDEVICE.  Calls that append to one
+ * block must be ordered (one stream).  Async on stream. */
+int shk_cuda_pages_append(shk_ctx *ctx, const struct shk_pages *pages, uint32_t n_tokens, const void *k_dev,
+                          const void *v_dev, uint32_t dtype, size_t row_stride, const int32_t *slots_dev,
+                          void *stream);
+/* The values at slots_dev[0 .. n_tokens) as fp32 rows of n_kv_heads * head_dim;
+ * rows of negative slots are left as they were. */
+int shk_cuda_pages_read(shk_ctx *ctx, const struct shk_pages *pages, uint32_t n_tokens, const int32_t *slots_dev,
+                        float *k_dev, float *v_dev, void *stream);
+/* Attention of n_rows query rows: row i belongs to request seq[i] (seq_dev NULL:
+ * request i) and sees its positions 0 .. pos[i], so a decode row, the draft
+ * rows of one request and the rows of a prompt all have the causal mask that
+ * pos gives.  Query head h reads KV head h % n_kv_heads, as op_attention does
+ * (engine/src/ops.c:423).  pos < 0: the row sees nothing and becomes zeros;
+ * seq < 0: no row (padding), out left as it was.  q and out are dtype F32, F16
+ * or BF16 rows of n_heads * head_dim, q_stride / out_stride elements apart (0 =
+ * dense); out may not overlap q.  Sums and softmax in fp32.  ws_dev:
+ * shk_cuda_pages_attend_ws bytes, 16-byte aligned, contents of no account
+ * before and after; calls that may run at the same time need one each. */
+struct shk_pages_rows {
+    uint32_t n_rows;  /* at most SHK_PAGES_MAX_ROWS */
+    uint32_t n_heads; /* a multiple of n_kv_heads, at most 4096 */
+    uint32_t dtype;
+    const void *q_dev;
+    void *out_dev;
+    size_t q_stride, out_stride;
+    const int32_t *seq_dev, *pos_dev; /* [n_rows] */
+    const int32_t *table_dev;         /* [n_seq][table_stride] */
+    uint32_t n_seq, table_stride;
+    float scale;
+    void *ws_dev;
+    size_t ws_bytes;
+};
+size_t shk_cuda_pages_attend_ws(uint32_t n_rows, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);
+int shk_cuda_pages_attend(shk_ctx *ctx, const struct shk_pages *pages, const struct shk_pages_rows *rows,
+                          void *stream);
+
+/* ---- sampling: one token per row of logits from given random numbers (the
+ *      reference only takes the argmax, engine/src/engine.c:424-431).  Row i of
+ *      the logits (dtype F32, F16 or BF16) is at i * row_stride elements (0 =
+ *      n_vocab).  temperature, top_k, top_p, min_p: one value per row, or NULL
+ *      for off.  u_dev: one number in [0, 1) per row.
+ *       - weights w = exp((z - z_max) / T); T <= 0 or NaN: the first index of
+ *         the maximum, as shk_cuda_argmax; NaN and -inf logits have weight 0;
+ *       - top_k > 0: the k largest logits stay, equal ones by lower index;
+ *       - top_p < 1: of those, from the largest down, each stays while the
+ *         weights before it sum to less than top_p of them all (one always does);
+ *       - min_p > 0: tokens with w < min_p go (w is 1 for the largest);
+ *       - the first token, in index order, at which the running sum of the
+ *         weights that stay exceeds u of their total.
+ *      out_dev[i] = its index, prob_dev[i] (if not NULL) = its weight over that
+ *      total.  A row without a logit above -inf gives SHK_SAMPLE_NONE and 0.
+ *      Weights are summed as whole multiples of 2^-40: the same inputs give the
+ *      same token on every run, and weights below 2^-40 count for nothing.
+ *      Async on stream; no workspace. ---- */
+#define SHK_SAMPLE_NONE 0xFFFFFFFFu
+#define SHK_SAMPLE_MAX_VOCAB 262144u /* larger: SHK_EUNSUPPORTED */
+int shk_cuda_sample(shk_ctx *ctx, const void *logits_dev, uint32_t dtype, uint32_t n_rows, uint32_t n_vocab,
+                    size_t row_stride, const float *temperature_dev, const int32_t *top_k_dev,
+                    const float *top_p_dev, const float *min_p_dev, const float *u_dev, uint32_t *out_dev,
+                    float *prob_dev, void *stream);
+
 /* ---- model: per-layer forward, embed, lm_head+argmax, captured decode step ---- */
 struct shk_model_desc {            /* struct model_info (model_loader.h:66-74) + resident */
     uint32_t n_layers, n_embd, n_heads, n_kv_heads, head_dim, n_ff, n_vocab;

@@ -19,8 +19,10 @@
 #include "gemv.cuh"
 #include "glue.cuh"
 #include "mmv.cuh"
+#include "pages.cuh"
 #include "q5k.cuh"
 #include "prefill_layer.cuh"
+#include "sample.cuh"
 #include "tp_ll.cuh"
 
 using // Fewest cached positions per attention split (CTA of a KV head's cluster).
@@ -445,6 +447,7 @@ shk_ctx* shk_cuda_init(const shk_cuda_config* cfg) {
   ok = ok && gemv_init() == cudaSuccess;
   ok = ok && mmv_init() == cudaSuccess;
   ok = ok && q5k_init() == cudaSuccess;
+  ok = ok && pages_init() == cudaSuccess;
   ok = ok && cudaMalloc(&c->mmv_scratch, MMV_SCRATCH_BYTES) == cudaSuccess;
   ok = ok && cudaMemset(c->mmv_scratch, 0, MMV_SCRATCH_BYTES) == cudaSuccess;
   if (!ok) {
@@ -871,6 +874,175 @@ void shk_cuda_kv_clear(shk_kv* kv) {
 uint32_t shk_cuda_kv_seq_len(shk_kv* kv, uint32_t layer) {
   return (kv && layer < kv->L.n_layers) ? kv->seq[layer] : 0;
 }
+
+// --------------------- paged 8-bit K/V pools, sampling ------------------------
+
+// Largest block counts keep every slot in an int32.
+static bool pages_dims(uint32_t n_blocks, uint32_t block_tokens, uint32_t* shift) {
+  if (block_tokens < 16 || block_tokens > 256 || (block_tokens & (block_tokens - 1))) return false;
+  *shift = 31u - (uint32_t)__builtin_clz(block_tokens);
+  return n_blocks > 0 && (uint64_t)n_blocks << *shift <= 0x7FFFFFFFull;
+}
+
+static bool act_dtype(uint32_t dt) { return dt == DT_F32 || dt == DT_F16 || dt == DT_BF16; }
+
+static bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+static int pages_pool(const shk_pages* p, PagesPool* out) {
+  if (!p || !p->k_dev || !p->v_dev || !p->k_scale_dev || !p->v_scale_dev || !p->n_kv_heads) return SHK_EINVAL;
+  if (!aligned(p->k_dev, 16) || !aligned(p->v_dev, 16) || !aligned(p->k_scale_dev, 4) || !aligned(p->v_scale_dev, 4))
+    return SHK_EINVAL;
+  if (p->type != SHK_PAGES_I8 && p->type != SHK_PAGES_E4M3) return SHK_EUNSUPPORTED;
+  if (p->head_dim != 64 && p->head_dim != 128) return SHK_EUNSUPPORTED;
+  out->k = static_cast<uint8_t*>(p->k_dev);
+  out->v = static_cast<uint8_t*>(p->v_dev);
+  out->ks = p->k_scale_dev;
+  out->vs = p->v_scale_dev;
+  out->type = p->type;
+  out->n_blocks = p->n_blocks;
+  out->n_kv = p->n_kv_heads;
+  out->hd = p->head_dim;
+  if (p->n_kv_heads > 1024) return SHK_EINVAL;
+  return pages_dims(p->n_blocks, p->block_tokens, &out->block_shift) ? SHK_OK : SHK_EINVAL;
+}
+
+int shk_cuda_pages_assign(shk_ctx* c, const shk_pages_assign* a, void* s) {
+  if (c) on_dev(c);
+  if (!c || !a || !a->have_dev || !a->add_dev || !a->table_dev || !a->free_dev || !a->n_free_dev || !a->lens_dev ||
+      !a->counts_dev || !a->last_dev)
+    return SHK_EINVAL;
+  if (a->n_rows && (!a->slots_dev || !a->pos_dev || !a->seq_dev)) return SHK_EINVAL;
+  AssignArgs g{};
+  if (!pages_dims(a->n_blocks, a->block_tokens, &g.block_shift)) return SHK_EINVAL;
+  if (!a->n_seq || a->n_seq > SHK_PAGES_MAX_SEQ || !a->table_stride || a->n_rows > 0x3FFFFFFFu) return SHK_EINVAL;
+  g.n_seq = a->n_seq;
+  g.n_blocks = a->n_blocks;
+  g.stride = a->table_stride;
+  g.n_rows = a->n_rows;
+  g.have = a->have_dev;
+  g.add = a->add_dev;
+  g.table = a->table_dev;
+  g.free_ids = a->free_dev;
+  g.n_free = a->n_free_dev;
+  g.lens = a->lens_dev;
+  g.counts = a->counts_dev;
+  g.slots = a->slots_dev;
+  g.pos = a->pos_dev;
+  g.seq = a->seq_dev;
+  g.last = a->last_dev;
+  g.err = c->d_err;
+  CK(pages_assign_launch(g, pick(c, s)));
+  return SHK_OK;
+}
+
+int shk_cuda_pages_release(shk_ctx* c, uint32_t n_seq, uint32_t block_tokens, uint32_t n_blocks, uint32_t table_stride,
+                           const int32_t* table, const int32_t* done, const int32_t* have, int32_t* lens,
+                           int32_t* free_ids, const int32_t* n_free, int32_t* n_free_out, void* s) {
+  if (c) on_dev(c);
+  if (!c || !table || !done || !have || !lens || !free_ids || !n_free || !n_free_out) return SHK_EINVAL;
+  ReleaseArgs g{};
+  if (!pages_dims(n_blocks, block_tokens, &g.block_shift)) return SHK_EINVAL;
+  if (!n_seq || n_seq > SHK_PAGES_MAX_SEQ || !table_stride) return SHK_EINVAL;
+  g.n_seq = n_seq;
+  g.n_blocks = n_blocks;
+  g.stride = table_stride;
+  g.table = table;
+  g.done = done;
+  g.have = have;
+  g.lens = lens;
+  g.free_ids = free_ids;
+  g.n_free = n_free;
+  g.n_free_out = n_free_out;
+  g.err = c->d_err;
+  CK(pages_release_launch(g, pick(c, s)));
+  return SHK_OK;
+}
+
+int shk_cuda_pages_append(shk_ctx* c, const shk_pages* p, uint32_t n_tokens, const void* k, const void* v,
+                          uint32_t dtype, size_t row_stride, const int32_t* slots, void* s) {
+  if (c) on_dev(c);
+  PagesPool g{};
+  const int rc = c ? pages_pool(p, &g) : SHK_EINVAL;
+  if (rc) return rc;
+  if (n_tokens == 0) return SHK_OK;
+  if (!act_dtype(dtype)) return SHK_EUNSUPPORTED;
+  const size_t width = (size_t)g.n_kv * g.hd, es = dtype == DT_F32 ? 4 : 2;
+  if (!k || !v || !slots || !aligned(k, es) || !aligned(v, es) || n_tokens > 0x7FFFFFFFu ||
+      (row_stride && row_stride < width))
+    return SHK_EINVAL;
+  CK(pages_append_launch(g, n_tokens, k, v, dtype, row_stride ? row_stride : width, slots, c->d_err, pick(c, s)));
+  return SHK_OK;
+}
+
+int shk_cuda_pages_read(shk_ctx* c, const shk_pages* p, uint32_t n_tokens, const int32_t* slots, float* k, float* v,
+                        void* s) {
+  if (c) on_dev(c);
+  PagesPool g{};
+  const int rc = c ? pages_pool(p, &g) : SHK_EINVAL;
+  if (rc) return rc;
+  if (n_tokens == 0) return SHK_OK;
+  if (!k || !v || !slots || !aligned(k, 4) || !aligned(v, 4) || n_tokens > 0x7FFFFFFFu) return SHK_EINVAL;
+  CK(pages_read_launch(g, n_tokens, slots, k, v, c->d_err, pick(c, s)));
+  return SHK_OK;
+}
+
+size_t shk_cuda_pages_attend_ws(uint32_t n_rows, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim) {
+  if (!n_heads || !n_kv_heads || n_heads % n_kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
+  return pages_attend_ws_bytes(n_rows, n_heads, n_kv_heads, head_dim);
+}
+
+int shk_cuda_pages_attend(shk_ctx* c, const shk_pages* p, const shk_pages_rows* r, void* s) {
+  if (c) on_dev(c);
+  PagesAttnArgs g{};
+  const int rc = c ? pages_pool(p, &g.pool) : SHK_EINVAL;
+  if (rc) return rc;
+  if (!r) return SHK_EINVAL;
+  if (r->n_rows == 0) return SHK_OK;
+  if (!act_dtype(r->dtype)) return SHK_EUNSUPPORTED;
+  const size_t width = (size_t)r->n_heads * g.pool.hd, es = r->dtype == DT_F32 ? 4 : 2;
+  if (!r->n_heads || r->n_heads % g.pool.n_kv || r->n_heads > 4096 || !r->q_dev || !r->out_dev || !r->pos_dev ||
+      !r->table_dev || !r->table_stride || !r->n_seq || !aligned(r->q_dev, es) || !aligned(r->out_dev, es) ||
+      (r->q_stride && r->q_stride < width) || (r->out_stride && r->out_stride < width) ||
+      (!r->seq_dev && r->n_rows > r->n_seq) || r->n_rows > SHK_PAGES_MAX_ROWS ||
+      (uint64_t)r->table_stride * p->block_tokens > 0x7FFFFFFFull)
+    return SHK_EINVAL;
+  if (!r->ws_dev || !aligned(r->ws_dev, 16) ||
+      r->ws_bytes < pages_attend_ws_bytes(r->n_rows, r->n_heads, g.pool.n_kv, g.pool.hd))
+    return SHK_EINVAL;
+  g.n_rows = r->n_rows;
+  g.n_seq = r->n_seq;
+  g.n_heads = r->n_heads;
+  g.dtype = r->dtype;
+  g.q = r->q_dev;
+  g.out = r->out_dev;
+  g.q_stride = r->q_stride ? r->q_stride : width;
+  g.out_stride = r->out_stride ? r->out_stride : width;
+  g.row_seq = r->seq_dev;
+  g.row_pos = r->pos_dev;
+  g.table = r->table_dev;
+  g.stride = r->table_stride;
+  g.scale = r->scale;
+  g.ws = r->ws_dev;
+  g.err = c->d_err;
+  CK(pages_attend_launch(g, c->num_sms, pick(c, s)));
+  return SHK_OK;
+}
+
+int shk_cuda_sample(shk_ctx* c, const void* logits, uint32_t dtype, uint32_t n_rows, uint32_t n_vocab,
+                    size_t row_stride, const float* temperature, const int32_t* top_k, const float* top_p,
+                    const float* min_p, const float* u, uint32_t* out, float* prob, void* s) {
+  if (c) on_dev(c);
+  if (!c || !n_vocab || (row_stride && row_stride < n_vocab)) return SHK_EINVAL;
+  if (n_rows == 0) return SHK_OK;
+  if (!act_dtype(dtype) || n_vocab > SHK_SAMPLE_MAX_VOCAB) return SHK_EUNSUPPORTED;
+  if (!logits || !u || !out || !aligned(logits, dtype == DT_F32 ? 4 : 2) || n_rows > SHK_PAGES_MAX_ROWS)
+    return SHK_EINVAL;
+  const SampleArgs g{logits, dtype, n_rows, n_vocab, row_stride ? row_stride : n_vocab, temperature, top_k, top_p,
+                     min_p,  u,     out,    prob};
+  CK(sample_launch(g, c->num_sms, pick(c, s)));
+  return SHK_OK;
+}
+
 
 // --------------------------------- model --------------------------------------
 

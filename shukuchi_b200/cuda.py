@@ -56,6 +56,26 @@ class LayerDesc(C.Structure):
                 ("row_stride_v", C.c_uint32), ("row_stride_down", C.c_uint32)]
 
 
+class PagesDesc(C.Structure):
+    _fields_ = [("k_dev", C.c_void_p), ("v_dev", C.c_void_p), ("k_scale_dev", C.c_void_p),
+                ("v_scale_dev", C.c_void_p), ("type", C.c_uint32), ("n_blocks", C.c_uint32),
+                ("n_kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("block_tokens", C.c_uint32)]
+
+
+class PagesAssign(C.Structure):
+    _fields_ = [("n_seq", C.c_uint32), ("block_tokens", C.c_uint32), ("n_blocks", C.c_uint32),
+                ("table_stride", C.c_uint32), ("n_rows", C.c_uint32)] + \
+               [(n + "_dev", C.c_void_p) for n in ("have", "add", "table", "free", "n_free", "lens", "counts",
+                                                   "slots", "pos", "seq", "last")]
+
+
+class PagesRows(C.Structure):
+    _fields_ = [("n_rows", C.c_uint32), ("n_heads", C.c_uint32), ("dtype", C.c_uint32), ("q_dev", C.c_void_p),
+                ("out_dev", C.c_void_p), ("q_stride", C.c_size_t), ("out_stride", C.c_size_t),
+                ("seq_dev", C.c_void_p), ("pos_dev", C.c_void_p), ("table_dev", C.c_void_p), ("n_seq", C.c_uint32),
+                ("table_stride", C.c_uint32), ("scale", C.c_float), ("ws_dev", C.c_void_p), ("ws_bytes", C.c_size_t)]
+
+
 P, U32, U64, I, F, SZ = C.c_void_p, C.c_uint32, C.c_uint64, C.c_int, C.c_float, C.c_size_t
 _SIGS = {
     "shk_cuda_init": (P, [C.POINTER(CudaConfig)]),
@@ -109,6 +129,13 @@ _SIGS = {
     "shk_cuda_kv_read_blocks": (I, [P, U32, U32, U32, P, P, P]),
     "shk_cuda_kv_attend": (I, [P, U32, P, P, P, P, U32, U32, F, P]),
     "shk_cuda_kv_attend_batch": (I, [P, U32, U32, P, P, P, P, U32, U32, F, P]),
+    "shk_cuda_pages_assign": (I, [P, C.POINTER(PagesAssign), P]),
+    "shk_cuda_pages_release": (I, [P, U32, U32, U32, U32, P, P, P, P, P, P, P, P]),
+    "shk_cuda_pages_append": (I, [P, C.POINTER(PagesDesc), U32, P, P, U32, SZ, P, P]),
+    "shk_cuda_pages_read": (I, [P, C.POINTER(PagesDesc), U32, P, P, P, P]),
+    "shk_cuda_pages_attend_ws": (SZ, [U32, U32, U32, U32]),
+    "shk_cuda_pages_attend": (I, [P, C.POINTER(PagesDesc), C.POINTER(PagesRows), P]),
+    "shk_cuda_sample": (I, [P, P, U32, U32, U32, SZ, P, P, P, P, P, P, P, P]),
     "shk_cuda_kv_clear": (None, [P]),
     "shk_cuda_kv_seq_len": (U32, [P, U32]),
     "shk_cuda_model_create": (P, [P, C.POINTER(ModelDesc), P]),
@@ -263,6 +290,26 @@ class Context:
         _call("shk_cuda_argmax", self.h, x, n, C.byref(out))
         return out.value
 
+    # request batches
+    def pages_assign(self, n_seq, block_tokens, n_blocks, table_stride, n_rows, have, add, table, free, n_free, lens,
+                     counts, slots, pos, seq, last, stream=None):
+        """Block tables, slots and positions of every request's new tokens (shk_cuda_pages_assign)."""
+        a = PagesAssign(n_seq, block_tokens, n_blocks, table_stride, n_rows, have, add, table, free, n_free, lens,
+                        counts, slots, pos, seq, last)
+        _call("shk_cuda_pages_assign", self.h, C.byref(a), stream)
+
+    def pages_release(self, n_seq, block_tokens, n_blocks, table_stride, table, done, have, lens, free, n_free,
+                      n_free_out, stream=None):
+        """Blocks of the requests that are done, back on the free stack."""
+        _call("shk_cuda_pages_release", self.h, n_seq, block_tokens, n_blocks, table_stride, table, done, have, lens,
+              free, n_free, n_free_out, stream)
+
+    def sample(self, logits, n_rows, n_vocab, u, out, prob=None, temperature=None, top_k=None, top_p=None,
+               min_p=None, dtype=0, row_stride=0, stream=None):
+        """One token per row of logits (shk_cuda_sample); settings are device arrays or None for off."""
+        _call("shk_cuda_sample", self.h, logits, dtype, n_rows, n_vocab, row_stride, temperature, top_k, top_p, min_p,
+              u, out, prob, stream)
+
     # staging
     def layer_stage(self, slot, dst_dev, src_host_ptr, nbytes):
         _call("shk_cuda_layer_stage", self.h, slot, dst_dev, src_host_ptr, nbytes)
@@ -339,6 +386,36 @@ class KvCache:
 
     def seq_len(self, layer) -> int:
         return lib().shk_cuda_kv_seq_len(self.h, layer)
+
+
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 30
+PAGES_I8, PAGES_E4M3 = 0, 1
+
+
+def pages_attend_ws(n_rows: int, n_heads: int, n_kv_heads: int, head_dim: int) -> int:
+    """Workspace bytes of Pages.attend (0 if it does not take this shape)."""
+    return int(lib().shk_cuda_pages_attend_ws(n_rows, n_heads, n_kv_heads, head_dim))
+
+
+class Pages:
+    """One layer's paged 8-bit K/V pools in the caller's buffers (struct shk_pages)."""
+
+    def __init__(self, ctx: Context, k, v, k_scale, v_scale, type_, n_blocks, n_kv_heads, head_dim, block_tokens):
+        self.ctx = ctx
+        self.desc = PagesDesc(k, v, k_scale, v_scale, type_, n_blocks, n_kv_heads, head_dim, block_tokens)
+
+    def append(self, n_tokens, k, v, slots, dtype=DTYPE_F32, row_stride=0, stream=None):
+        _call("shk_cuda_pages_append", self.ctx.h, C.byref(self.desc), n_tokens, k, v, dtype, row_stride, slots, stream)
+
+    def read(self, n_tokens, slots, k, v, stream=None):
+        _call("shk_cuda_pages_read", self.ctx.h, C.byref(self.desc), n_tokens, slots, k, v, stream)
+
+    def attend(self, n_rows, q, out, n_heads, row_pos, table, table_stride, n_seq, scale, ws, ws_bytes, row_seq=None,
+               dtype=DTYPE_F32, q_stride=0, out_stride=0, stream=None):
+        """Rows of q over the positions 0 .. row_pos of their requests; ws_bytes >= pages_attend_ws(...)."""
+        r = PagesRows(n_rows, n_heads, dtype, q, out, q_stride, out_stride, row_seq, row_pos, table, n_seq,
+                      table_stride, scale, ws, ws_bytes)
+        _call("shk_cuda_pages_attend", self.ctx.h, C.byref(self.desc), C.byref(r), stream)
 
 
 class DeviceModel:
