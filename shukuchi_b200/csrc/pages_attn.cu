@@ -1,7 +1,31 @@
 // pages_attn.cu -- attention of a batch's rows over the paged 8-bit K/V pools.
+//
+// A row reads its request's keys and values once and does 4 hd flops per
+// position and query head with them: bound by memory.  So the work is laid out
+// by bytes.  An item is one row's positions for up to 8 query heads of one KV
+// head; items are cut into units of 64 positions, all units of all items are
+// put in one line, and each CTA takes an equal part of it, whatever the
+// lengths.  A CTA's part may begin and end inside an item: its (max, sum,
+// output) for that piece goes to the workspace and a second, small kernel joins
+// the pieces.  Lengths are read on the device only.
+//
+// Inside a unit each of the 4 warps takes 16 positions, which lie in one block
+// and so share one scale of K and one of V.  Every lane copies the bytes that
+// its own tensor-core fragments hold (cp.async, three slots deep), so nothing
+// in the loop waits for another thread.
+//
+//   S = q K^T by mma.m16n8k16 in f16: the bytes of both pool types are exact in
+//   f16, q is scaled by a power of two and split into two f16 parts (22 bits):
+//   head g's high part is row g of the A operand and its low part row g + 8, so
+//   both go through one instruction and their sums meet in one lane.
+//   O = P V the same way: the weights' high and low parts are rows g and g + 8.
+//
+// The softmax runs with two maxima per head: m of the scores for the sum, and M
+// of score + E, E the exponent of the block's V scale (V = 2^E f byte), for the
+// weights 2^(s - M + E) f of the output, so that neither overflows or
+// underflows however far the scales of blocks are apart.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -12,9 +36,36 @@
 namespace shk {
 namespace {
 
-__device__ __forceinline__ float value_of(uint8_t b, uint32_t type) {
-  return type == PAGES_I8 ? (float)(int8_t)b : __half2float(__half(__nv_cvt_fp8_to_halfraw(b, __NV_E4M3)));
-}
+constexpr int WARPS = 4;
+constexpr int THREADS = 32 * WARPS;
+constexpr int HEADS = 8;          // query heads of an item: the MMA's rows g
+constexpr int CHUNK = 16;         // positions of a warp's step
+constexpr int UNIT = CHUNK * WARPS;
+constexpr int SLOTS = 3;
+constexpr int CTAS_PER_SM = 4;    // 128 registers a thread
+constexpr int MAX_CTAS = 640;     // 4 x the SMs of a B200 (148), rounded up
+constexpr int MIN_UNITS = 2;      // a CTA's part: shorter ones cost more in joining than they save
+constexpr int MERGE_THREADS = 512;
+
+template <int HD>
+struct Lay {
+  static constexpr int NP = HD / 64;            // 16-byte pieces of a K row per lane
+  static constexpr int NW = HD / 32;            // words of a V row per lane
+  static constexpr int STEPS = HD / 16;         // k-steps of q K^T
+  static constexpr int SLOT = 2 * CHUNK * HD;   // bytes: K, then V
+  static constexpr int RING = SLOTS * SLOT;     // per warp
+  static constexpr int QF = STEPS * 32 * 16;    // q fragments
+  static constexpr int TROW = HD / 4 + 4;       // floats of a lane's output run, padded
+  static constexpr int HROW = 4 * TROW;
+  static constexpr int BYTES = WARPS * RING + QF;
+  static constexpr int REC = HEADS * (HD + 3);  // floats of a piece's record: O, m, M, l
+  static_assert(HEADS * HROW * 4 <= RING, "a warp's output fits its ring");
+};
+
+struct Header {  // the item that begins in a CTA's part and ends in a later one's
+  int32_t row, item, last, slot;
+};
+
 __device__ __forceinline__ float load_dt(const void* p, size_t i, uint32_t dt) {
   if (dt == DT_F32) return static_cast<const float*>(p)[i];
   if (dt == DT_F16) return __half2float(static_cast<const __half*>(p)[i]);
@@ -29,56 +80,500 @@ __device__ __forceinline__ void store_dt(void* p, size_t i, uint32_t dt, float v
     static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
-// One warp per (row, query head): online softmax over the row's positions,
-// hd / 32 dims per lane.
-template <int HD>
-__global__ void __launch_bounds__(256) attend_kernel(const __grid_constant__ PagesAttnArgs a) {
-  constexpr int E = HD / 32;
-  const uint32_t row = blockIdx.x, lane = threadIdx.x & 31;
-  const uint32_t bs = a.pool.block_shift, bt = 1u << bs;
-  const int32_t z = a.row_seq ? a.row_seq[row] : (int32_t)row;
-  if (z < 0) return;
-  int64_t len = (int64_t)a.row_pos[row] + 1;
-  if ((uint32_t)z >= a.n_seq || len > (int64_t)a.stride << bs) {
-    if (threadIdx.x == 0) set_error(a.err, DERR_BAD_POS);
-    len = 0;
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// src_bytes 0 fills with zeros and reads nothing
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t src_bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
+}
+__device__ __forceinline__ void copy8(uint32_t dst, const void* src, uint32_t src_bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+
+// The low and the high two bytes of a word as f16 pairs, exactly.
+template <uint32_t TYPE>
+__device__ __forceinline__ void to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (TYPE == PAGES_I8) {
+    // byte + 128 under the exponent of 1024, less 1152
+    const uint32_t x = w ^ 0x80808080u;
+    uint32_t a = __byte_perm(x, 0x64646464u, 0x4140), b = __byte_perm(x, 0x64646464u, 0x4342);
+    const __half2 c = __half2half2(__ushort_as_half(0x6480));
+    const __half2 ra = __hsub2(*reinterpret_cast<__half2*>(&a), c), rb = __hsub2(*reinterpret_cast<__half2*>(&b), c);
+    lo = *reinterpret_cast<const uint32_t*>(&ra);
+    hi = *reinterpret_cast<const uint32_t*>(&rb);
+  } else {
+    asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;\n}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
   }
-  for (uint32_t h = blockIdx.y * 8 + (threadIdx.x >> 5); h < a.n_heads; h += gridDim.y * 8) {
-    const uint32_t kvh = h % a.pool.n_kv;
-    float q[E], o[E] = {}, m = -INFINITY, l = 0.f;
-    for (int e = 0; e < E; ++e) q[e] = load_dt(a.q, row * a.q_stride + (size_t)h * HD + lane * E + e, a.dtype) * a.scale;
-    for (int64_t t = 0; t < len; ++t) {
-      const int32_t b = a.table[(size_t)z * a.stride + (t >> bs)];
-      if ((uint32_t)b >= a.pool.n_blocks) {
-        if (lane == 0) set_error(a.err, DERR_BAD_POS);
-        continue;
-      }
-      const size_t bh = (size_t)b * a.pool.n_kv + kvh, at = ((bh << bs) + (t & (bt - 1))) * HD + lane * E;
-      float s = 0.f;
-      for (int e = 0; e < E; ++e) s += q[e] * value_of(a.pool.k[at + e], a.pool.type);
-      s = warp_sum(s) * a.pool.ks[bh];
-      const float mn = fmaxf(m, s), c = m == mn ? 1.f : expf(m - mn), p = expf(s - mn);
-      m = mn;
-      l = l * c + p;
-      for (int e = 0; e < E; ++e) o[e] = o[e] * c + p * a.pool.vs[bh] * value_of(a.pool.v[at + e], a.pool.type);
+}
+
+// x = hi + lo in two f16 parts, for two values at once.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+struct Row {
+  int32_t z;
+  uint32_t len, units;
+};
+
+// A live row has at least one unit, so that a row which sees nothing is
+// written (zeros); a padding row has none.
+__device__ __forceinline__ Row row_of(const PagesAttnArgs& a, uint32_t r) {
+  Row w;
+  w.z = a.row_seq ? a.row_seq[r] : (int32_t)r;
+  const int32_t p = a.row_pos[r];
+  w.len = 0;
+  w.units = 0;
+  if (w.z < 0) return w;
+  if (p >= 0) {
+    if ((uint32_t)w.z >= a.n_seq || (uint64_t)p >= ((uint64_t)a.stride << a.pool.block_shift))
+      set_error(a.err, DERR_BAD_POS);
+    else
+      w.len = (uint32_t)p + 1;
+  } else if ((uint32_t)w.z >= a.n_seq) {
+    set_error(a.err, DERR_BAD_POS);
+  }
+  w.units = w.len ? (w.len + UNIT - 1) / UNIT : 1;
+  return w;
+}
+
+struct Sums {
+  uint64_t warp[WARPS];
+  uint64_t base;
+  uint32_t row;
+};
+
+template <int HD, uint32_t TYPE>
+struct Piece {
+  using L = Lay<HD>;
+
+  // This lane's bytes of one chunk (positions p0 .. p0 + 15 of block id; `rows`
+  // of them are the row's, the others become zeros).
+  static __device__ __forceinline__ void fetch(const PagesAttnArgs& a, uint32_t dst, int32_t id, uint32_t kvh, uint32_t p0,
+                                               uint32_t rows, uint32_t lane) {
+    const uint32_t g = lane >> 2, t = lane & 3, bs = a.pool.block_shift;
+    const size_t at = ((((size_t)id * a.pool.n_kv + kvh) << bs) + (p0 & ((1u << bs) - 1))) * HD;
+    const uint8_t* k = a.pool.k + at + g * HD + 16 * t;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < L::NP; ++i)
+        copy16(dst + ((j * L::NP + i) * 32 + lane) * 16, k + j * 8 * HD + 64 * i, 8 * j + g < rows ? 16 : 0);
+    const uint8_t* v = a.pool.v + at + 2 * t * HD + 4 * L::NW * g;
+    const uint32_t vd = dst + CHUNK * HD;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t row = (r & 1) + 8 * (r >> 1);
+      const uint32_t n = 2 * t + row < rows ? 4 * L::NW : 0;
+      if constexpr (HD == 128)
+        copy16(vd + (r * 32 + lane) * 16, v + row * HD, n);
+      else
+        copy8(vd + (r * 32 + lane) * 8, v + row * HD, n);
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    for (int e = 0; e < E; ++e)
-      store_dt(a.out, row * a.out_stride + (size_t)h * HD + lane * E + e, a.dtype, o[e] * inv);
   }
+};
+
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  return v;
+}
+
+template <int HD, uint32_t TYPE>
+__global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __grid_constant__ PagesAttnArgs a) {
+  using L = Lay<HD>;
+  extern __shared__ __align__(16) uint8_t att_smem[];
+  __shared__ Sums sums;
+  __shared__ int32_t qmax[HEADS];
+  __shared__ float stat[WARPS][HEADS][3];
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const uint32_t c = blockIdx.x, bs = a.pool.block_shift, n_kv = a.pool.n_kv, G = a.n_heads / n_kv;
+  const uint32_t nsub = (G + HEADS - 1) / HEADS, NI = n_kv * nsub;
+  Header* headers = static_cast<Header*>(a.ws);
+  float* records = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + MAX_CTAS * sizeof(Header));
+  pdl_trigger();
+  pdl_wait();
+
+  // ---- this CTA's part of the line of units ----
+  uint64_t mine = 0;
+  for (uint32_t r = tid; r < a.n_rows; r += THREADS) mine += row_of(a, r).units;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) sums.warp[warp] = mine;
+  __syncthreads();
+  const uint64_t U = NI * (sums.warp[0] + sums.warp[1] + sums.warp[2] + sums.warp[3]);
+  const uint64_t want = U / MIN_UNITS;
+  const uint32_t C = want < 1 ? 1 : want < gridDim.x ? (uint32_t)want : gridDim.x;
+  if (tid == 0) headers[c] = Header{-1, 0, 0, 0};
+  if (c >= C || U == 0) return;
+  uint64_t s = c * U / C;
+  const uint64_t first = s, end = (c + 1) * U / C;
+  uint64_t carry = 0;
+  for (uint32_t r0 = 0;; r0 += THREADS) {  // the row that unit s belongs to
+    __syncthreads();
+    const uint32_t n = r0 + tid < a.n_rows ? row_of(a, r0 + tid).units : 0;
+    uint64_t v = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= (uint32_t)o) v += u;
+    }
+    if (lane == 31) sums.warp[warp] = v;
+    __syncthreads();
+    uint64_t before = carry;
+    for (uint32_t w = 0; w < WARPS; ++w) {
+      if (w < warp) before += sums.warp[w];
+      carry += sums.warp[w];
+    }
+    const uint64_t lo = NI * (before + v - n);
+    if (n && s >= lo && s < NI * (before + v)) {
+      sums.row = r0 + tid;
+      sums.base = lo;
+    }
+    if (s < NI * carry || r0 + THREADS >= a.n_rows) break;
+  }
+  __syncthreads();
+  uint32_t row = sums.row;
+  uint64_t base = sums.base;
+  Row rw = row_of(a, row);
+
+  const uint32_t ring = smem_u32(att_smem) + warp * L::RING;
+  uint4* qf = reinterpret_cast<uint4*>(att_smem + WARPS * L::RING);
+
+  while (s < end) {
+    const uint32_t item = (uint32_t)((s - base) / rw.units);
+    const uint32_t ua = (uint32_t)(s - base - (uint64_t)item * rw.units);
+    const uint32_t ub = (uint32_t)min((uint64_t)rw.units, ua + (end - s));
+    const uint32_t kvh = item / nsub, sub = item % nsub;
+    const uint32_t n_heads = min(G - sub * HEADS, (uint32_t)HEADS);
+    const int32_t* table = a.table + (size_t)rw.z * a.stride;  // z is in range where len > 0
+
+    // ---- q: scaled by a power of two so that the largest magnitude of a head is in [2^14, 2^15) ----
+    if (tid < HEADS) qmax[tid] = 0;
+    __syncthreads();
+    float q[L::STEPS / WARPS][4];
+#pragma unroll
+    for (int i = 0; i < L::STEPS / WARPS; ++i) {
+      const uint32_t st = warp + WARPS * i;
+      // k-step st covers, for lane (g, t), the 4 dims of word st % 4 of its piece st / 4
+      const uint32_t d = 64 * (st >> 2) + 16 * t + 4 * (st & 3);
+      float m = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        q[i][e] = g < n_heads ? load_dt(a.q, row * a.q_stride + (size_t)((sub * HEADS + g) * n_kv + kvh) * HD + d + e, a.dtype)
+                              : 0.f;
+        m = fmaxf(m, fabsf(q[i][e]));
+      }
+      atomicMax(&qmax[g], __float_as_int(m));
+    }
+    __syncthreads();
+    const float top = __int_as_float(qmax[g]);
+    int ex = 0;
+    if (top > 0.f && top < INFINITY) ex = min(14 - ilogbf(top), 126);
+    const float up = ldexpf(1.f, ex);
+    const float qscale = a.scale * 1.4426950408889634f * ldexpf(1.f, -ex);
+#pragma unroll
+    for (int i = 0; i < L::STEPS / WARPS; ++i) {
+      uint4 f;
+      split2(q[i][0] * up, q[i][1] * up, f.x, f.y);
+      split2(q[i][2] * up, q[i][3] * up, f.z, f.w);
+      qf[(warp + WARPS * i) * 32 + lane] = f;
+    }
+    __syncthreads();
+
+    // ---- this warp's chunks: units ua .. ub - 1, positions 64 u + 16 warp ----
+    const uint32_t chunks = (rw.len + CHUNK - 1) / CHUNK;
+    const uint32_t last_u = chunks > warp ? (chunks - warp + WARPS - 1) / WARPS : 0;  // units with a chunk of this warp
+    const int32_t n = (int32_t)min(ub, last_u) - (int32_t)ua;
+    auto place = [&](int32_t i) { return (ua + (uint32_t)i) * UNIT + warp * CHUNK; };
+    auto block_id = [&](int32_t i) -> int32_t {
+      if (i >= n) return -1;
+      const int32_t id = table[place(i) >> bs];
+      if ((uint32_t)id < a.pool.n_blocks) return id;
+      set_error(a.err, DERR_BAD_POS);
+      return -1;
+    };
+    auto issue = [&](int32_t i, int32_t id, uint32_t slot) {
+      if (id >= 0) Piece<HD, TYPE>::fetch(a, ring + slot * L::SLOT, id, kvh, place(i), rw.len - place(i), lane);
+      copy_commit();
+    };
+    auto scales = [&](int32_t id) {
+      const size_t at = (size_t)(id < 0 ? 0 : id) * n_kv + kvh;
+      return make_float2(a.pool.ks[at], a.pool.vs[at]);
+    };
+    float m = -INFINITY, M = -INFINITY, l = 0.f;
+    float o[HD / 8][4];
+#pragma unroll
+    for (int j = 0; j < HD / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    if (n > 0) {
+      int32_t id0 = block_id(0), id1 = block_id(1), id2 = block_id(2), id3 = block_id(3);
+      issue(0, id0, 0);
+      issue(1, id1, 1);
+      float2 sc0 = scales(id0), sc1 = scales(id1);
+      uint32_t slot = 0;
+      for (int32_t i = 0; i < n; ++i) {
+        copy_wait<1>();
+        issue(i + 2, id2, slot == 0 ? 2 : slot - 1);
+        const float2 sc2 = scales(id2);
+        const int32_t id4 = block_id(i + 4);
+        const uint32_t kb = ring + slot * L::SLOT + lane * 16;
+        if (id0 >= 0) {
+          float acc[2][4] = {};
+#pragma unroll
+          for (int pi = 0; pi < L::NP; ++pi) {
+            const uint4 k0 = lds128(kb + pi * 512), k1 = lds128(kb + (L::NP + pi) * 512);
+            const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const uint4 qa = qf[(4 * pi + w) * 32 + lane];
+              uint32_t b0, b1;
+              to_f16<TYPE>(w0[w], b0, b1);
+              mma_f16(acc[0], qa, b0, b1);
+              to_f16<TYPE>(w1[w], b0, b1);
+              mma_f16(acc[1], qa, b0, b1);
+            }
+          }
+          // scores in powers of two; lane (g, t) holds head g at positions 2t, 2t + 1, 8 + 2t, 9 + 2t
+          const float f = sc0.x * qscale;
+          float sv[4] = {(acc[0][0] + acc[0][2]) * f, (acc[0][1] + acc[0][3]) * f, (acc[1][0] + acc[1][2]) * f,
+                         (acc[1][1] + acc[1][3]) * f};
+          const uint32_t left = rw.len - place(i);
+          if (left < CHUNK) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (2 * t + (e & 1) + 8 * (e >> 1) >= left) sv[e] = -INFINITY;
+          }
+          float cm = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
+          cm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, 1));
+          cm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, 2));
+          // the V scale as 2^E * vf, vf below 2 (also for a scale of 0, an infinite one or NaN)
+          const int e8 = max(1, min(254, (int)((__float_as_uint(sc0.y) >> 23) & 255)));
+          const float E = (float)(e8 - 127);
+          const float vf = e8 == 254 ? sc0.y * 0x1p-127f : sc0.y * __int_as_float((254 - e8) << 23);
+          const float mn = fmaxf(m, cm), Mn = fmaxf(M, cm + E);
+          if (__any_sync(0xffffffffu, mn > m || Mn > M)) {
+            const float al = m == mn ? 1.f : ex2(m - mn), aM = M == Mn ? 1.f : ex2(M - Mn);
+            l *= al;
+#pragma unroll
+            for (int j = 0; j < HD / 8; ++j) o[j][0] *= aM, o[j][1] *= aM, o[j][2] *= aM, o[j][3] *= aM;
+            m = mn;
+            M = Mn;
+          }
+          l += (ex2(sv[0] - m) + ex2(sv[1] - m)) + (ex2(sv[2] - m) + ex2(sv[3] - m));
+          const float vo = E + 14.f;  // weights up to 2^15: their low parts stay normal f16
+          float wt[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) wt[e] = ex2((sv[e] - M) + vo) * vf;
+          uint4 pa;
+          split2(wt[0], wt[1], pa.x, pa.y);
+          split2(wt[2], wt[3], pa.z, pa.w);
+          // lane (g, t): rows 2t, 2t + 1, 2t + 8, 2t + 9, dims NW * 4 * g ..; n-tile j is dim j of each run
+          uint32_t vr[4][L::NW];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if constexpr (HD == 128) {
+              const uint4 x = lds128(kb + CHUNK * HD + r * 512);
+              vr[r][0] = x.x, vr[r][1] = x.y, vr[r][2] = x.z, vr[r][3] = x.w;
+            } else {
+              const uint2 x = lds64(kb - lane * 8 + CHUNK * HD + r * 256);
+              vr[r][0] = x.x, vr[r][1] = x.y;
+            }
+          }
+#pragma unroll
+          for (int w = 0; w < L::NW; ++w) {
+            uint32_t b0[4], b1[4];
+            to_f16<TYPE>(__byte_perm(vr[0][w], vr[1][w], 0x5140), b0[0], b0[1]);
+            to_f16<TYPE>(__byte_perm(vr[0][w], vr[1][w], 0x7362), b0[2], b0[3]);
+            to_f16<TYPE>(__byte_perm(vr[2][w], vr[3][w], 0x5140), b1[0], b1[1]);
+            to_f16<TYPE>(__byte_perm(vr[2][w], vr[3][w], 0x7362), b1[2], b1[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mma_f16(o[4 * w + e], pa, b0[e], b1[e]);
+          }
+        }
+        slot = slot == 2 ? 0 : slot + 1;
+        id0 = id1, id1 = id2, id2 = id3, id3 = id4;
+        sc0 = sc1, sc1 = sc2;
+      }
+      copy_wait<0>();
+    }
+
+    // ---- the warps' outputs meet in shared memory (each in its own ring) ----
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    float* mo = reinterpret_cast<float*>(att_smem + warp * L::RING) + g * L::HROW + t * L::TROW;
+    // tile j, column 2t / 2t + 1 is dim j of run 2t / 2t + 1: the lane's outputs are HD / 4 dims in a row
+    __syncwarp();
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int j = 0; j < HD / 8; j += 4)
+        *reinterpret_cast<float4*>(mo + r * (HD / 8) + j) =
+            make_float4(o[j][r] + o[j][r + 2], o[j + 1][r] + o[j + 1][r + 2], o[j + 2][r] + o[j + 2][r + 2],
+                        o[j + 3][r] + o[j + 3][r + 2]);
+    if (t == 0) stat[warp][g][0] = m, stat[warp][g][1] = M, stat[warp][g][2] = l;
+    __syncthreads();
+    const bool whole = ua == 0 && ub == rw.units;
+    float* rec = records + (size_t)(2 * c + (s == first ? 0 : 1)) * L::REC;
+    {
+      constexpr int PER = HD * HEADS / THREADS;  // consecutive dims of one head per thread
+      const uint32_t h = tid / (HD / PER), d = (tid % (HD / PER)) * PER;
+      float mm = -INFINITY, MM = -INFINITY, ll = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, stat[w][h][0]), MM = fmaxf(MM, stat[w][h][1]);
+      float out[PER] = {};
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float lw = stat[w][h][2];
+        if (lw == 0.f) continue;  // a warp without positions
+        ll += lw * ex2(stat[w][h][0] - mm);
+        const float x = ex2(stat[w][h][1] - MM);
+        const float* src = reinterpret_cast<const float*>(att_smem + w * L::RING) + h * L::HROW + (d / (HD / 4)) * L::TROW + d % (HD / 4);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) out[e] += src[e] * x;
+      }
+      if (whole) {
+        if (h < n_heads) {
+          // MM - mm is at most the largest exponent of a scale
+          const float f = ll == 0.f ? 0.f : ex2(MM - mm - 14.f) / ll;
+          const size_t at = row * a.out_stride + (size_t)((sub * HEADS + h) * n_kv + kvh) * HD + d;
+#pragma unroll
+          for (int e = 0; e < PER; ++e) store_dt(a.out, at + e, a.dtype, ll == 0.f ? 0.f : out[e] * f);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < PER; e += 4)
+          *reinterpret_cast<float4*>(rec + h * HD + d + e) = make_float4(out[e], out[e + 1], out[e + 2], out[e + 3]);
+        if (d == 0) rec[HEADS * HD + h] = mm, rec[HEADS * (HD + 1) + h] = MM, rec[HEADS * (HD + 2) + h] = ll;
+        if (tid == 0 && ua == 0)
+          headers[c] = Header{(int32_t)row, (int32_t)item, (int32_t)(((s + rw.units) * C - 1) / U), s == first ? 0 : 1};
+      }
+    }
+    __syncthreads();  // the rings and stat are free again
+
+    s += ub - ua;
+    if (s < end && s == base + (uint64_t)NI * rw.units) {
+      base = s;
+      do rw = row_of(a, ++row);
+      while (rw.units == 0);
+    }
+  }
+}
+
+// Joins the pieces of the item that begins in CTA blockIdx.x's part: one head
+// per pair of warps, each warp every second piece.
+template <int HD>
+__global__ void __launch_bounds__(MERGE_THREADS) attend_join_kernel(const __grid_constant__ PagesAttnArgs a) {
+  using L = Lay<HD>;
+  constexpr int V = HD / 32;
+  __shared__ float half_o[HEADS][HD];
+  __shared__ float half_s[HEADS][3];
+  pdl_wait();
+  const uint32_t c = blockIdx.x;
+  const Header hd = static_cast<const Header*>(a.ws)[c];
+  if (hd.row < 0) return;
+  const float* records = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.ws) + MAX_CTAS * sizeof(Header));
+  const uint32_t n_kv = a.pool.n_kv, G = a.n_heads / n_kv, nsub = (G + HEADS - 1) / HEADS;
+  const uint32_t kvh = hd.item / nsub, sub = hd.item % nsub;
+  const uint32_t h = threadIdx.x >> 6, part = (threadIdx.x >> 5) & 1, lane = threadIdx.x & 31;
+  float m = -INFINITY, M = -INFINITY, l = 0.f, o[V] = {};
+#pragma unroll 4
+  for (uint32_t i = c + part; i <= (uint32_t)hd.last; i += 2) {
+    const float* rec = records + (size_t)(2 * i + (i == c ? hd.slot : 0)) * L::REC;
+    const float rm = rec[HEADS * HD + h], rM = rec[HEADS * (HD + 1) + h], rl = rec[HEADS * (HD + 2) + h];
+    float x[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[e] = rec[h * HD + lane * V + e];
+    if (rl == 0.f) continue;
+    const float mn = fmaxf(m, rm), Mn = fmaxf(M, rM);
+    const float am = m == mn ? 1.f : ex2(m - mn), aM = M == Mn ? 1.f : ex2(M - Mn);
+    const float bm = ex2(rm - mn), bM = ex2(rM - Mn);
+    l = l * am + rl * bm;
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[e] = o[e] * aM + x[e] * bM;
+    m = mn, M = Mn;
+  }
+  if (part) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) half_o[h][lane * V + e] = o[e];
+    if (lane == 0) half_s[h][0] = m, half_s[h][1] = M, half_s[h][2] = l;
+  }
+  __syncthreads();
+  if (part || sub * HEADS + h >= G) return;
+  const float m2 = half_s[h][0], M2 = half_s[h][1], l2 = half_s[h][2];
+  const float mm = fmaxf(m, m2), MM = fmaxf(M, M2);
+  const float ll = (l == 0.f ? 0.f : l * ex2(m - mm)) + (l2 == 0.f ? 0.f : l2 * ex2(m2 - mm));
+  const float f = ex2(MM - mm - 14.f) / ll;
+  const float f1 = l == 0.f ? 0.f : ex2(M - MM), f2 = l2 == 0.f ? 0.f : ex2(M2 - MM);
+  const size_t at = (uint32_t)hd.row * a.out_stride + (size_t)((sub * HEADS + h) * n_kv + kvh) * HD + lane * V;
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    store_dt(a.out, at + e, a.dtype, ll == 0.f ? 0.f : (o[e] * f1 + half_o[h][lane * V + e] * f2) * f);
+}
+
+template <int HD, uint32_t TYPE>
+cudaError_t attend_go(const PagesAttnArgs& a, int num_sms, cudaStream_t st) {
+  const uint32_t ctas = (uint32_t)min(num_sms * CTAS_PER_SM, MAX_CTAS);
+  cudaError_t e = launch_k(attend_kernel<HD, TYPE>, dim3(ctas), dim3(THREADS), Lay<HD>::BYTES, st, a);
+  if (e != cudaSuccess) return e;
+  // the join waits for the kernel above by itself (griddepcontrol.wait)
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(MERGE_THREADS);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attend_join_kernel<HD>, a);
 }
 
 }  // namespace
 
-size_t pages_attend_ws_bytes(uint32_t, uint32_t, uint32_t, uint32_t) { return 16; }
-cudaError_t pages_attend_init() { return cudaSuccess; }
-cudaError_t pages_attend_launch(const PagesAttnArgs& a, int, cudaStream_t st) {
-  const dim3 grid(a.n_rows, (a.n_heads + 7) / 8);
+size_t pages_attend_ws_bytes(uint32_t, uint32_t, uint32_t, uint32_t hd) {
+  return MAX_CTAS * (sizeof(Header) + 2 * 4 * (size_t)(hd == 64 ? Lay<64>::REC : Lay<128>::REC));
+}
+
+cudaError_t pages_attend_init() {
+  const auto big = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  cudaError_t e = cudaFuncSetAttribute(attend_kernel<64, PAGES_I8>, big, Lay<64>::BYTES);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(attend_kernel<64, PAGES_E4M3>, big, Lay<64>::BYTES);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(attend_kernel<128, PAGES_I8>, big, Lay<128>::BYTES);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(attend_kernel<128, PAGES_E4M3>, big, Lay<128>::BYTES);
+  return e;
+}
+
+cudaError_t pages_attend_launch(const PagesAttnArgs& a, int num_sms, cudaStream_t st) {
   if (a.pool.hd == 64)
-    attend_kernel<64><<<grid, 256, 0, st>>>(a);
-  else
-    attend_kernel<128><<<grid, 256, 0, st>>>(a);
-  return cudaGetLastError();
+    return a.pool.type == PAGES_I8 ? attend_go<64, PAGES_I8>(a, num_sms, st) : attend_go<64, PAGES_E4M3>(a, num_sms, st);
+  return a.pool.type == PAGES_I8 ? attend_go<128, PAGES_I8>(a, num_sms, st) : attend_go<128, PAGES_E4M3>(a, num_sms, st);
 }
 
 }  // namespace shk
