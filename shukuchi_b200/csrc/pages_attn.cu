@@ -3,16 +3,16 @@
 // A row reads its request's keys and values once and does 4 hd flops per
 // position and query head with them: bound by memory.  So the work is laid out
 // by bytes.  An item is one row's positions for up to 8 query heads of one KV
-// head; items are cut into units of 64 positions, all units of all items are
+// head; items are cut into units of 128 positions, all units of all items are
 // put in one line, and each CTA takes an equal part of it, whatever the
 // lengths.  A CTA's part may begin and end inside an item: its (max, sum,
 // output) for that piece goes to the workspace and a second, small kernel joins
 // the pieces.  Lengths are read on the device only.
 //
-// Inside a unit each of the 4 warps takes 16 positions, which lie in one block
-// and so share one scale of K and one of V.  Every lane copies the bytes that
-// its own tensor-core fragments hold (cp.async, three slots deep), so nothing
-// in the loop waits for another thread.
+// Inside a unit each of the 4 warps takes 32 positions: two times 16, which lie
+// in one block each and so share one scale of K and one of V.  Every lane copies
+// the bytes that its own tensor-core fragments hold (cp.async, the next step's
+// while this one is computed), so nothing in the loop waits for another thread.
 //
 //   S = q K^T by mma.m16n8k16 in f16: the bytes of both pool types are exact in
 //   f16, q is scaled by a power of two and split into two f16 parts (22 bits):
@@ -38,21 +38,24 @@ namespace {
 
 constexpr int WARPS = 4;
 constexpr int THREADS = 32 * WARPS;
-constexpr int HEADS = 8;          // query heads of an item: the MMA's rows g
-constexpr int CHUNK = 16;         // positions of a warp's step
-constexpr int UNIT = CHUNK * WARPS;
-constexpr int SLOTS = 3;
-constexpr int CTAS_PER_SM = 4;    // 128 registers a thread
-constexpr int MAX_CTAS = 640;     // 4 x the SMs of a B200 (148), rounded up
-constexpr int MIN_UNITS = 2;      // a CTA's part: shorter ones cost more in joining than they save
-constexpr int MERGE_THREADS = 512;
+constexpr int HEADS = 8;        // query heads of an item: the MMA's rows g
+constexpr int SUB = 16;         // positions under one pair of scales
+constexpr int STEP = 2 * SUB;   // positions of a warp's step
+constexpr int UNIT = STEP * WARPS;
+constexpr int SLOTS = 2;
+constexpr int CTAS_PER_SM = 3;  // 168 registers a thread
+constexpr int MAX_CTAS = 480;   // 3 x the SMs of a B200 (148), rounded up
+constexpr int ITEM_UNITS = 1;   // what an item costs besides its positions, in units
+constexpr int MIN_UNITS = 2;    // a CTA's part: shorter ones cost more in joining than they save
+constexpr int JOIN_THREADS = 512;
 
 template <int HD>
 struct Lay {
   static constexpr int NP = HD / 64;            // 16-byte pieces of a K row per lane
   static constexpr int NW = HD / 32;            // words of a V row per lane
   static constexpr int STEPS = HD / 16;         // k-steps of q K^T
-  static constexpr int SLOT = 2 * CHUNK * HD;   // bytes: K, then V
+  static constexpr int HALF = 2 * SUB * HD;     // bytes of 16 positions: K, then V
+  static constexpr int SLOT = 2 * HALF;
   static constexpr int RING = SLOTS * SLOT;     // per warp
   static constexpr int QF = STEPS * 32 * 16;    // q fragments
   static constexpr int TROW = HD / 4 + 4;       // floats of a lane's output run, padded
@@ -86,12 +89,20 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// src_bytes 0 fills with zeros and reads nothing
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t src_bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
+template <int BYTES>
+__device__ __forceinline__ void copy(uint32_t dst, const void* src) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void copy8(uint32_t dst, const void* src, uint32_t src_bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
+template <int BYTES>
+__device__ __forceinline__ void copy_or_zero(uint32_t dst, const void* src, bool take) {
+  const uint32_t n = take ? BYTES : 0;  // 0: reads nothing, writes zeros
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -162,38 +173,36 @@ __device__ __forceinline__ Row row_of(const PagesAttnArgs& a, uint32_t r) {
 struct Sums {
   uint64_t warp[WARPS];
   uint64_t base;
+  Row at;
   uint32_t row;
 };
 
+// This lane's bytes of 16 positions p0 .. p0 + 15 of block id.  Of the last
+// ones only `rows` are the row's: what lies behind them is masked, and e4m3
+// values become zeros here, as a NaN byte would outlive a weight of 0.
 template <int HD, uint32_t TYPE>
-struct Piece {
+__device__ __forceinline__ void fetch(const PagesAttnArgs& a, uint32_t dst, int32_t id, uint32_t kvh, uint32_t p0,
+                                      uint32_t rows, uint32_t lane) {
   using L = Lay<HD>;
-
-  // This lane's bytes of one chunk (positions p0 .. p0 + 15 of block id; `rows`
-  // of them are the row's, the others become zeros).
-  static __device__ __forceinline__ void fetch(const PagesAttnArgs& a, uint32_t dst, int32_t id, uint32_t kvh, uint32_t p0,
-                                               uint32_t rows, uint32_t lane) {
-    const uint32_t g = lane >> 2, t = lane & 3, bs = a.pool.block_shift;
-    const size_t at = ((((size_t)id * a.pool.n_kv + kvh) << bs) + (p0 & ((1u << bs) - 1))) * HD;
-    const uint8_t* k = a.pool.k + at + g * HD + 16 * t;
+  const uint32_t g = lane >> 2, t = lane & 3, bs = a.pool.block_shift;
+  const size_t at = ((((size_t)id * a.pool.n_kv + kvh) << bs) + (p0 & ((1u << bs) - 1))) * HD;
+  const uint8_t* k = a.pool.k + at + g * HD + 16 * t;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+  for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int i = 0; i < L::NP; ++i)
-        copy16(dst + ((j * L::NP + i) * 32 + lane) * 16, k + j * 8 * HD + 64 * i, 8 * j + g < rows ? 16 : 0);
-    const uint8_t* v = a.pool.v + at + 2 * t * HD + 4 * L::NW * g;
-    const uint32_t vd = dst + CHUNK * HD;
+    for (int i = 0; i < L::NP; ++i) copy<16>(dst + lane * 16 + (j * L::NP + i) * 512, k + j * 8 * HD + 64 * i);
+  constexpr int NB = 4 * L::NW;
+  const uint8_t* v = a.pool.v + at + 2 * t * HD + NB * g;
+  const uint32_t vd = dst + SUB * HD + lane * NB;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const uint32_t row = (r & 1) + 8 * (r >> 1);
-      const uint32_t n = 2 * t + row < rows ? 4 * L::NW : 0;
-      if constexpr (HD == 128)
-        copy16(vd + (r * 32 + lane) * 16, v + row * HD, n);
-      else
-        copy8(vd + (r * 32 + lane) * 8, v + row * HD, n);
-    }
+  for (int r = 0; r < 4; ++r) {
+    const int row = (r & 1) + 8 * (r >> 1);
+    if constexpr (TYPE == PAGES_I8)
+      copy<NB>(vd + r * 32 * NB, v + row * HD);
+    else
+      copy_or_zero<NB>(vd + r * 32 * NB, v + row * HD, 2 * t + row < rows);
   }
-};
+}
 
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
@@ -222,23 +231,10 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
   pdl_wait();
 
   // ---- this CTA's part of the line of units ----
-  uint64_t mine = 0;
-  for (uint32_t r = tid; r < a.n_rows; r += THREADS) mine += row_of(a, r).units;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) sums.warp[warp] = mine;
-  __syncthreads();
-  const uint64_t U = NI * (sums.warp[0] + sums.warp[1] + sums.warp[2] + sums.warp[3]);
-  const uint64_t want = U / MIN_UNITS;
-  const uint32_t C = want < 1 ? 1 : want < gridDim.x ? (uint32_t)want : gridDim.x;
   if (tid == 0) headers[c] = Header{-1, 0, 0, 0};
-  if (c >= C || U == 0) return;
-  uint64_t s = c * U / C;
-  const uint64_t first = s, end = (c + 1) * U / C;
-  uint64_t carry = 0;
-  for (uint32_t r0 = 0;; r0 += THREADS) {  // the row that unit s belongs to
-    __syncthreads();
-    const uint32_t n = r0 + tid < a.n_rows ? row_of(a, r0 + tid).units : 0;
+  // cost of this thread's row (the first THREADS rows), running sums over the warp and the CTA
+  auto cost = [](const Row& r) -> uint32_t { return r.units ? r.units + ITEM_UNITS : 0; };
+  auto scan = [&](uint32_t n, uint64_t& total) -> uint64_t {  // inclusive; one barrier before the next call
     uint64_t v = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -247,52 +243,130 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
     }
     if (lane == 31) sums.warp[warp] = v;
     __syncthreads();
-    uint64_t before = carry;
+    total = 0;
+#pragma unroll
     for (uint32_t w = 0; w < WARPS; ++w) {
-      if (w < warp) before += sums.warp[w];
-      carry += sums.warp[w];
+      if (w < warp) v += sums.warp[w];
+      total += sums.warp[w];
     }
-    const uint64_t lo = NI * (before + v - n);
-    if (n && s >= lo && s < NI * (before + v)) {
+    return v;
+  };
+  Row rw = tid < a.n_rows ? row_of(a, tid) : Row{-1, 0, 0};
+  uint64_t total;
+  uint64_t upto = scan(cost(rw), total);
+  uint64_t carry = total;
+  if (a.n_rows > THREADS) {
+    uint64_t more = 0;
+    for (uint32_t r = THREADS + tid; r < a.n_rows; r += THREADS) more += cost(row_of(a, r));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
+    __syncthreads();
+    if (lane == 0) sums.warp[warp] = more;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) total += sums.warp[w];
+  }
+  const uint64_t U = NI * total, want = U / MIN_UNITS;
+  const uint32_t C = want < 1 ? 1 : want < gridDim.x ? (uint32_t)want : gridDim.x;
+  if (c >= C || U == 0) return;
+  uint64_t s = c * U / C;
+  const uint64_t first = s, end = (c + 1) * U / C;
+  for (uint32_t r0 = 0;; r0 += THREADS) {  // the row that unit s belongs to
+    if (r0) {
+      __syncthreads();
+      rw = r0 + tid < a.n_rows ? row_of(a, r0 + tid) : Row{-1, 0, 0};
+      uint64_t n;
+      upto = carry + scan(cost(rw), n);
+      carry += n;
+    }
+    const uint64_t lo = NI * (upto - cost(rw));
+    if (rw.units && s >= lo && s < NI * upto) {
       sums.row = r0 + tid;
       sums.base = lo;
+      sums.at = rw;
     }
     if (s < NI * carry || r0 + THREADS >= a.n_rows) break;
   }
   __syncthreads();
   uint32_t row = sums.row;
   uint64_t base = sums.base;
-  Row rw = row_of(a, row);
+  rw = sums.at;
 
   const uint32_t ring = smem_u32(att_smem) + warp * L::RING;
   uint4* qf = reinterpret_cast<uint4*>(att_smem + WARPS * L::RING);
 
   while (s < end) {
-    const uint32_t item = (uint32_t)((s - base) / rw.units);
-    const uint32_t ua = (uint32_t)(s - base - (uint64_t)item * rw.units);
-    const uint32_t ub = (uint32_t)min((uint64_t)rw.units, ua + (end - s));
+    // the item, and this piece of it: units ua .. ub - 1 (its first ITEM_UNITS places in the line stand for its fixed cost)
+    const uint32_t span = rw.units + ITEM_UNITS;
+    const uint32_t item = (uint32_t)((s - base) / span);
+    const uint32_t va = (uint32_t)(s - base - (uint64_t)item * span);
+    const uint32_t vb = (uint32_t)min((uint64_t)span, va + (end - s));
+    const uint32_t ua = va > ITEM_UNITS ? va - ITEM_UNITS : 0, ub = vb > ITEM_UNITS ? vb - ITEM_UNITS : 0;
+    const uint64_t start = s;
+    s += vb - va;
+    const bool next_row = s < end && s == base + (uint64_t)NI * span;
+    if (ub > 0) {
     const uint32_t kvh = item / nsub, sub = item % nsub;
     const uint32_t n_heads = min(G - sub * HEADS, (uint32_t)HEADS);
     const int32_t* table = a.table + (size_t)rw.z * a.stride;  // z is in range where len > 0
 
-    // ---- q: scaled by a power of two so that the largest magnitude of a head is in [2^14, 2^15) ----
-    if (tid < HEADS) qmax[tid] = 0;
-    __syncthreads();
+    // q of this lane's fragments: k-step st covers, for lane (g, t), the 4 dims of word st % 4 of its piece st / 4
     float q[L::STEPS / WARPS][4];
 #pragma unroll
     for (int i = 0; i < L::STEPS / WARPS; ++i) {
-      const uint32_t st = warp + WARPS * i;
-      // k-step st covers, for lane (g, t), the 4 dims of word st % 4 of its piece st / 4
-      const uint32_t d = 64 * (st >> 2) + 16 * t + 4 * (st & 3);
-      float m = 0.f;
+      const uint32_t st = warp + WARPS * i, d = 64 * (st >> 2) + 16 * t + 4 * (st & 3);
+      const size_t at = row * a.q_stride + (size_t)((sub * HEADS + g) * n_kv + kvh) * HD + d;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        q[i][e] = g < n_heads ? load_dt(a.q, row * a.q_stride + (size_t)((sub * HEADS + g) * n_kv + kvh) * HD + d + e, a.dtype)
-                              : 0.f;
-        m = fmaxf(m, fabsf(q[i][e]));
-      }
-      atomicMax(&qmax[g], __float_as_int(m));
+      for (int e = 0; e < 4; ++e) q[i][e] = g < n_heads ? load_dt(a.q, at + e, a.dtype) : 0.f;
     }
+
+    // ---- this warp's steps: units ua .. ub - 1, positions UNIT u + STEP warp ----
+    const uint32_t steps = (rw.len + STEP - 1) / STEP;
+    const uint32_t last_u = steps > warp ? (steps - warp + WARPS - 1) / WARPS : 0;  // units with a step of this warp
+    const int32_t n = (int32_t)min(ub, last_u) - (int32_t)ua;
+    auto place = [&](int32_t i, int half) { return (ua + (uint32_t)i) * UNIT + warp * STEP + half * SUB; };
+    auto block_id = [&](int32_t i, int half) -> int32_t {
+      const uint32_t p = place(i, half);
+      if (i >= n || p >= rw.len) return -1;
+      const int32_t id = table[p >> bs];
+      if ((uint32_t)id < a.pool.n_blocks) return id;
+      set_error(a.err, DERR_BAD_POS);
+      return -1;
+    };
+    auto issue = [&](int32_t i, int2 id) {
+      const uint32_t dst = ring + (i & 1) * L::SLOT;
+      if (id.x >= 0) fetch<HD, TYPE>(a, dst, id.x, kvh, place(i, 0), rw.len - place(i, 0), lane);
+      if (id.y >= 0) fetch<HD, TYPE>(a, dst + L::HALF, id.y, kvh, place(i, 1), rw.len - place(i, 1), lane);
+      copy_commit();
+    };
+    auto scales = [&](int32_t id) {
+      const size_t at = (size_t)(id < 0 ? 0 : id) * n_kv + kvh;
+      return make_float2(a.pool.ks[at], a.pool.vs[at]);
+    };
+    float m = -INFINITY, M = -INFINITY, l = 0.f;
+    float o[HD / 8][4];
+#pragma unroll
+    for (int j = 0; j < HD / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    int2 id0{-1, -1}, id1{-1, -1};
+    float2 sx{}, sy{};
+    if (n > 0) {  // the first copies are on their way before q is needed
+      id0 = int2{block_id(0, 0), block_id(0, 1)};
+      id1 = int2{block_id(1, 0), block_id(1, 1)};
+      issue(0, id0);
+      sx = scales(id0.x), sy = scales(id0.y);
+    }
+
+    // q scaled by a power of two so that the largest magnitude of a head is in [2^14, 2^15)
+    if (tid < HEADS) qmax[tid] = 0;
+    __syncthreads();
+    float big = 0.f;
+#pragma unroll
+    for (int i = 0; i < L::STEPS / WARPS; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(q[i][e]));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    if (t == 0) atomicMax(&qmax[g], __float_as_int(big));
     __syncthreads();
     const float top = __int_as_float(qmax[g]);
     int ex = 0;
@@ -308,101 +382,103 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
     }
     __syncthreads();
 
-    // ---- this warp's chunks: units ua .. ub - 1, positions 64 u + 16 warp ----
-    const uint32_t chunks = (rw.len + CHUNK - 1) / CHUNK;
-    const uint32_t last_u = chunks > warp ? (chunks - warp + WARPS - 1) / WARPS : 0;  // units with a chunk of this warp
-    const int32_t n = (int32_t)min(ub, last_u) - (int32_t)ua;
-    auto place = [&](int32_t i) { return (ua + (uint32_t)i) * UNIT + warp * CHUNK; };
-    auto block_id = [&](int32_t i) -> int32_t {
-      if (i >= n) return -1;
-      const int32_t id = table[place(i) >> bs];
-      if ((uint32_t)id < a.pool.n_blocks) return id;
-      set_error(a.err, DERR_BAD_POS);
-      return -1;
-    };
-    auto issue = [&](int32_t i, int32_t id, uint32_t slot) {
-      if (id >= 0) Piece<HD, TYPE>::fetch(a, ring + slot * L::SLOT, id, kvh, place(i), rw.len - place(i), lane);
-      copy_commit();
-    };
-    auto scales = [&](int32_t id) {
-      const size_t at = (size_t)(id < 0 ? 0 : id) * n_kv + kvh;
-      return make_float2(a.pool.ks[at], a.pool.vs[at]);
-    };
-    float m = -INFINITY, M = -INFINITY, l = 0.f;
-    float o[HD / 8][4];
+    for (int32_t i = 0; i < n; ++i) {
+      issue(i + 1, id1);
+      const float2 nx = scales(id1.x), ny = scales(id1.y);
+      const int2 id2{block_id(i + 2, 0), block_id(i + 2, 1)};
+      copy_wait<1>();
+      const uint32_t kb = ring + (i & 1) * L::SLOT + lane * 16;
+      float acc[4][4] = {};
 #pragma unroll
-    for (int j = 0; j < HD / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    if (n > 0) {
-      int32_t id0 = block_id(0), id1 = block_id(1), id2 = block_id(2), id3 = block_id(3);
-      issue(0, id0, 0);
-      issue(1, id1, 1);
-      float2 sc0 = scales(id0), sc1 = scales(id1);
-      uint32_t slot = 0;
-      for (int32_t i = 0; i < n; ++i) {
-        copy_wait<1>();
-        issue(i + 2, id2, slot == 0 ? 2 : slot - 1);
-        const float2 sc2 = scales(id2);
-        const int32_t id4 = block_id(i + 4);
-        const uint32_t kb = ring + slot * L::SLOT + lane * 16;
-        if (id0 >= 0) {
-          float acc[2][4] = {};
+      for (int pi = 0; pi < L::NP; ++pi) {
+        uint32_t kw[4][4];
 #pragma unroll
-          for (int pi = 0; pi < L::NP; ++pi) {
-            const uint4 k0 = lds128(kb + pi * 512), k1 = lds128(kb + (L::NP + pi) * 512);
-            const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+        for (int j = 0; j < 4; ++j) {
+          const uint4 x = lds128(kb + (j >> 1) * L::HALF + ((j & 1) * L::NP + pi) * 512);
+          kw[j][0] = x.x, kw[j][1] = x.y, kw[j][2] = x.z, kw[j][3] = x.w;
+        }
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const uint4 qa = qf[(4 * pi + w) * 32 + lane];
-              uint32_t b0, b1;
-              to_f16<TYPE>(w0[w], b0, b1);
-              mma_f16(acc[0], qa, b0, b1);
-              to_f16<TYPE>(w1[w], b0, b1);
-              mma_f16(acc[1], qa, b0, b1);
-            }
+        for (int w = 0; w < 4; ++w) {
+          const uint4 qa = qf[(4 * pi + w) * 32 + lane];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t b0, b1;
+            to_f16<TYPE>(kw[j][w], b0, b1);
+            mma_f16(acc[j], qa, b0, b1);
           }
-          // scores in powers of two; lane (g, t) holds head g at positions 2t, 2t + 1, 8 + 2t, 9 + 2t
-          const float f = sc0.x * qscale;
-          float sv[4] = {(acc[0][0] + acc[0][2]) * f, (acc[0][1] + acc[0][3]) * f, (acc[1][0] + acc[1][2]) * f,
-                         (acc[1][1] + acc[1][3]) * f};
-          const uint32_t left = rw.len - place(i);
-          if (left < CHUNK) {
+        }
+      }
+      // scores in powers of two; lane (g, t) holds head g at positions 8 j + 2t, 8 j + 2t + 1
+      float sv[4][2];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (2 * t + (e & 1) + 8 * (e >> 1) >= left) sv[e] = -INFINITY;
-          }
-          float cm = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
-          cm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, 1));
-          cm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, 2));
-          // the V scale as 2^E * vf, vf below 2 (also for a scale of 0, an infinite one or NaN)
-          const int e8 = max(1, min(254, (int)((__float_as_uint(sc0.y) >> 23) & 255)));
-          const float E = (float)(e8 - 127);
-          const float vf = e8 == 254 ? sc0.y * 0x1p-127f : sc0.y * __int_as_float((254 - e8) << 23);
-          const float mn = fmaxf(m, cm), Mn = fmaxf(M, cm + E);
-          if (__any_sync(0xffffffffu, mn > m || Mn > M)) {
-            const float al = m == mn ? 1.f : ex2(m - mn), aM = M == Mn ? 1.f : ex2(M - Mn);
-            l *= al;
+      for (int j = 0; j < 4; ++j) {
+        const float f = (j < 2 ? sx.x : sy.x) * qscale;
+        sv[j][0] = (acc[j][0] + acc[j][2]) * f;
+        sv[j][1] = (acc[j][1] + acc[j][3]) * f;
+      }
+      const int32_t left = (int32_t)(rw.len - place(i, 0));
+      if (left < STEP || id0.x < 0 || id0.y < 0) {
 #pragma unroll
-            for (int j = 0; j < HD / 8; ++j) o[j][0] *= aM, o[j][1] *= aM, o[j][2] *= aM, o[j][3] *= aM;
-            m = mn;
-            M = Mn;
-          }
-          l += (ex2(sv[0] - m) + ex2(sv[1] - m)) + (ex2(sv[2] - m) + ex2(sv[3] - m));
-          const float vo = E + 14.f;  // weights up to 2^15: their low parts stay normal f16
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if ((int32_t)(8 * j + 2 * t + e) >= left || (j < 2 ? id0.x : id0.y) < 0) sv[j][e] = -INFINITY;
+      }
+      // a V scale is 2^E * vf, vf below 2 (also for a scale of 0, an infinite one or NaN)
+      float E[2], vf[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float vs = h ? sy.y : sx.y;
+        const int e8 = max(1, min(254, (int)((__float_as_uint(vs) >> 23) & 255)));
+        E[h] = (float)(e8 - 127);
+        vf[h] = e8 == 254 ? vs * 0x1p-127f : vs * __int_as_float((254 - e8) << 23);
+      }
+      const float c0 = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
+      const float c1 = fmaxf(fmaxf(sv[2][0], sv[2][1]), fmaxf(sv[3][0], sv[3][1]));
+      float mn = fmaxf(c0, c1), Mn = fmaxf(c0 + E[0], c1 + E[1]);
+#pragma unroll
+      for (int x = 1; x <= 2; x <<= 1) {
+        mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, x));
+        Mn = fmaxf(Mn, __shfl_xor_sync(0xffffffffu, Mn, x));
+      }
+      mn = fmaxf(m, mn), Mn = fmaxf(M, Mn);
+      if (__any_sync(0xffffffffu, mn > m || Mn > M)) {
+        const float al = m == mn ? 1.f : ex2(m - mn), aM = M == Mn ? 1.f : ex2(M - Mn);
+        l *= al;
+#pragma unroll
+        for (int j = 0; j < HD / 8; ++j) o[j][0] *= aM, o[j][1] *= aM, o[j][2] *= aM, o[j][3] *= aM;
+        m = mn;
+        M = Mn;
+      }
+      // a step without positions (its blocks are bad) leaves both maxima at -inf
+      if (id0.x >= 0 || id0.y >= 0) {
+        uint4 pa[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
           float wt[4];
+          const float vo = E[h] + 14.f;  // weights up to 2^15: their low parts stay normal f16
 #pragma unroll
-          for (int e = 0; e < 4; ++e) wt[e] = ex2((sv[e] - M) + vo) * vf;
-          uint4 pa;
-          split2(wt[0], wt[1], pa.x, pa.y);
-          split2(wt[2], wt[3], pa.z, pa.w);
-          // lane (g, t): rows 2t, 2t + 1, 2t + 8, 2t + 9, dims NW * 4 * g ..; n-tile j is dim j of each run
+          for (int e = 0; e < 4; ++e) {
+            const float x = sv[2 * h + (e >> 1)][e & 1];
+            l += ex2(x - m);
+            wt[e] = ex2((x - M) + vo) * vf[h];
+          }
+          split2(wt[0], wt[1], pa[h].x, pa[h].y);
+          split2(wt[2], wt[3], pa[h].z, pa[h].w);
+        }
+        // lane (g, t): rows 2t, 2t + 1, 2t + 8, 2t + 9, dims 4 NW g ..; n-tile j is dim j of each run
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if ((h ? id0.y : id0.x) < 0) continue;
           uint32_t vr[4][L::NW];
+          const uint32_t vb = ring + (i & 1) * L::SLOT + h * L::HALF + SUB * HD + lane * 4 * L::NW;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             if constexpr (HD == 128) {
-              const uint4 x = lds128(kb + CHUNK * HD + r * 512);
+              const uint4 x = lds128(vb + r * 512);
               vr[r][0] = x.x, vr[r][1] = x.y, vr[r][2] = x.z, vr[r][3] = x.w;
             } else {
-              const uint2 x = lds64(kb - lane * 8 + CHUNK * HD + r * 256);
+              const uint2 x = lds64(vb + r * 256);
               vr[r][0] = x.x, vr[r][1] = x.y;
             }
           }
@@ -414,15 +490,14 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
             to_f16<TYPE>(__byte_perm(vr[2][w], vr[3][w], 0x5140), b1[0], b1[1]);
             to_f16<TYPE>(__byte_perm(vr[2][w], vr[3][w], 0x7362), b1[2], b1[3]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mma_f16(o[4 * w + e], pa, b0[e], b1[e]);
+            for (int e = 0; e < 4; ++e) mma_f16(o[4 * w + e], pa[h], b0[e], b1[e]);
           }
         }
-        slot = slot == 2 ? 0 : slot + 1;
-        id0 = id1, id1 = id2, id2 = id3, id3 = id4;
-        sc0 = sc1, sc1 = sc2;
       }
-      copy_wait<0>();
+      id0 = id1, id1 = id2;
+      sx = nx, sy = ny;
     }
+    copy_wait<0>();
 
     // ---- the warps' outputs meet in shared memory (each in its own ring) ----
     l += __shfl_xor_sync(0xffffffffu, l, 1);
@@ -440,7 +515,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
     if (t == 0) stat[warp][g][0] = m, stat[warp][g][1] = M, stat[warp][g][2] = l;
     __syncthreads();
     const bool whole = ua == 0 && ub == rw.units;
-    float* rec = records + (size_t)(2 * c + (s == first ? 0 : 1)) * L::REC;
+    float* rec = records + (size_t)(2 * c + (start == first ? 0 : 1)) * L::REC;
     {
       constexpr int PER = HD * HEADS / THREADS;  // consecutive dims of one head per thread
       const uint32_t h = tid / (HD / PER), d = (tid % (HD / PER)) * PER;
@@ -472,13 +547,13 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
           *reinterpret_cast<float4*>(rec + h * HD + d + e) = make_float4(out[e], out[e + 1], out[e + 2], out[e + 3]);
         if (d == 0) rec[HEADS * HD + h] = mm, rec[HEADS * (HD + 1) + h] = MM, rec[HEADS * (HD + 2) + h] = ll;
         if (tid == 0 && ua == 0)
-          headers[c] = Header{(int32_t)row, (int32_t)item, (int32_t)(((s + rw.units) * C - 1) / U), s == first ? 0 : 1};
+          headers[c] = Header{(int32_t)row, (int32_t)item, (int32_t)(((base + (uint64_t)(item + 1) * span) * C - 1) / U),
+                              start == first ? 0 : 1};
       }
     }
     __syncthreads();  // the rings and stat are free again
-
-    s += ub - ua;
-    if (s < end && s == base + (uint64_t)NI * rw.units) {
+    }
+    if (next_row) {
       base = s;
       do rw = row_of(a, ++row);
       while (rw.units == 0);
@@ -486,55 +561,68 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
   }
 }
 
-// Joins the pieces of the item that begins in CTA blockIdx.x's part: one head
-// per pair of warps, each warp every second piece.
+// Joins the pieces of the item that begins in CTA blockIdx.x's part: first
+// every piece's (max, sum) at once, then the outputs, 4 dims per thread and
+// the pieces dealt to the thread groups.
 template <int HD>
-__global__ void __launch_bounds__(MERGE_THREADS) attend_join_kernel(const __grid_constant__ PagesAttnArgs a) {
+__global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const __grid_constant__ PagesAttnArgs a) {
   using L = Lay<HD>;
-  constexpr int V = HD / 32;
-  __shared__ float half_o[HEADS][HD];
-  __shared__ float half_s[HEADS][3];
+  constexpr int PER_GROUP = HEADS * HD / 4, GROUPS = JOIN_THREADS / PER_GROUP;
+  __shared__ __align__(16) float st[3][HEADS][MAX_CTAS + 1];
+  __shared__ float fin[HEADS];
+  float4* sum = reinterpret_cast<float4*>(st[0]);  // the maxima are done with by then
+  static_assert(sizeof(st[0]) >= JOIN_THREADS * sizeof(float4), "outputs fit where the maxima were");
+  const uint32_t c = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
   pdl_wait();
-  const uint32_t c = blockIdx.x;
   const Header hd = static_cast<const Header*>(a.ws)[c];
   if (hd.row < 0) return;
   const float* records = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.ws) + MAX_CTAS * sizeof(Header));
   const uint32_t n_kv = a.pool.n_kv, G = a.n_heads / n_kv, nsub = (G + HEADS - 1) / HEADS;
-  const uint32_t kvh = hd.item / nsub, sub = hd.item % nsub;
-  const uint32_t h = threadIdx.x >> 6, part = (threadIdx.x >> 5) & 1, lane = threadIdx.x & 31;
-  float m = -INFINITY, M = -INFINITY, l = 0.f, o[V] = {};
-#pragma unroll 4
-  for (uint32_t i = c + part; i <= (uint32_t)hd.last; i += 2) {
-    const float* rec = records + (size_t)(2 * i + (i == c ? hd.slot : 0)) * L::REC;
-    const float rm = rec[HEADS * HD + h], rM = rec[HEADS * (HD + 1) + h], rl = rec[HEADS * (HD + 2) + h];
-    float x[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) x[e] = rec[h * HD + lane * V + e];
-    if (rl == 0.f) continue;
-    const float mn = fmaxf(m, rm), Mn = fmaxf(M, rM);
-    const float am = m == mn ? 1.f : ex2(m - mn), aM = M == Mn ? 1.f : ex2(M - Mn);
-    const float bm = ex2(rm - mn), bM = ex2(rM - Mn);
-    l = l * am + rl * bm;
-#pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = o[e] * aM + x[e] * bM;
-    m = mn, M = Mn;
-  }
-  if (part) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) half_o[h][lane * V + e] = o[e];
-    if (lane == 0) half_s[h][0] = m, half_s[h][1] = M, half_s[h][2] = l;
+  const uint32_t kvh = hd.item / nsub, sub = hd.item % nsub, n = (uint32_t)hd.last - c + 1;
+  auto rec = [&](uint32_t i) { return records + (size_t)(2 * (c + i) + (i == 0 ? hd.slot : 0)) * L::REC; };
+  for (uint32_t i = tid; i < n * 3 * HEADS; i += JOIN_THREADS) {
+    const uint32_t p = i / (3 * HEADS), k = i % (3 * HEADS);
+    st[k / HEADS][k % HEADS][p] = rec(p)[HEADS * HD + k];
   }
   __syncthreads();
-  if (part || sub * HEADS + h >= G) return;
-  const float m2 = half_s[h][0], M2 = half_s[h][1], l2 = half_s[h][2];
-  const float mm = fmaxf(m, m2), MM = fmaxf(M, M2);
-  const float ll = (l == 0.f ? 0.f : l * ex2(m - mm)) + (l2 == 0.f ? 0.f : l2 * ex2(m2 - mm));
-  const float f = ex2(MM - mm - 14.f) / ll;
-  const float f1 = l == 0.f ? 0.f : ex2(M - MM), f2 = l2 == 0.f ? 0.f : ex2(M2 - MM);
-  const size_t at = (uint32_t)hd.row * a.out_stride + (size_t)((sub * HEADS + h) * n_kv + kvh) * HD + lane * V;
+  if (tid < 32 * HEADS) {
+    const uint32_t h = tid >> 5;
+    float m = -INFINITY, M = -INFINITY, l = 0.f;
+    for (uint32_t i = lane; i < n; i += 32) m = fmaxf(m, st[0][h][i]), M = fmaxf(M, st[1][h][i]);
+    m = warp_max(m);
+    M = warp_max(M);
+    for (uint32_t i = lane; i < n; i += 32) {
+      const float x = st[2][h][i];
+      const bool some = x != 0.f;  // else a piece without positions
+      l += some ? x * ex2(st[0][h][i] - m) : 0.f;
+      st[1][h][i] = some ? ex2(st[1][h][i] - M) : 0.f;
+    }
+    l = warp_sum(l);
+    if (lane == 0) fin[h] = l == 0.f ? 0.f : ex2(M - m - 14.f) / l;
+  }
+  __syncthreads();
+  const uint32_t grp = tid / PER_GROUP, e = tid % PER_GROUP, h = e / (HD / 4);
+  float4 o{};
+#pragma unroll 8
+  for (uint32_t i = grp; i < n; i += GROUPS) {
+    const float4 x = reinterpret_cast<const float4*>(rec(i))[e];
+    const float f = st[1][h][i];
+    o.x += x.x * f, o.y += x.y * f, o.z += x.z * f, o.w += x.w * f;
+  }
+  sum[tid] = o;
+  __syncthreads();
+  if (grp || sub * HEADS + h >= G) return;
 #pragma unroll
-  for (int e = 0; e < V; ++e)
-    store_dt(a.out, at + e, a.dtype, ll == 0.f ? 0.f : (o[e] * f1 + half_o[h][lane * V + e] * f2) * f);
+  for (int k = 1; k < GROUPS; ++k) {
+    const float4 x = sum[k * PER_GROUP + e];
+    o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+  }
+  const float f = fin[h];
+  const size_t at = (uint32_t)hd.row * a.out_stride + (size_t)((sub * HEADS + h) * n_kv + kvh) * HD + 4 * (e % (HD / 4));
+  store_dt(a.out, at, a.dtype, o.x * f);
+  store_dt(a.out, at + 1, a.dtype, o.y * f);
+  store_dt(a.out, at + 2, a.dtype, o.z * f);
+  store_dt(a.out, at + 3, a.dtype, o.w * f);
 }
 
 template <int HD, uint32_t TYPE>
@@ -545,7 +633,7 @@ cudaError_t attend_go(const PagesAttnArgs& a, int num_sms, cudaStream_t st) {
   // the join waits for the kernel above by itself (griddepcontrol.wait)
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(MERGE_THREADS);
+  cfg.blockDim = dim3(JOIN_THREADS);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
