@@ -111,8 +111,7 @@ __device__ __forceinline__ void copy_wait() {
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
@@ -177,42 +176,36 @@ struct Sums {
   uint32_t row;
 };
 
-// This lane's bytes of 16 positions p0 .. p0 + 15 of block id.  Of the last
-// ones only `rows` are the row's: what lies behind them is masked, and e4m3
-// values become zeros here, as a NaN byte would outlive a weight of 0.
-template <int HD, uint32_t TYPE>
-__device__ __forceinline__ void fetch(const PagesAttnArgs& a, uint32_t dst, int32_t id, uint32_t kvh, uint32_t p0,
-                                      uint32_t rows, uint32_t lane) {
-  using L = Lay<HD>;
-  const uint32_t g = lane >> 2, t = lane & 3, bs = a.pool.block_shift;
-  const size_t at = ((((size_t)id * a.pool.n_kv + kvh) << bs) + (p0 & ((1u << bs) - 1))) * HD;
-  const uint8_t* k = a.pool.k + at + g * HD + 16 * t;
+// This lane's bytes of 16 positions p0 .. p0 + 15 of block id: of K the 16 bytes
+// at 16 t (and 64 + 16 t) of rows g and g + 8, of V the HD / 8 bytes at HD / 8 g
+// of rows 2t, 2t + 1, 2t + 8, 2t + 9.
+__device__ __forceinline__ size_t first_row(const PagesAttnArgs& a, int32_t id, uint32_t kvh, uint32_t p0) {
+  const uint32_t bs = a.pool.block_shift;
+  return (((size_t)id * a.pool.n_kv + kvh) << bs) + (p0 & ((1u << bs) - 1));
+}
+template <int HD>
+__device__ __forceinline__ void fetch_k(const uint8_t* row0, uint32_t dst, uint32_t lane) {
+  const uint8_t* k = row0 + (lane >> 2) * HD + 16 * (lane & 3);
 #pragma unroll
   for (int j = 0; j < 2; ++j)
 #pragma unroll
-    for (int i = 0; i < L::NP; ++i) copy<16>(dst + lane * 16 + (j * L::NP + i) * 512, k + j * 8 * HD + 64 * i);
-  constexpr int NB = 4 * L::NW;
-  const uint8_t* v = a.pool.v + at + 2 * t * HD + NB * g;
-  const uint32_t vd = dst + SUB * HD + lane * NB;
+    for (int i = 0; i < Lay<HD>::NP; ++i) copy<16>(dst + lane * 16 + (j * Lay<HD>::NP + i) * 512, k + j * 8 * HD + 64 * i);
+}
+// Only `rows` of the positions are the row's.  What lies behind them gets
+// weight 0; e4m3 values become zeros here too, as a NaN byte would outlive that.
+template <int HD, uint32_t TYPE>
+__device__ __forceinline__ void fetch_v(const uint8_t* row0, uint32_t dst, uint32_t rows, uint32_t lane) {
+  constexpr int NB = HD / 8;
+  const uint32_t t = lane & 3;
+  const uint8_t* v = row0 + 2 * t * HD + NB * (lane >> 2);
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int row = (r & 1) + 8 * (r >> 1);
     if constexpr (TYPE == PAGES_I8)
-      copy<NB>(vd + r * 32 * NB, v + row * HD);
+      copy<NB>(dst + (r * 32 + lane) * NB, v + row * HD);
     else
-      copy_or_zero<NB>(vd + r * 32 * NB, v + row * HD, 2 * t + row < rows);
+      copy_or_zero<NB>(dst + (r * 32 + lane) * NB, v + row * HD, 2 * t + row < rows);
   }
-}
-
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
-  return v;
 }
 
 template <int HD, uint32_t TYPE>
@@ -325,18 +318,37 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
     const uint32_t last_u = steps > warp ? (steps - warp + WARPS - 1) / WARPS : 0;  // units with a step of this warp
     const int32_t n = (int32_t)min(ub, last_u) - (int32_t)ua;
     auto place = [&](int32_t i, int half) { return (ua + (uint32_t)i) * UNIT + warp * STEP + half * SUB; };
-    auto block_id = [&](int32_t i, int half) -> int32_t {
+    // a table entry is checked a step after it is read, when it has arrived
+    auto entry = [&](int32_t i, int half) -> int32_t {
       const uint32_t p = place(i, half);
-      if (i >= n || p >= rw.len) return -1;
-      const int32_t id = table[p >> bs];
-      if ((uint32_t)id < a.pool.n_blocks) return id;
-      set_error(a.err, DERR_BAD_POS);
-      return -1;
+      return i < n && p < rw.len ? table[p >> bs] : -1;
     };
-    auto issue = [&](int32_t i, int2 id) {
+    auto checked = [&](int32_t i, int2 id) {
+      if ((uint32_t)id.x >= a.pool.n_blocks || (uint32_t)id.y >= a.pool.n_blocks) {
+        if (i < n && ((uint32_t)id.x >= a.pool.n_blocks || place(i, 1) < rw.len)) set_error(a.err, DERR_BAD_POS);
+        if ((uint32_t)id.x >= a.pool.n_blocks) id.x = -1;
+        if ((uint32_t)id.y >= a.pool.n_blocks) id.y = -1;
+      }
+      return id;
+    };
+    auto issue_k = [&](int32_t i, int2 id) {
       const uint32_t dst = ring + (i & 1) * L::SLOT;
-      if (id.x >= 0) fetch<HD, TYPE>(a, dst, id.x, kvh, place(i, 0), rw.len - place(i, 0), lane);
-      if (id.y >= 0) fetch<HD, TYPE>(a, dst + L::HALF, id.y, kvh, place(i, 1), rw.len - place(i, 1), lane);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if ((h ? id.y : id.x) >= 0)
+          fetch_k<HD>(a.pool.k + first_row(a, h ? id.y : id.x, kvh, place(i, h)) * HD, dst + h * L::HALF, lane);
+      copy_commit();
+    };
+    auto issue_v = [&](int32_t i, int2 id) {
+      const uint32_t dst = ring + (i & 1) * L::SLOT + SUB * HD;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if ((h ? id.y : id.x) >= 0)
+          fetch_v<HD, TYPE>(a.pool.v + first_row(a, h ? id.y : id.x, kvh, place(i, h)) * HD, dst + h * L::HALF,
+                            rw.len - place(i, h), lane);
+        else if (TYPE == PAGES_E4M3 && i < n)
+          fetch_v<HD, TYPE>(a.pool.v, dst + h * L::HALF, 0, lane);
+      }
       copy_commit();
     };
     auto scales = [&](int32_t id) {
@@ -347,12 +359,18 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
     float o[HD / 8][4];
 #pragma unroll
     for (int j = 0; j < HD / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    int2 id0{-1, -1}, id1{-1, -1};
+    int2 id0{-1, -1}, id1{-1, -1}, id2{-1, -1};
     float2 sx{}, sy{};
     if (n > 0) {  // the first copies are on their way before q is needed
-      id0 = int2{block_id(0, 0), block_id(0, 1)};
-      id1 = int2{block_id(1, 0), block_id(1, 1)};
-      issue(0, id0);
+      id0 = int2{entry(0, 0), entry(0, 1)};
+      id1 = int2{entry(1, 0), entry(1, 1)};
+      id2 = int2{entry(2, 0), entry(2, 1)};
+      id0 = checked(0, id0);
+      issue_k(0, id0);
+      issue_v(0, id0);
+      id1 = checked(1, id1);
+      issue_k(1, id1);
+      issue_v(1, id1);
       sx = scales(id0.x), sy = scales(id0.y);
     }
 
@@ -383,18 +401,17 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
     __syncthreads();
 
     for (int32_t i = 0; i < n; ++i) {
-      issue(i + 1, id1);
       const float2 nx = scales(id1.x), ny = scales(id1.y);
-      const int2 id2{block_id(i + 2, 0), block_id(i + 2, 1)};
-      copy_wait<1>();
-      const uint32_t kb = ring + (i & 1) * L::SLOT + lane * 16;
+      const int2 id3{entry(i + 3, 0), entry(i + 3, 1)};
+      copy_wait<2>();  // this step's; the next one's K and V may be on their way
+      const uint8_t* here = att_smem + warp * L::RING + (i & 1) * L::SLOT;
       float acc[4][4] = {};
 #pragma unroll
       for (int pi = 0; pi < L::NP; ++pi) {
         uint32_t kw[4][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint4 x = lds128(kb + (j >> 1) * L::HALF + ((j & 1) * L::NP + pi) * 512);
+          const uint4 x = *reinterpret_cast<const uint4*>(here + lane * 16 + (j >> 1) * L::HALF + ((j & 1) * L::NP + pi) * 512);
           kw[j][0] = x.x, kw[j][1] = x.y, kw[j][2] = x.z, kw[j][3] = x.w;
         }
 #pragma unroll
@@ -408,6 +425,22 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
           }
         }
       }
+      id2 = checked(i + 2, id2);
+      issue_k(i + 2, id2);  // K of this step is in registers
+      uint32_t vr[2][4][L::NW];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const uint8_t* v = here + h * L::HALF + SUB * HD + (r * 32 + lane) * 4 * L::NW;
+          if constexpr (HD == 128) {
+            const uint4 x = *reinterpret_cast<const uint4*>(v);
+            vr[h][r][0] = x.x, vr[h][r][1] = x.y, vr[h][r][2] = x.z, vr[h][r][3] = x.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(v);
+            vr[h][r][0] = x.x, vr[h][r][1] = x.y;
+          }
+        }
       // scores in powers of two; lane (g, t) holds head g at positions 8 j + 2t, 8 j + 2t + 1
       float sv[4][2];
 #pragma unroll
@@ -428,7 +461,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
       float E[2], vf[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float vs = h ? sy.y : sx.y;
+        const float vs = (h ? id0.y : id0.x) < 0 ? 0.f : h ? sy.y : sx.y;
         const int e8 = max(1, min(254, (int)((__float_as_uint(vs) >> 23) & 255)));
         E[h] = (float)(e8 - 127);
         vf[h] = e8 == 254 ? vs * 0x1p-127f : vs * __int_as_float((254 - e8) << 23);
@@ -450,51 +483,35 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
         m = mn;
         M = Mn;
       }
-      // a step without positions (its blocks are bad) leaves both maxima at -inf
-      if (id0.x >= 0 || id0.y >= 0) {
-        uint4 pa[2];
+      // a step without positions (its blocks are bad) may leave the maxima at -inf: its weights are 0
+      const float m0 = m == -INFINITY ? 0.f : m, M0 = M == -INFINITY ? 0.f : M;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float wt[4];
-          const float vo = E[h] + 14.f;  // weights up to 2^15: their low parts stay normal f16
+      for (int h = 0; h < 2; ++h) {
+        float wt[4];
+        const float vo = E[h] + 14.f;  // weights up to 2^15: their low parts stay normal f16
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = sv[2 * h + (e >> 1)][e & 1];
-            l += ex2(x - m);
-            wt[e] = ex2((x - M) + vo) * vf[h];
-          }
-          split2(wt[0], wt[1], pa[h].x, pa[h].y);
-          split2(wt[2], wt[3], pa[h].z, pa[h].w);
+        for (int e = 0; e < 4; ++e) {
+          const float x = sv[2 * h + (e >> 1)][e & 1];
+          l += ex2(x - m0);
+          wt[e] = ex2((x - M0) + vo) * vf[h];
         }
-        // lane (g, t): rows 2t, 2t + 1, 2t + 8, 2t + 9, dims 4 NW g ..; n-tile j is dim j of each run
+        uint4 pa;
+        split2(wt[0], wt[1], pa.x, pa.y);
+        split2(wt[2], wt[3], pa.z, pa.w);
+        // n-tile j is dim j of each lane's run of V
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if ((h ? id0.y : id0.x) < 0) continue;
-          uint32_t vr[4][L::NW];
-          const uint32_t vb = ring + (i & 1) * L::SLOT + h * L::HALF + SUB * HD + lane * 4 * L::NW;
+        for (int w = 0; w < L::NW; ++w) {
+          uint32_t b0[4], b1[4];
+          to_f16<TYPE>(__byte_perm(vr[h][0][w], vr[h][1][w], 0x5140), b0[0], b0[1]);
+          to_f16<TYPE>(__byte_perm(vr[h][0][w], vr[h][1][w], 0x7362), b0[2], b0[3]);
+          to_f16<TYPE>(__byte_perm(vr[h][2][w], vr[h][3][w], 0x5140), b1[0], b1[1]);
+          to_f16<TYPE>(__byte_perm(vr[h][2][w], vr[h][3][w], 0x7362), b1[2], b1[3]);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            if constexpr (HD == 128) {
-              const uint4 x = lds128(vb + r * 512);
-              vr[r][0] = x.x, vr[r][1] = x.y, vr[r][2] = x.z, vr[r][3] = x.w;
-            } else {
-              const uint2 x = lds64(vb + r * 256);
-              vr[r][0] = x.x, vr[r][1] = x.y;
-            }
-          }
-#pragma unroll
-          for (int w = 0; w < L::NW; ++w) {
-            uint32_t b0[4], b1[4];
-            to_f16<TYPE>(__byte_perm(vr[0][w], vr[1][w], 0x5140), b0[0], b0[1]);
-            to_f16<TYPE>(__byte_perm(vr[0][w], vr[1][w], 0x7362), b0[2], b0[3]);
-            to_f16<TYPE>(__byte_perm(vr[2][w], vr[3][w], 0x5140), b1[0], b1[1]);
-            to_f16<TYPE>(__byte_perm(vr[2][w], vr[3][w], 0x7362), b1[2], b1[3]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mma_f16(o[4 * w + e], pa[h], b0[e], b1[e]);
-          }
+          for (int e = 0; e < 4; ++e) mma_f16(o[4 * w + e], pa, b0[e], b1[e]);
         }
       }
-      id0 = id1, id1 = id2;
+      issue_v(i + 2, id2);
+      id0 = id1, id1 = id2, id2 = id3;
       sx = nx, sy = ny;
     }
     copy_wait<0>();
