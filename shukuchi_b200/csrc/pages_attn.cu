@@ -10,15 +10,17 @@
 // the pieces.  Lengths are read on the device only.
 //
 // Inside a unit each of the 4 warps takes 32 positions: two times 16, which lie
-// in one block each and so share one scale of K and one of V.  Every lane copies
-// the bytes that its own tensor-core fragments hold (cp.async, the next step's
-// while this one is computed), so nothing in the loop waits for another thread.
+// in one block each and so share one scale of K and one of V.  A warp copies its
+// own steps (cp.async: the next V while this step is computed, the next K from
+// the moment this one has been multiplied), so no warp waits for another.
 //
 //   S = q K^T by mma.m16n8k16 in f16: the bytes of both pool types are exact in
 //   f16, q is scaled by a power of two and split into two f16 parts (22 bits):
 //   head g's high part is row g of the A operand and its low part row g + 8, so
 //   both go through one instruction and their sums meet in one lane.
-//   O = P V the same way: the weights' high and low parts are rows g and g + 8.
+//   O^T = V^T P^T, the weights in two f16 parts as well, one instruction each:
+//   lane (g, t) has the scores of head g that its B fragment asks for, and a
+//   head's outputs take half the registers that they would as rows.
 //
 // The softmax runs with two maxima per head: m of the scores for the sum, and M
 // of score + E, E the exponent of the block's V scale (V = 2^E f byte), for the
@@ -42,9 +44,8 @@ constexpr int HEADS = 8;        // query heads of an item: the MMA's rows g
 constexpr int SUB = 16;         // positions under one pair of scales
 constexpr int STEP = 2 * SUB;   // positions of a warp's step
 constexpr int UNIT = STEP * WARPS;
-constexpr int SLOTS = 2;
-constexpr int CTAS_PER_SM = 3;  // 168 registers a thread
-constexpr int MAX_CTAS = 480;   // 3 x the SMs of a B200 (148), rounded up
+constexpr int CTAS_PER_SM = 4;  // 128 registers a thread
+constexpr int MAX_CTAS = 640;   // 4 x the SMs of a B200 (148), rounded up
 constexpr int ITEM_UNITS = 1;   // what an item costs besides its positions, in units
 constexpr int MIN_UNITS = 2;    // a CTA's part: shorter ones cost more in joining than they save
 constexpr int JOIN_THREADS = 512;
@@ -54,12 +55,11 @@ struct Lay {
   static constexpr int NP = HD / 64;            // 16-byte pieces of a K row per lane
   static constexpr int NW = HD / 32;            // words of a V row per lane
   static constexpr int STEPS = HD / 16;         // k-steps of q K^T
-  static constexpr int HALF = 2 * SUB * HD;     // bytes of 16 positions: K, then V
-  static constexpr int SLOT = 2 * HALF;
-  static constexpr int RING = SLOTS * SLOT;     // per warp
+  static constexpr int HALF = SUB * HD;         // bytes of 16 positions of K or V
+  static constexpr int KBUF = 2 * HALF;         // a step's K; V has two such buffers behind it
+  static constexpr int RING = 3 * KBUF;         // per warp
   static constexpr int QF = STEPS * 32 * 16;    // q fragments
-  static constexpr int TROW = HD / 4 + 4;       // floats of a lane's output run, padded
-  static constexpr int HROW = 4 * TROW;
+  static constexpr int HROW = HD + 4;           // floats of a head's outputs in shared memory, padded
   static constexpr int BYTES = WARPS * RING + QF;
   static constexpr int REC = HEADS * (HD + 3);  // floats of a piece's record: O, m, M, l
   static_assert(HEADS * HROW * 4 <= RING, "a warp's output fits its ring");
@@ -89,20 +89,12 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-template <int BYTES>
 __device__ __forceinline__ void copy(uint32_t dst, const void* src) {
-  if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-template <int BYTES>
 __device__ __forceinline__ void copy_or_zero(uint32_t dst, const void* src, bool take) {
-  const uint32_t n = take ? BYTES : 0;  // 0: reads nothing, writes zeros
-  if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  const uint32_t n = take ? 16 : 0;  // 0: reads nothing, writes zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -176,35 +168,39 @@ struct Sums {
   uint32_t row;
 };
 
-// This lane's bytes of 16 positions p0 .. p0 + 15 of block id: of K the 16 bytes
-// at 16 t (and 64 + 16 t) of rows g and g + 8, of V the HD / 8 bytes at HD / 8 g
-// of rows 2t, 2t + 1, 2t + 8, 2t + 9.
+// Row of a request's position p0 in a pool.
 __device__ __forceinline__ size_t first_row(const PagesAttnArgs& a, int32_t id, uint32_t kvh, uint32_t p0) {
   const uint32_t bs = a.pool.block_shift;
   return (((size_t)id * a.pool.n_kv + kvh) << bs) + (p0 & ((1u << bs) - 1));
 }
-template <int HD>
-__device__ __forceinline__ void fetch_k(const uint8_t* row0, uint32_t dst, uint32_t lane) {
-  const uint8_t* k = row0 + (lane >> 2) * HD + 16 * (lane & 3);
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-#pragma unroll
-    for (int i = 0; i < Lay<HD>::NP; ++i) copy<16>(dst + lane * 16 + (j * Lay<HD>::NP + i) * 512, k + j * 8 * HD + 64 * i);
+
+// 16 rows of K or V go to shared memory as they lie, 512 bytes by an
+// instruction: quarter warps that reach into several lines halve the rate (V's
+// fragments fetched directly, 16 bytes of 4 rows each: 4.4 against 6.0 TB/s).
+// 16-byte piece p of 128-byte line r is stored at piece p ^ swizzle(r), which
+// spreads the pieces that 8 lanes read at a time over all banks: K's are pieces
+// t (+ 4) of rows 2q and 2q + 1, V's pieces g of rows 2t (head_dim 64: two rows
+// a line, V's are the halves of piece g / 2 of line t).
+template <int HD, bool V>
+__device__ __forceinline__ constexpr uint32_t swizzle(uint32_t line) {
+  return HD == 64 ? (line & 3) * 2 : V ? line & 6 : (line & 1) * 4;
 }
-// Only `rows` of the positions are the row's.  What lies behind them gets
-// weight 0; e4m3 values become zeros here too, as a NaN byte would outlive that.
-template <int HD, uint32_t TYPE>
-__device__ __forceinline__ void fetch_v(const uint8_t* row0, uint32_t dst, uint32_t rows, uint32_t lane) {
-  constexpr int NB = HD / 8;
-  const uint32_t t = lane & 3;
-  const uint8_t* v = row0 + 2 * t * HD + NB * (lane >> 2);
+template <int HD, bool V>
+__device__ __forceinline__ uint32_t at_piece(uint32_t line, uint32_t piece) {
+  return line * 128 + ((piece ^ swizzle<HD, V>(line)) << 4);
+}
+// Only `rows` of V's positions are the row's.  What lies behind them gets weight
+// 0; e4m3 values become zeros here too, as a NaN byte would outlive that.
+template <int HD, uint32_t TYPE, bool V>
+__device__ __forceinline__ void fetch(const uint8_t* row0, uint32_t dst, uint32_t rows, uint32_t lane) {
+  const uint8_t* src = row0 + 16 * lane;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int row = (r & 1) + 8 * (r >> 1);
-    if constexpr (TYPE == PAGES_I8)
-      copy<NB>(dst + (r * 32 + lane) * NB, v + row * HD);
+  for (int j = 0; j < Lay<HD>::HALF / 512; ++j) {
+    const uint32_t to = dst + at_piece<HD, V>(4 * j + (lane >> 3), lane & 7);
+    if constexpr (V && TYPE == PAGES_E4M3)
+      copy_or_zero(to, src + 512 * j, (512 * j + 16 * lane) / HD < rows);
     else
-      copy_or_zero<NB>(dst + (r * 32 + lane) * NB, v + row * HD, 2 * t + row < rows);
+      copy(to, src + 512 * j);
   }
 }
 
@@ -288,6 +284,13 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
   const uint32_t ring = smem_u32(att_smem) + warp * L::RING;
   uint4* qf = reinterpret_cast<uint4*>(att_smem + WARPS * L::RING);
 
+  // where this lane's fragments lie: pieces of K's row g, of V's row 2t (rows 8 further on are swizzled alike)
+  uint32_t k_at[L::NP];
+#pragma unroll
+  for (int i = 0; i < L::NP; ++i)
+    k_at[i] = HD == 128 ? at_piece<HD, false>(g, 4 * i + t) : at_piece<HD, false>(g >> 1, 4 * (g & 1) + t);
+  const uint32_t v_at = HD == 128 ? at_piece<HD, true>(2 * t, g) : at_piece<HD, true>(t, g >> 1) + 8 * (g & 1);
+
   while (s < end) {
     // the item, and this piece of it: units ua .. ub - 1 (its first ITEM_UNITS places in the line stand for its fixed cost)
     const uint32_t span = rw.units + ITEM_UNITS;
@@ -332,22 +335,21 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
       return id;
     };
     auto issue_k = [&](int32_t i, int2 id) {
-      const uint32_t dst = ring + (i & 1) * L::SLOT;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         if ((h ? id.y : id.x) >= 0)
-          fetch_k<HD>(a.pool.k + first_row(a, h ? id.y : id.x, kvh, place(i, h)) * HD, dst + h * L::HALF, lane);
+          fetch<HD, TYPE, false>(a.pool.k + first_row(a, h ? id.y : id.x, kvh, place(i, h)) * HD, ring + h * L::HALF, 0, lane);
       copy_commit();
     };
     auto issue_v = [&](int32_t i, int2 id) {
-      const uint32_t dst = ring + (i & 1) * L::SLOT + SUB * HD;
+      const uint32_t dst = ring + L::KBUF + (i & 1) * L::KBUF;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if ((h ? id.y : id.x) >= 0)
-          fetch_v<HD, TYPE>(a.pool.v + first_row(a, h ? id.y : id.x, kvh, place(i, h)) * HD, dst + h * L::HALF,
-                            rw.len - place(i, h), lane);
+          fetch<HD, TYPE, true>(a.pool.v + first_row(a, h ? id.y : id.x, kvh, place(i, h)) * HD, dst + h * L::HALF,
+                                rw.len - place(i, h), lane);
         else if (TYPE == PAGES_E4M3 && i < n)
-          fetch_v<HD, TYPE>(a.pool.v, dst + h * L::HALF, 0, lane);
+          fetch<HD, TYPE, true>(a.pool.v, dst + h * L::HALF, 0, lane);
       }
       copy_commit();
     };
@@ -356,21 +358,17 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
       return make_float2(a.pool.ks[at], a.pool.vs[at]);
     };
     float m = -INFINITY, M = -INFINITY, l = 0.f;
-    float o[HD / 8][4];
+    float o[HD / 16][4];
 #pragma unroll
-    for (int j = 0; j < HD / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    int2 id0{-1, -1}, id1{-1, -1}, id2{-1, -1};
+    for (int j = 0; j < HD / 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    int2 id0{-1, -1}, id1{-1, -1};
     float2 sx{}, sy{};
     if (n > 0) {  // the first copies are on their way before q is needed
       id0 = int2{entry(0, 0), entry(0, 1)};
       id1 = int2{entry(1, 0), entry(1, 1)};
-      id2 = int2{entry(2, 0), entry(2, 1)};
       id0 = checked(0, id0);
       issue_k(0, id0);
       issue_v(0, id0);
-      id1 = checked(1, id1);
-      issue_k(1, id1);
-      issue_v(1, id1);
       sx = scales(id0.x), sy = scales(id0.y);
     }
 
@@ -401,17 +399,20 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
     __syncthreads();
 
     for (int32_t i = 0; i < n; ++i) {
+      id1 = checked(i + 1, id1);
+      issue_v(i + 1, id1);
       const float2 nx = scales(id1.x), ny = scales(id1.y);
-      const int2 id3{entry(i + 3, 0), entry(i + 3, 1)};
-      copy_wait<2>();  // this step's; the next one's K and V may be on their way
-      const uint8_t* here = att_smem + warp * L::RING + (i & 1) * L::SLOT;
+      const int2 id2{entry(i + 2, 0), entry(i + 2, 1)};
+      copy_wait<1>();  // this step's K and V; the next V may be on its way
+      __syncwarp();
+      const uint8_t* here = att_smem + warp * L::RING;
       float acc[4][4] = {};
 #pragma unroll
       for (int pi = 0; pi < L::NP; ++pi) {
         uint32_t kw[4][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint4 x = *reinterpret_cast<const uint4*>(here + lane * 16 + (j >> 1) * L::HALF + ((j & 1) * L::NP + pi) * 512);
+          const uint4 x = *reinterpret_cast<const uint4*>(here + (j >> 1) * L::HALF + k_at[pi] + (j & 1) * 8 * HD);
           kw[j][0] = x.x, kw[j][1] = x.y, kw[j][2] = x.z, kw[j][3] = x.w;
         }
 #pragma unroll
@@ -425,22 +426,8 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
           }
         }
       }
-      id2 = checked(i + 2, id2);
-      issue_k(i + 2, id2);  // K of this step is in registers
-      uint32_t vr[2][4][L::NW];
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const uint8_t* v = here + h * L::HALF + SUB * HD + (r * 32 + lane) * 4 * L::NW;
-          if constexpr (HD == 128) {
-            const uint4 x = *reinterpret_cast<const uint4*>(v);
-            vr[h][r][0] = x.x, vr[h][r][1] = x.y, vr[h][r][2] = x.z, vr[h][r][3] = x.w;
-          } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(v);
-            vr[h][r][0] = x.x, vr[h][r][1] = x.y;
-          }
-        }
+      __syncwarp();
+      issue_k(i + 1, id1);  // this step's K has been multiplied
       // scores in powers of two; lane (g, t) holds head g at positions 8 j + 2t, 8 j + 2t + 1
       float sv[4][2];
 #pragma unroll
@@ -478,8 +465,10 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
       if (__any_sync(0xffffffffu, mn > m || Mn > M)) {
         const float al = m == mn ? 1.f : ex2(m - mn), aM = M == Mn ? 1.f : ex2(M - Mn);
         l *= al;
+        // the outputs of lane (g, t) are heads 2t and 2t + 1
+        const float a0 = __shfl_sync(0xffffffffu, aM, 8 * t), a1 = __shfl_sync(0xffffffffu, aM, 8 * t + 4);
 #pragma unroll
-        for (int j = 0; j < HD / 8; ++j) o[j][0] *= aM, o[j][1] *= aM, o[j][2] *= aM, o[j][3] *= aM;
+        for (int j = 0; j < HD / 16; ++j) o[j][0] *= a0, o[j][1] *= a1, o[j][2] *= a0, o[j][3] *= a1;
         m = mn;
         M = Mn;
       }
@@ -495,40 +484,50 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
           l += ex2(x - m0);
           wt[e] = ex2((x - M0) + vo) * vf[h];
         }
-        uint4 pa;
-        split2(wt[0], wt[1], pa.x, pa.y);
-        split2(wt[2], wt[3], pa.z, pa.w);
-        // n-tile j is dim j of each lane's run of V
+        uint32_t hi0, lo0, hi1, lo1;
+        split2(wt[0], wt[1], hi0, lo0);
+        split2(wt[2], wt[3], hi1, lo1);
+        const uint8_t* vp = here + L::KBUF + (i & 1) * L::KBUF + h * L::HALF;
+        uint32_t vr[4][L::NW];
 #pragma unroll
-        for (int w = 0; w < L::NW; ++w) {
-          uint32_t b0[4], b1[4];
-          to_f16<TYPE>(__byte_perm(vr[h][0][w], vr[h][1][w], 0x5140), b0[0], b0[1]);
-          to_f16<TYPE>(__byte_perm(vr[h][0][w], vr[h][1][w], 0x7362), b0[2], b0[3]);
-          to_f16<TYPE>(__byte_perm(vr[h][2][w], vr[h][3][w], 0x5140), b1[0], b1[1]);
-          to_f16<TYPE>(__byte_perm(vr[h][2][w], vr[h][3][w], 0x7362), b1[2], b1[3]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mma_f16(o[4 * w + e], pa, b0[e], b1[e]);
+        for (int r = 0; r < 4; ++r) {
+          if constexpr (HD == 128) {
+            const uint4 x = *reinterpret_cast<const uint4*>(vp + v_at + ((r & 1) + 8 * (r >> 1)) * HD);
+            vr[r][0] = x.x, vr[r][1] = x.y, vr[r][2] = x.z, vr[r][3] = x.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(vp + (v_at ^ ((r & 1) * 64)) + 8 * (r >> 1) * HD);
+            vr[r][0] = x.x, vr[r][1] = x.y;
+          }
         }
+        // tile j: rows g and g + 8 are dims 2j and 2j + 1 of the lane's run
+#pragma unroll
+        for (int w = 0; w < L::NW; ++w)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            uint4 va;
+            to_f16<TYPE>(__byte_perm(vr[0][w], vr[1][w], e ? 0x7362 : 0x5140), va.x, va.y);
+            to_f16<TYPE>(__byte_perm(vr[2][w], vr[3][w], e ? 0x7362 : 0x5140), va.z, va.w);
+            mma_f16(o[2 * w + e], va, hi0, hi1);
+            mma_f16(o[2 * w + e], va, lo0, lo1);
+          }
       }
-      issue_v(i + 2, id2);
-      id0 = id1, id1 = id2, id2 = id3;
+      id0 = id1, id1 = id2;
       sx = nx, sy = ny;
+      __syncwarp();  // the next V goes where this one was
     }
     copy_wait<0>();
 
     // ---- the warps' outputs meet in shared memory (each in its own ring) ----
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
-    float* mo = reinterpret_cast<float*>(att_smem + warp * L::RING) + g * L::HROW + t * L::TROW;
-    // tile j, column 2t / 2t + 1 is dim j of run 2t / 2t + 1: the lane's outputs are HD / 4 dims in a row
+    // lane (g, t): heads 2t and 2t + 1, the HD / 8 dims from HD / 8 g
+    float* mo = reinterpret_cast<float*>(att_smem + warp * L::RING) + 2 * t * L::HROW + g * (HD / 8);
     __syncwarp();
 #pragma unroll
     for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int j = 0; j < HD / 8; j += 4)
-        *reinterpret_cast<float4*>(mo + r * (HD / 8) + j) =
-            make_float4(o[j][r] + o[j][r + 2], o[j + 1][r] + o[j + 1][r + 2], o[j + 2][r] + o[j + 2][r + 2],
-                        o[j + 3][r] + o[j + 3][r + 2]);
+      for (int j = 0; j < HD / 16; j += 2)
+        *reinterpret_cast<float4*>(mo + r * L::HROW + 2 * j) = make_float4(o[j][r], o[j][r + 2], o[j + 1][r], o[j + 1][r + 2]);
     if (t == 0) stat[warp][g][0] = m, stat[warp][g][1] = M, stat[warp][g][2] = l;
     __syncthreads();
     const bool whole = ua == 0 && ub == rw.units;
@@ -546,7 +545,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
         if (lw == 0.f) continue;  // a warp without positions
         ll += lw * ex2(stat[w][h][0] - mm);
         const float x = ex2(stat[w][h][1] - MM);
-        const float* src = reinterpret_cast<const float*>(att_smem + w * L::RING) + h * L::HROW + (d / (HD / 4)) * L::TROW + d % (HD / 4);
+        const float* src = reinterpret_cast<const float*>(att_smem + w * L::RING) + h * L::HROW + d;
 #pragma unroll
         for (int e = 0; e < PER; ++e) out[e] += src[e] * x;
       }
@@ -585,7 +584,7 @@ template <int HD>
 __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const __grid_constant__ PagesAttnArgs a) {
   using L = Lay<HD>;
   constexpr int PER_GROUP = HEADS * HD / 4, GROUPS = JOIN_THREADS / PER_GROUP;
-  __shared__ __align__(16) float st[3][HEADS][MAX_CTAS + 1];
+  __shared__ __align__(16) float st[2][HEADS][MAX_CTAS + 1];
   __shared__ float fin[HEADS];
   float4* sum = reinterpret_cast<float4*>(st[0]);  // the maxima are done with by then
   static_assert(sizeof(st[0]) >= JOIN_THREADS * sizeof(float4), "outputs fit where the maxima were");
@@ -597,8 +596,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const __grid_
   const uint32_t n_kv = a.pool.n_kv, G = a.n_heads / n_kv, nsub = (G + HEADS - 1) / HEADS;
   const uint32_t kvh = hd.item / nsub, sub = hd.item % nsub, n = (uint32_t)hd.last - c + 1;
   auto rec = [&](uint32_t i) { return records + (size_t)(2 * (c + i) + (i == 0 ? hd.slot : 0)) * L::REC; };
-  for (uint32_t i = tid; i < n * 3 * HEADS; i += JOIN_THREADS) {
-    const uint32_t p = i / (3 * HEADS), k = i % (3 * HEADS);
+  for (uint32_t i = tid; i < n * 2 * HEADS; i += JOIN_THREADS) {
+    const uint32_t p = i / (2 * HEADS), k = i % (2 * HEADS);
     st[k / HEADS][k % HEADS][p] = rec(p)[HEADS * HD + k];
   }
   __syncthreads();
@@ -609,7 +608,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const __grid_
     m = warp_max(m);
     M = warp_max(M);
     for (uint32_t i = lane; i < n; i += 32) {
-      const float x = st[2][h][i];
+      const float x = rec(i)[HEADS * (HD + 2) + h];
       const bool some = x != 0.f;  // else a piece without positions
       l += some ? x * ex2(st[0][h][i] - m) : 0.f;
       st[1][h][i] = some ? ex2(st[1][h][i] - M) : 0.f;
