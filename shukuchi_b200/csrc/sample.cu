@@ -4,6 +4,17 @@
 // both in fp32, and the weights become whole numbers W = floor(w * 2^40):
 // every sum below is a sum of integers, so that the token that a random
 // number picks does not depend on the order in which threads add.
+//
+// The row is read once: a thread-block cluster takes it, each CTA a run of the
+// vocabulary that stays in its shared memory, and what the CTAs need of one
+// another (maximum, histograms, sums) goes over distributed shared memory.
+// Nothing is sorted.  Tokens are ordered by (logit, lower index), each one's
+// place being one 50-bit number c, and top-k and top-p together keep c >= C.
+// C is found from a histogram over x (count and weight per bin, 1024 bins down
+// to the x whose weight is 0): the bin that holds the border token has some
+// hundred tokens in a row of 128k, which every CTA gets and ranks by
+// comparison.  A bin with more than CAP tokens (equal logits, mostly) is
+// searched by the digits of c instead.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -17,33 +28,49 @@
 namespace shk {
 namespace {
 
-constexpr int THREADS = 1024;
+constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
+constexpr int MAX_CL = 8;
+constexpr int NB = 2 * THREADS;      // bins; thread t owns 2t and 2t + 1
+constexpr int CAP = 512;             // candidates that are ranked by comparison
+constexpr int SEGS = 128;            // runs of a slice whose kept weights are summed apart, 8 a warp
+constexpr float X_MIN = -27.75f;     // exp(x) * 2^40 < 1 below
+constexpr int IDX_BITS = 18;
+constexpr uint32_t IDX_MASK = (1u << IDX_BITS) - 1;
+static_assert(SAMPLE_MAX_VOCAB <= 1u << IDX_BITS, "an index fits its bits of c");
+constexpr uint32_t MAX_SLICE = SAMPLE_MAX_VOCAB / MAX_CL;
 
 template <uint32_t DT>
 __device__ __forceinline__ float logit(const void* p, size_t i) {
-  float z;
-  if constexpr (DT == DT_F32)
-    z = static_cast<const float*>(p)[i];
-  else if constexpr (DT == DT_F16)
-    z = __half2float(static_cast<const __half*>(p)[i]);
-  else
-    z = __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-  return z + 0.f;  // -0 becomes +0: the two compare equal, and so do their keys
+  if constexpr (DT == DT_F32) return static_cast<const float*>(p)[i];
+  if constexpr (DT == DT_F16) return __half2float(static_cast<const __half*>(p)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
 }
+// As the row is held: NaN as -inf, and -0 as +0 (the two compare equal).
+__device__ __forceinline__ float clean(float z) { return z == z ? z + 0.f : -INFINITY; }
 
-// Larger logits have larger keys; NaN comes last.
+// Larger logits have larger keys.
 __device__ __forceinline__ uint32_t key_of(float z) {
-  if (z != z) return 0;
   const uint32_t u = __float_as_uint(z);
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
-
-__device__ __forceinline__ float weight_of(float z, float zmax, float inv_t) {
-  const float x = (z - zmax) * inv_t;
-  if (z == zmax) return 1.f;
-  return x <= 0.f ? expf(x) : 0.f;  // NaN (masked or not a number): 0
+__device__ __forceinline__ uint64_t place_of(float z, uint32_t i) {
+  return ((uint64_t)key_of(z) << IDX_BITS) | (IDX_MASK - i);
 }
+
+struct Scale {
+  float zmax, inv_t;
+  __device__ __forceinline__ float x(float z) const { return (z - zmax) * inv_t; }
+  __device__ __forceinline__ float weight(float z) const {
+    const float v = x(z);
+    if (z == zmax) return 1.f;
+    return v <= 0.f ? expf(v) : 0.f;  // NaN (a masked token at an infinite T): 0
+  }
+  // Falls with z from bin 0 on.
+  __device__ __forceinline__ int bin(float z) const {
+    return z == zmax ? 0 : min(NB - 1, (int)(x(z) * (NB / X_MIN)));
+  }
+};
 __device__ __forceinline__ uint64_t mass_of(float w) { return (uint64_t)(w * 1099511627776.f); }
 
 __device__ __forceinline__ uint64_t warp_sum64(uint64_t v) {
@@ -51,198 +78,418 @@ __device__ __forceinline__ uint64_t warp_sum64(uint64_t v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+template <typename T>
+__device__ __forceinline__ T warp_scan(T v, uint32_t lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const T u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= (uint32_t)o) v += u;
+  }
+  return v;
+}
 
-struct Shared {
-  uint64_t mass[256];
-  uint32_t count[256];
-  uint64_t part[WARPS];
-  uint32_t ties[WARPS];
-  float red[WARPS];
-  uint32_t idx[WARPS];
-  uint32_t key;        // radix select: the border key
-  uint64_t above;      // mass (or count) of larger keys
+// ---- cluster ----
+__device__ __forceinline__ uint32_t cl_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cl_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cl_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void put32(uint32_t a, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+__device__ __forceinline__ void put64(uint32_t a, uint64_t v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t get32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 get32x2(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ ulonglong2 get64x2(uint32_t a) {
+  ulonglong2 v;
+  asm volatile("ld.shared::cluster.v2.u64 {%0, %1}, [%2];" : "=l"(v.x), "=l"(v.y) : "r"(a) : "memory");
+  return v;
+}
+
+struct Hist {
+  unsigned long long mass[NB];
+  uint32_t cnt[NB];
 };
 
-__device__ __forceinline__ uint64_t block_sum64(uint64_t v, Shared& s) {
-  v = warp_sum64(v);
+struct Shared {
+  Hist hist, digits;
+  uint64_t cand[2][CAP];    // places and weights of the border bin's tokens (top-k's, top-p's)
+  uint64_t cand_w[2][CAP];
+  uint64_t seg[SEGS];
+  uint64_t part[WARPS];
+  uint64_t xsum[MAX_CL];
+  uint32_t part32[WARPS];
+  float xmax[MAX_CL];
+  uint32_t xidx[MAX_CL];
+  // the border that one thread found
+  uint64_t border, above_mass, inside;
+  uint32_t above_cnt, bin, in_bin;
+  uint32_t taken;
+};
+
+// Totals of a cluster's histograms at this thread's two bins, and the running
+// totals before them (bin 0 holds the largest tokens).
+struct Totals {
+  uint32_t c[2], before_c;
+  uint64_t m[2], before_m;
+};
+
+__device__ Totals totals(const Hist& h, uint32_t cl, Shared& s) {
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Totals t{};
+  for (uint32_t r = 0; r < cl; ++r) {
+    const uint2 c = get32x2(peer(&h.cnt[2 * threadIdx.x], r));
+    const ulonglong2 m = get64x2(peer(&h.mass[2 * threadIdx.x], r));
+    t.c[0] += c.x, t.c[1] += c.y;
+    t.m[0] += m.x, t.m[1] += m.y;
+  }
+  const uint32_t sc = warp_scan(t.c[0] + t.c[1], lane);
+  const uint64_t sm = warp_scan(t.m[0] + t.m[1], lane);
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) s.part[threadIdx.x >> 5] = v;
+  if (lane == 31) s.part32[warp] = sc, s.part[warp] = sm;
   __syncthreads();
-  uint64_t t = 0;
-  for (int w = 0; w < WARPS; ++w) t += s.part[w];
+  t.before_c = sc - t.c[0] - t.c[1];
+  t.before_m = sm - t.m[0] - t.m[1];
+  for (uint32_t w = 0; w < warp; ++w) t.before_c += s.part32[w], t.before_m += s.part[w];
   return t;
 }
 
-// The largest key at which the running total from the largest key down
-// reaches `need`: by count (BY_MASS false) or by mass, over keys >= floor_key.
-// Returns the key; `above` is the total of the keys over it.
-template <uint32_t DT, bool BY_MASS>
-__device__ uint32_t border(const void* z, uint32_t n, float zmax, float inv_t, uint32_t floor_key, uint64_t need,
-                           uint64_t& above, Shared& s) {
-  uint32_t prefix = 0;
-  uint64_t over = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += THREADS) s.mass[i] = 0;
+// The bin at which the running total reaches `need`: s.bin, s.above_cnt,
+// s.above_mass, s.in_bin; s.bin == NB where it does not.
+template <bool BY_MASS>
+__device__ void find_bin(const Totals& t, uint64_t need, Shared& s) {
+  __syncthreads();
+  if (threadIdx.x == 0) s.bin = NB;
+  __syncthreads();
+  uint32_t c = t.before_c;
+  uint64_t m = t.before_m;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint64_t lo = BY_MASS ? m : c, hi = BY_MASS ? m + t.m[i] : c + t.c[i];
+    if (lo < need && need <= hi) s.bin = 2 * threadIdx.x + i, s.above_cnt = c, s.above_mass = m, s.in_bin = t.c[i];
+    c += t.c[i];
+    m += t.m[i];
+  }
+  __syncthreads();
+}
+
+// The border token in the bin that find_bin left: s.border = its place, and
+// s.inside = the weight of the bin's tokens down to it.  `list`: which of the
+// two candidate lists is used.
+template <bool BY_MASS>
+__device__ void find_border(const float* z, uint32_t n, uint32_t base, const Scale& sc, uint64_t need, int list,
+                            uint32_t rank, uint32_t cl, Shared& s) {
+  const int bin = (int)s.bin;
+  const uint64_t left = need - (BY_MASS ? s.above_mass : s.above_cnt);  // of the bin's own
+  const uint32_t m = s.in_bin;
+  if (m <= CAP) {
+    if (threadIdx.x == 0) {
+      uint32_t off = 0;
+      for (uint32_t r = 0; r < rank; ++r) off += get32(peer(&s.hist.cnt[bin], r));
+      s.taken = off;
+    }
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-      const float v = logit<DT>(z, i);
-      const uint32_t key = key_of(v);
-      if (key < floor_key || (shift < 24 && (key >> (shift + 8)) != (prefix >> (shift + 8)))) continue;
-      const uint64_t add = BY_MASS ? mass_of(weight_of(v, zmax, inv_t)) : 1;
-      if (add) atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[(key >> shift) & 255]), (unsigned long long)add);
+      const float v = z[i];
+      if (sc.bin(v) != bin) continue;
+      const uint64_t w = mass_of(sc.weight(v));
+      if (w == 0) continue;
+      const uint32_t at = atomicAdd(&s.taken, 1);
+      for (uint32_t r = 0; r < cl; ++r) {
+        put64(peer(&s.cand[list][at], r), place_of(v, base + i));
+        put64(peer(&s.cand_w[list][at], r), w);
+      }
+    }
+    cl_sync();
+    if (threadIdx.x < m) {
+      const uint64_t me = s.cand[list][threadIdx.x], mine = s.cand_w[list][threadIdx.x];
+      uint64_t over = 0, over_w = 0;
+      for (uint32_t j = 0; j < m; ++j)
+        if (s.cand[list][j] > me) over += 1, over_w += s.cand_w[list][j];
+      const uint64_t o = BY_MASS ? over_w : over, own = BY_MASS ? mine : 1;
+      if (o < left && left <= o + own) s.border = me, s.inside = over_w + mine;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-      uint64_t c = over;
-      int b = 255;
-      while (b > 0 && c + s.mass[b] < need) c += s.mass[b--];
-      s.key = prefix | ((uint32_t)b << shift);
-      s.above = c;
-    }
-    __syncthreads();
-    prefix = s.key;
-    over = s.above;
-    __syncthreads();
+    return;
   }
-  above = over;
-  return prefix;
+  // digit by digit, from the top
+  uint64_t prefix = 0, over = 0, over_w = 0;
+  for (int shift = 40; shift >= 0; shift -= 10) {
+    for (int i = threadIdx.x; i < NB; i += THREADS) s.digits.cnt[i] = 0, s.digits.mass[i] = 0;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+      const float v = z[i];
+      if (sc.bin(v) != bin) continue;
+      const uint64_t w = mass_of(sc.weight(v)), c = place_of(v, base + i);
+      if (w == 0 || (c >> (shift + 10)) != prefix) continue;
+      const uint32_t d = NB - 1 - ((uint32_t)(c >> shift) & (NB - 1));
+      atomicAdd(&s.digits.cnt[d], 1u);
+      atomicAdd(&s.digits.mass[d], (unsigned long long)w);
+    }
+    cl_sync();
+    const Totals t = totals(s.digits, cl, s);
+    find_bin<BY_MASS>(t, left - (BY_MASS ? over_w : over), s);
+    over += s.above_cnt;
+    over_w += s.above_mass;
+    prefix = (prefix << 10) | (NB - 1 - s.bin);
+    cl_sync();  // every CTA has read the digits
+  }
+  if (threadIdx.x == 0) {
+    s.border = prefix;
+    const uint32_t key = (uint32_t)(prefix >> IDX_BITS);
+    s.inside = over_w + mass_of(sc.weight(__uint_as_float((key & 0x80000000u) ? key & 0x7FFFFFFFu : ~key)));
+  }
+  __syncthreads();
 }
 
 template <uint32_t DT>
-__global__ void __launch_bounds__(THREADS) sample_kernel(const __grid_constant__ SampleArgs a) {
-  __shared__ Shared s;
-  const uint32_t row = blockIdx.x, n = a.n_vocab, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const void* z = static_cast<const uint8_t*>(a.logits) + row * a.row_stride * (DT == DT_F32 ? 4 : 2);
+__global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constant__ SampleArgs a, uint32_t slice) {
+  extern __shared__ __align__(16) uint8_t sample_smem[];
+  float* z = reinterpret_cast<float*>(sample_smem);
+  Shared& s = *reinterpret_cast<Shared*>(sample_smem + sizeof(float) * slice);
+  const uint32_t rank = cl_rank(), cl = cl_size(), row = blockIdx.x / cl;
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t base = min(a.n_vocab, rank * slice), n = min(a.n_vocab - base, slice);
 
+  // ---- the slice, and its first maximum ----
+  constexpr int PER = DT == DT_F32 ? 4 : 8;  // logits in 16 bytes
+  const uint8_t* src = static_cast<const uint8_t*>(a.logits) + ((size_t)row * a.row_stride + base) * (16 / PER);
   float m = -INFINITY;
   uint32_t mi = 0xFFFFFFFFu;
-  for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-    const float v = logit<DT>(z, i);
+  auto take = [&](uint32_t i, float v) {
+    v = clean(v);
     if (v > m) m = v, mi = i;
+    return v;
+  };
+  uint32_t done = 0;
+  if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+    done = n / PER * PER;
+#pragma unroll 4
+    for (uint32_t i = tid; i < n / PER; i += THREADS) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < PER; e += 4) {
+        float4 f;
+        if constexpr (DT == DT_F32)
+          f = make_float4(__uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]), __uint_as_float(w[3]));
+        else if constexpr (DT == DT_F16) {
+          const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[e / 2]));
+          const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&w[e / 2 + 1]));
+          f = make_float4(x.x, x.y, y.x, y.y);
+        } else
+          f = make_float4(__uint_as_float(w[e / 2] << 16), __uint_as_float(w[e / 2] & 0xFFFF0000u),
+                          __uint_as_float(w[e / 2 + 1] << 16), __uint_as_float(w[e / 2 + 1] & 0xFFFF0000u));
+        const uint32_t at = i * PER + e;
+        f.x = take(at, f.x), f.y = take(at + 1, f.y), f.z = take(at + 2, f.z), f.w = take(at + 3, f.w);
+        *reinterpret_cast<float4*>(z + at) = f;
+      }
+    }
   }
+  for (uint32_t i = done + tid; i < n; i += THREADS) z[i] = take(i, logit<DT>(src, i));
+  if (mi != 0xFFFFFFFFu) mi += base;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float v = __shfl_xor_sync(0xffffffffu, m, o);
     const uint32_t i = __shfl_xor_sync(0xffffffffu, mi, o);
     if (v > m || (v == m && i < mi)) m = v, mi = i;
   }
-  if (lane == 0) s.red[warp] = m, s.idx[warp] = mi;
+  if (lane == 0) s.part32[warp] = mi, s.part[warp] = __float_as_uint(m);
+  for (int i = tid; i < NB; i += THREADS) s.hist.cnt[i] = 0, s.hist.mass[i] = 0;
   __syncthreads();
-  m = s.red[0], mi = s.idx[0];
-  for (int w = 1; w < WARPS; ++w)
-    if (s.red[w] > m || (s.red[w] == m && s.idx[w] < mi)) m = s.red[w], mi = s.idx[w];
+  if (tid < cl) {  // thread r tells CTA r
+    for (int w = 0; w < WARPS; ++w) {
+      const float v = __uint_as_float((uint32_t)s.part[w]);
+      const uint32_t i = s.part32[w];
+      if (v > m || (v == m && i < mi)) m = v, mi = i;
+    }
+    put32(peer(&s.xmax[rank], tid), __float_as_uint(m));
+    put32(peer(&s.xidx[rank], tid), mi);
+  }
+  cl_sync();
+  m = s.xmax[0], mi = s.xidx[0];
+  for (uint32_t r = 1; r < cl; ++r)
+    if (s.xmax[r] > m || (s.xmax[r] == m && s.xidx[r] < mi)) m = s.xmax[r], mi = s.xidx[r];
 
-  const float t = a.temperature ? a.temperature[row] : 1.f;
-  if (mi == 0xFFFFFFFFu || !(t > 0.f)) {
-    if (threadIdx.x == 0) {
+  const float temp = a.temperature ? a.temperature[row] : 1.f;
+  if (mi == 0xFFFFFFFFu || !(temp > 0.f)) {
+    if (rank == 0 && tid == 0) {
       a.out[row] = mi;
       if (a.prob) a.prob[row] = mi == 0xFFFFFFFFu ? 0.f : 1.f;
     }
     return;
   }
-  const float inv_t = __frcp_rn(t);
+  const Scale sc{m, __frcp_rn(temp)};
 
-  // the kept tokens are those over `floor_key` and the first `ties` at it
-  uint32_t floor_key = 0, ties = 0xFFFFFFFFu;
+  // ---- the border of top-k and top-p ----
+  uint64_t border = 0;  // tokens with a place of at least this stay
   const int32_t k = a.top_k ? a.top_k[row] : 0;
-  if (k > 0 && (uint32_t)k < n) {
-    uint64_t above;
-    floor_key = border<DT, false>(z, n, m, inv_t, 0, (uint64_t)k, above, s);
-    ties = (uint32_t)(k - above);
-  }
   const float top_p = a.top_p ? a.top_p[row] : 1.f;
-  if (top_p < 1.f) {
-    uint64_t sum = 0;
-    for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-      const float v = logit<DT>(z, i);
-      if (key_of(v) > floor_key) sum += mass_of(weight_of(v, m, inv_t));
+  const bool by_k = k > 0 && (uint32_t)k < a.n_vocab, by_p = top_p < 1.f;
+  if (by_k || by_p) {
+    for (uint32_t i = tid; i < n; i += THREADS) {
+      const float v = z[i];
+      const uint64_t w = mass_of(sc.weight(v));
+      if (w == 0) continue;
+      const int b = sc.bin(v);
+      atomicAdd(&s.hist.cnt[b], 1u);
+      atomicAdd(&s.hist.mass[b], (unsigned long long)w);
     }
-    sum = block_sum64(sum, s);
-    uint64_t at = 0;  // one token at the border
-    if (ties != 0xFFFFFFFFu) {
-      const uint32_t u = (floor_key & 0x80000000u) ? floor_key & 0x7FFFFFFFu : ~floor_key;
-      at = floor_key ? mass_of(weight_of(__uint_as_float(u), m, inv_t)) : 0;
-      sum += at * ties;
+    cl_sync();
+    const Totals t = totals(s.hist, cl, s);
+    uint64_t sum;  // of the top-k set
+    {
+      __syncthreads();
+      if (tid == THREADS - 1) s.inside = t.before_m + t.m[0] + t.m[1];
+      __syncthreads();
+      sum = s.inside;
     }
-    const double need_d = ceil((double)top_p * (double)sum);
-    const uint64_t need = need_d >= 1.0 ? (uint64_t)need_d : 1;
-    uint64_t above;
-    const uint32_t key = border<DT, true>(z, n, m, inv_t, floor_key, need, above, s);
-    const uint32_t u = (key & 0x80000000u) ? key & 0x7FFFFFFFu : ~key;
-    const uint64_t one = mass_of(weight_of(__uint_as_float(u), m, inv_t));
-    floor_key = key;
-    ties = one ? (uint32_t)min((need - above + one - 1) / one, (uint64_t)n) : n;
+    if (by_k) {
+      find_bin<false>(t, (uint64_t)k, s);
+      if (s.bin < NB) {  // else fewer than k tokens have a weight
+        find_border<false>(z, n, base, sc, (uint64_t)k, 0, rank, cl, s);
+        border = s.border;
+        // find_bin's sums may have been replaced by those of the digits: the bin's own again
+        sum = s.inside;
+        find_bin<false>(t, (uint64_t)k, s);
+        sum += s.above_mass;
+      }
+    }
+    if (by_p) {
+      const double need_d = ceil((double)top_p * (double)sum);
+      const uint64_t need = need_d >= 1.0 ? (uint64_t)need_d : 1;
+      find_bin<true>(t, need, s);
+      if (s.bin < NB) {
+        find_border<true>(z, n, base, sc, need, 1, rank, cl, s);
+        border = max(border, s.border);
+      }
+    }
   }
   float min_p = a.min_p ? a.min_p[row] : 0.f;
   min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;  // the largest weight, 1, always stays
 
-  // each warp takes a run of the vocabulary: ties at the border, then kept mass
-  const uint32_t per = ((n + WARPS - 1) / WARPS + 31) & ~31u;
-  const uint32_t lo = min(n, warp * per), hi = min(n, lo + per);
-  uint32_t mine = 0;
-  for (uint32_t i = lo + lane; i < hi; i += 32) mine += key_of(logit<DT>(z, i)) == floor_key;
-  mine = __reduce_add_sync(0xffffffffu, mine);
-  if (lane == 0) s.ties[warp] = mine;
-  __syncthreads();
-  uint32_t seen0 = 0;
-  for (uint32_t w = 0; w < warp; ++w) seen0 += s.ties[w];
-  auto kept = [&](uint32_t i, bool in, uint32_t& seen) -> uint64_t {
-    const float v = in ? logit<DT>(z, i) : -INFINITY;
-    const uint32_t key = in ? key_of(v) : 0;
-    const uint32_t eq = __ballot_sync(0xffffffffu, in && key == floor_key);
-    const uint32_t rank = seen + __popc(eq & ((1u << lane) - 1));
-    seen += __popc(eq);
-    if (!in || key < floor_key || (key == floor_key && rank >= ties)) return 0;
-    const float w = weight_of(v, m, inv_t);
+  // ---- weights that stay, summed over runs of the slice ----
+  const uint32_t border_key = (uint32_t)(border >> IDX_BITS), border_idx = IDX_MASK - ((uint32_t)border & IDX_MASK);
+  auto kept = [&](uint32_t i) -> uint64_t {
+    const float v = z[i];
+    const uint32_t key = key_of(v);
+    if (key < border_key || (key == border_key && base + i > border_idx)) return 0;
+    const float w = sc.weight(v);
     return w < min_p ? 0 : mass_of(w);
   };
+  const uint32_t run = (slice + SEGS - 1) / SEGS;
   uint64_t sum = 0;
-  uint32_t seen = seen0;
-  for (uint32_t i0 = lo; i0 < hi; i0 += 32) sum += kept(i0 + lane, i0 + lane < hi, seen);
-  sum = warp_sum64(sum);
-  __syncthreads();
+  for (uint32_t g = warp * (SEGS / WARPS); g < (warp + 1) * (SEGS / WARPS); ++g) {
+    uint64_t v = 0;
+    for (uint32_t i = g * run + lane; i < min(n, (g + 1) * run); i += 32) v += kept(i);
+    v = warp_sum64(v);
+    if (lane == 0) s.seg[g] = v;
+    sum += v;
+  }
+  __syncthreads();  // part: the scans above are done with it
   if (lane == 0) s.part[warp] = sum;
   __syncthreads();
+  if (tid < cl) {
+    uint64_t v = 0;
+    for (int w = 0; w < WARPS; ++w) v += s.part[w];
+    put64(peer(&s.xsum[rank], tid), v);
+  }
+  cl_sync();
   uint64_t total = 0, before = 0;
-  for (uint32_t w = 0; w < (uint32_t)WARPS; ++w) {
-    if (w == warp) before = total;
-    total += s.part[w];
+  for (uint32_t r = 0; r < cl; ++r) {
+    if (r == rank) before = total;
+    total += s.xsum[r];
   }
   const float uf = a.u[row];
   uint64_t target = uf > 0.f ? (uint64_t)fmin((double)uf * (double)total, 1.8e19) : 0;
   if (target >= total) target = total - 1;
-  if (target < before || target >= before + sum) return;
-  seen = seen0;
-  for (uint32_t i0 = lo; i0 < hi; i0 += 32) {
-    const uint64_t w = kept(i0 + lane, i0 + lane < hi, seen);
-    uint64_t c = w;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t u = __shfl_up_sync(0xffffffffu, c, o);
-      if (lane >= (uint32_t)o) c += u;
-    }
-    const uint32_t hit = __ballot_sync(0xffffffffu, before + c > target);
+  if (target < before || target >= before + s.xsum[rank]) return;
+  if (warp != 0) return;
+  // the run, then the token
+  static_assert(SEGS == 128, "4 runs a lane");
+  uint64_t c = s.seg[4 * lane] + s.seg[4 * lane + 1] + s.seg[4 * lane + 2] + s.seg[4 * lane + 3];
+  const uint64_t upto = before + warp_scan(c, lane);
+  const uint32_t lane_hit = (uint32_t)__ffs(__ballot_sync(0xffffffffu, upto > target)) - 1;
+  before = __shfl_sync(0xffffffffu, upto - c, lane_hit);
+  uint32_t g = 4 * lane_hit;
+  while (before + s.seg[g] <= target) before += s.seg[g++];
+  for (uint32_t i0 = g * run;; i0 += 32) {
+    const uint32_t i = i0 + lane;
+    const uint64_t w = i < min(n, (g + 1) * run) ? kept(i) : 0;
+    const uint64_t to = before + warp_scan(w, lane);
+    const uint32_t hit = __ballot_sync(0xffffffffu, to > target);
     if (hit) {
       if (lane == (uint32_t)__ffs(hit) - 1) {
-        a.out[row] = i0 + lane;
+        a.out[row] = base + i;
         if (a.prob) a.prob[row] = (float)((double)w / (double)total);
       }
       return;
     }
-    before += __shfl_sync(0xffffffffu, c, 31);
+    if (i0 >= (g + 1) * run) return;  // not reached: the run's sum holds the target
+    before = __shfl_sync(0xffffffffu, to, 31);
   }
+}
+
+template <uint32_t DT>
+cudaError_t sample_go(const SampleArgs& a, int num_sms, cudaStream_t st) {
+  // As many CTAs a row as its slice needs, more while the rows leave SMs idle.
+  uint32_t cl = 1;
+  while (cl < MAX_CL && (a.n_vocab > cl * 16384 || (a.n_rows * cl * 2 <= (uint32_t)num_sms && a.n_vocab > cl * 2048))) cl *= 2;
+  const uint32_t slice = ((a.n_vocab + cl - 1) / cl + 127) / 128 * 128;
+  const size_t smem = sizeof(float) * slice + sizeof(Shared);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.n_rows * cl);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cl;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, sample_kernel<DT>, a, slice);
 }
 
 }  // namespace
 
-cudaError_t sample_launch(const SampleArgs& a, int, cudaStream_t st) {
-  if (a.dtype == DT_F32)
-    sample_kernel<DT_F32><<<a.n_rows, THREADS, 0, st>>>(a);
-  else if (a.dtype == DT_F16)
-    sample_kernel<DT_F16><<<a.n_rows, THREADS, 0, st>>>(a);
-  else
-    sample_kernel<DT_BF16><<<a.n_rows, THREADS, 0, st>>>(a);
-  return cudaGetLastError();
+cudaError_t sample_init() {
+  const int smem = sizeof(float) * MAX_SLICE + sizeof(Shared);
+  const auto big = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  cudaError_t e = cudaFuncSetAttribute(sample_kernel<DT_F32>, big, smem);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(sample_kernel<DT_F16>, big, smem);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(sample_kernel<DT_BF16>, big, smem);
+  return e;
+}
+
+cudaError_t sample_launch(const SampleArgs& a, int num_sms, cudaStream_t st) {
+  if (a.dtype == DT_F32) return sample_go<DT_F32>(a, num_sms, st);
+  return a.dtype == DT_F16 ? sample_go<DT_F16>(a, num_sms, st) : sample_go<DT_BF16>(a, num_sms, st);
 }
 
 }  // namespace shk

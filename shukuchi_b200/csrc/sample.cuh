@@ -22,6 +22,7 @@ struct SampleArgs {
 
 constexpr uint32_t SAMPLE_MAX_VOCAB = 262144;
 
+cudaError_t sample_init();  // kernel attributes, once per device
 cudaError_t sample_launch(const SampleArgs& a, int num_sms, cudaStream_t st);
 
 }  // namespace shk

@@ -448,6 +448,7 @@ shk_ctx* shk_cuda_init(const shk_cuda_config* cfg) {
   ok = ok && mmv_init() == cudaSuccess;
   ok = ok && q5k_init() == cudaSuccess;
   ok = ok && pages_init() == cudaSuccess;
+  ok = ok && sample_init() == cudaSuccess;
   ok = ok && cudaMalloc(&c->mmv_scratch, MMV_SCRATCH_BYTES) == cudaSuccess;
   ok = ok && cudaMemset(c->mmv_scratch, 0, MMV_SCRATCH_BYTES) == cudaSuccess;
   if (!ok) {

@@ -132,6 +132,19 @@ def test_sample_ties(ctx, settings):
 
 
 @gpu
+@pytest.mark.parametrize("vocab", [20000, 70001, 200003])
+@pytest.mark.parametrize("settings", [(1.0, 5000, None, None), (0.5, None, 0.61, None), (2.0, 9001, 0.377, 0.2), (1.0, 1, None, None),
+                                      (1.0, 700, 0.0, None)])
+def test_sample_many_ties(ctx, vocab, settings):
+    """Thousands of equal logits at the border, spread over every part of the vocabulary."""
+    rng = np.random.default_rng(vocab)
+    z = np.stack([rng.integers(-4, 4, vocab) * 0.5, np.zeros(vocab), np.where(rng.random(vocab) < 0.9, -1.0, rng.normal(0, 1, vocab)),
+                  -20.0 + 1e-6 * rng.integers(0, 3, vocab)])
+    for u in (0.0, 0.3337, 0.999):
+        check(ctx, z, np.full(len(z), u), settings)
+
+
+@gpu
 def test_sample_masked(ctx):
     """-inf, the type's lowest value, NaN and +inf among the logits; a row with nothing left; one token left."""
     rng = np.random.default_rng(2)
