@@ -10,11 +10,14 @@
 // another (maximum, histograms, sums) goes over distributed shared memory.
 // Nothing is sorted.  Tokens are ordered by (logit, lower index), each one's
 // place being one 50-bit number c, and top-k and top-p together keep c >= C.
-// C is found from a histogram over x (count and weight per bin, 1024 bins down
-// to the x whose weight is 0): the bin that holds the border token has some
-// hundred tokens in a row of 128k, which every CTA gets and ranks by
-// comparison.  A bin with more than CAP tokens (equal logits, mostly) is
-// searched by the digits of c instead.
+// C is found from a histogram over x, 1024 bins down to the x whose weight is 0:
+// counts, and for top-p weights in 16 bits (two 32-bit atomics a token; sums in
+// 64 bits there took three times as long).  That names the bin of the border
+// token; what lies above it is then summed exactly, and the bin's own tokens,
+// some hundred in a row of 128k, go to every CTA of the cluster, which ranks them
+// by comparison.  Where the exact sums disagree with the 16-bit ones the next bin
+// is taken.  A bin with more than CAP tokens (equal logits, mostly) is searched
+// by the digits of c instead.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -33,7 +36,6 @@ constexpr int WARPS = THREADS / 32;
 constexpr int MAX_CL = 8;
 constexpr int NB = 2 * THREADS;      // bins; thread t owns 2t and 2t + 1
 constexpr int CAP = 512;             // candidates that are ranked by comparison
-constexpr int SEGS = 128;            // runs of a slice whose kept weights are summed apart, 8 a warp
 constexpr float X_MIN = -27.75f;     // exp(x) * 2^40 < 1 below
 constexpr int IDX_BITS = 18;
 constexpr uint32_t IDX_MASK = (1u << IDX_BITS) - 1;
@@ -66,12 +68,21 @@ struct Scale {
     if (z == zmax) return 1.f;
     return v <= 0.f ? expf(v) : 0.f;  // NaN (a masked token at an infinite T): 0
   }
-  // Falls with z from bin 0 on.
+  // Rises as z falls, from bin 0 on; NB for a token without weight.
   __device__ __forceinline__ int bin(float z) const {
-    return z == zmax ? 0 : min(NB - 1, (int)(x(z) * (NB / X_MIN)));
+    const float v = x(z);
+    return z == zmax ? 0 : v > X_MIN ? (int)(v * (NB / X_MIN)) : NB;
   }
 };
-__device__ __forceinline__ uint64_t mass_of(float w) { return (uint64_t)(w * 1099511627776.f); }
+static_assert(X_MIN * (NB / X_MIN) <= NB, "a weight's bin is below NB");
+// floor(w * 2^40) for w in [0, 1], from its mantissa and exponent (the
+// conversion instruction for 64-bit integers runs at a fraction of the rate).
+__device__ __forceinline__ uint64_t mass_of(float w) {
+  const uint32_t u = __float_as_uint(w);
+  return ((uint64_t)((u & 0x7FFFFFu) | 0x800000u) << 17) >> min(63u, 127u - (u >> 23));
+}
+// Weights of bin b shifted by this fit 16 bits and a bit over.
+__device__ __forceinline__ int bin_shift(int b) { return max(0, 24 - ((b * 2562) >> 16)); }
 
 __device__ __forceinline__ uint64_t warp_sum64(uint64_t v) {
 #pragma unroll
@@ -130,43 +141,38 @@ __device__ __forceinline__ ulonglong2 get64x2(uint32_t a) {
   return v;
 }
 
-struct Hist {
-  unsigned long long mass[NB];
-  uint32_t cnt[NB];
-};
-
 struct Shared {
-  Hist hist, digits;
-  uint64_t cand[2][CAP];    // places and weights of the border bin's tokens (top-k's, top-p's)
-  uint64_t cand_w[2][CAP];
-  uint64_t seg[SEGS];
-  uint64_t part[WARPS];
-  uint64_t xsum[MAX_CL];
+  uint32_t cnt[NB];   // tokens of the slice per bin
+  uint32_t mass[NB];  // their weights >> bin_shift
+  union {
+    struct {  // the border bin's tokens; two lists in turn, so that one can be written while a peer reads the other
+      uint64_t place[2][CAP], mass[2][CAP];
+    } cand;
+    struct {
+      unsigned long long mass[NB];
+      uint32_t cnt[NB];
+    } digits;
+  };
+  uint64_t part[WARPS], part2[WARPS];
+  uint64_t xsum[MAX_CL], xabove[2][MAX_CL], xin[2][MAX_CL];
   uint32_t part32[WARPS];
   float xmax[MAX_CL];
   uint32_t xidx[MAX_CL];
-  // the border that one thread found
-  uint64_t border, above_mass, inside;
+  // what one thread found
+  uint64_t border, inside, above_mass;
   uint32_t above_cnt, bin, in_bin;
   uint32_t taken;
 };
 
-// Totals of a cluster's histograms at this thread's two bins, and the running
-// totals before them (bin 0 holds the largest tokens).
+// A cluster's totals at this thread's two bins (bin 0 holds the largest
+// tokens), and the running totals before them.
 struct Totals {
   uint32_t c[2], before_c;
   uint64_t m[2], before_m;
 };
 
-__device__ Totals totals(const Hist& h, uint32_t cl, Shared& s) {
+__device__ __forceinline__ void run_totals(Totals& t, Shared& s) {
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  Totals t{};
-  for (uint32_t r = 0; r < cl; ++r) {
-    const uint2 c = get32x2(peer(&h.cnt[2 * threadIdx.x], r));
-    const ulonglong2 m = get64x2(peer(&h.mass[2 * threadIdx.x], r));
-    t.c[0] += c.x, t.c[1] += c.y;
-    t.m[0] += m.x, t.m[1] += m.y;
-  }
   const uint32_t sc = warp_scan(t.c[0] + t.c[1], lane);
   const uint64_t sm = warp_scan(t.m[0] + t.m[1], lane);
   __syncthreads();
@@ -175,13 +181,12 @@ __device__ Totals totals(const Hist& h, uint32_t cl, Shared& s) {
   t.before_c = sc - t.c[0] - t.c[1];
   t.before_m = sm - t.m[0] - t.m[1];
   for (uint32_t w = 0; w < warp; ++w) t.before_c += s.part32[w], t.before_m += s.part[w];
-  return t;
 }
 
 // The bin at which the running total reaches `need`: s.bin, s.above_cnt,
 // s.above_mass, s.in_bin; s.bin == NB where it does not.
 template <bool BY_MASS>
-__device__ void find_bin(const Totals& t, uint64_t need, Shared& s) {
+__device__ __forceinline__ void find_bin(const Totals& t, uint64_t need, Shared& s) {
   __syncthreads();
   if (threadIdx.x == 0) s.bin = NB;
   __syncthreads();
@@ -197,73 +202,150 @@ __device__ void find_bin(const Totals& t, uint64_t need, Shared& s) {
   __syncthreads();
 }
 
-// The border token in the bin that find_bin left: s.border = its place, and
-// s.inside = the weight of the bin's tokens down to it.  `list`: which of the
-// two candidate lists is used.
+// The nearest bin with tokens before (step -1) or after (1) bin b: s.bin and
+// s.in_bin; s.bin == NB if there is none.
+__device__ __forceinline__ void next_bin(const Totals& t, int b, int step, Shared& s) {
+  __syncthreads();
+  if (threadIdx.x == 0) s.taken = step > 0 ? NB : 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int mine = 2 * (int)threadIdx.x + i;
+    if (t.c[i] && step > 0 && mine > b) atomicMin(&s.taken, (uint32_t)mine);
+    if (t.c[i] && step < 0 && mine < b) atomicMax(&s.taken, (uint32_t)mine + 1);
+  }
+  __syncthreads();
+  const uint32_t to = step > 0 ? s.taken : s.taken - 1;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (to == 2 * threadIdx.x + i) s.in_bin = t.c[i];
+  if (threadIdx.x == 0) s.bin = to < (uint32_t)NB ? to : NB;
+  __syncthreads();
+}
+
+struct Part {  // one CTA's part of a row
+  const float* z;
+  uint32_t n, base, rank, cl;
+  Scale sc;
+};
+
+template <typename F>
+__device__ __forceinline__ void each(const Part& p, F f) {
+  for (uint32_t i = 4 * threadIdx.x; i + 3 < p.n; i += 4 * THREADS) {
+    const float4 v = *reinterpret_cast<const float4*>(p.z + i);
+    f(i, v.x), f(i + 1, v.y), f(i + 2, v.z), f(i + 3, v.w);
+  }
+  const uint32_t i = (p.n & ~3u) + threadIdx.x;
+  if (i < p.n) f(i, p.z[i]);
+}
+
+// The border token, from s.bin of find_bin on: s.border = its place, and the
+// weight of the tokens down to it in s.inside.  need: by rank (BY_MASS false)
+// or by weight.  `turn` alternates between the candidate lists.
 template <bool BY_MASS>
-__device__ void find_border(const float* z, uint32_t n, uint32_t base, const Scale& sc, uint64_t need, int list,
-                            uint32_t rank, uint32_t cl, Shared& s) {
-  const int bin = (int)s.bin;
-  const uint64_t left = need - (BY_MASS ? s.above_mass : s.above_cnt);  // of the bin's own
-  const uint32_t m = s.in_bin;
-  if (m <= CAP) {
+__device__ void find_border(const Part& p, const Totals& t, uint64_t need, uint32_t& turn, Shared& s) {
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (;;) {
+    const int bin = (int)s.bin;
+    const uint32_t m = s.in_bin, list = turn & 1;
+    const uint64_t above_cnt = s.above_cnt;
+    ++turn;
     if (threadIdx.x == 0) {
-      uint32_t off = 0;
-      for (uint32_t r = 0; r < rank; ++r) off += get32(peer(&s.hist.cnt[bin], r));
+      uint32_t off = 0;  // of this CTA's tokens in the list
+      for (uint32_t r = 0; r < p.rank; ++r) off += get32(peer(&s.cnt[bin], r));
       s.taken = off;
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-      const float v = z[i];
-      if (sc.bin(v) != bin) continue;
-      const uint64_t w = mass_of(sc.weight(v));
-      if (w == 0) continue;
-      const uint32_t at = atomicAdd(&s.taken, 1);
-      for (uint32_t r = 0; r < cl; ++r) {
-        put64(peer(&s.cand[list][at], r), place_of(v, base + i));
-        put64(peer(&s.cand_w[list][at], r), w);
+    uint64_t above = 0, in = 0;
+    each(p, [&](uint32_t i, float v) {
+      const int b = p.sc.bin(v);
+      if (b > bin) return;
+      const uint64_t w = mass_of(p.sc.weight(v));
+      if (b < bin) {
+        above += w;
+        return;
       }
+      in += w;
+      if (m > CAP) return;
+      const uint32_t at = atomicAdd(&s.taken, 1);
+      for (uint32_t r = 0; r < p.cl; ++r) {
+        put64(peer(&s.cand.place[list][at], r), place_of(v, p.base + i));
+        put64(peer(&s.cand.mass[list][at], r), w);
+      }
+    });
+    above = warp_sum64(above);
+    in = warp_sum64(in);
+    if (lane == 0) s.part[warp] = above, s.part2[warp] = in;
+    __syncthreads();
+    if (threadIdx.x < p.cl) {
+      uint64_t x = 0, y = 0;
+      for (int w = 0; w < WARPS; ++w) x += s.part[w], y += s.part2[w];
+      put64(peer(&s.xabove[list][p.rank], threadIdx.x), x);
+      put64(peer(&s.xin[list][p.rank], threadIdx.x), y);
     }
     cl_sync();
-    if (threadIdx.x < m) {
-      const uint64_t me = s.cand[list][threadIdx.x], mine = s.cand_w[list][threadIdx.x];
-      uint64_t over = 0, over_w = 0;
-      for (uint32_t j = 0; j < m; ++j)
-        if (s.cand[list][j] > me) over += 1, over_w += s.cand_w[list][j];
-      const uint64_t o = BY_MASS ? over_w : over, own = BY_MASS ? mine : 1;
-      if (o < left && left <= o + own) s.border = me, s.inside = over_w + mine;
+    above = in = 0;
+    for (uint32_t r = 0; r < p.cl; ++r) above += s.xabove[list][r], in += s.xin[list][r];
+    if (BY_MASS && need <= above) {
+      next_bin(t, bin, -1, s);
+      continue;
+    }
+    if (BY_MASS && need > above + in) {
+      next_bin(t, bin, 1, s);
+      if (s.bin < NB) continue;
+      if (threadIdx.x == 0) s.border = 0, s.inside = above + in;  // not reached: every token stays
+      __syncthreads();
+      return;
+    }
+    const uint64_t left = BY_MASS ? need - above : need - above_cnt;  // of the bin's own
+    if (m <= CAP) {
+      if (threadIdx.x < m) {
+        const uint64_t me = s.cand.place[list][threadIdx.x], mine = s.cand.mass[list][threadIdx.x];
+        uint64_t over = 0, over_w = 0;
+        for (uint32_t j = 0; j < m; ++j)
+          if (s.cand.place[list][j] > me) over += 1, over_w += s.cand.mass[list][j];
+        const uint64_t o = BY_MASS ? over_w : over, own = BY_MASS ? mine : 1;
+        if (o < left && left <= o + own) s.border = me, s.inside = above + over_w + mine;
+      }
+      __syncthreads();
+      return;
+    }
+    // digit by digit, from the top
+    uint64_t prefix = 0, over = 0, over_w = 0;
+    for (int shift = 40; shift >= 0; shift -= 10) {
+      for (int i = threadIdx.x; i < NB; i += THREADS) s.digits.cnt[i] = 0, s.digits.mass[i] = 0;
+      __syncthreads();
+      each(p, [&](uint32_t i, float v) {
+        if (p.sc.bin(v) != bin) return;
+        const uint64_t c = place_of(v, p.base + i);
+        if ((c >> (shift + 10)) != prefix) return;
+        const uint32_t d = NB - 1 - ((uint32_t)(c >> shift) & (NB - 1));
+        atomicAdd(&s.digits.cnt[d], 1u);
+        atomicAdd(&s.digits.mass[d], (unsigned long long)mass_of(p.sc.weight(v)));
+      });
+      cl_sync();
+      Totals u{};
+      for (uint32_t r = 0; r < p.cl; ++r) {
+        const uint2 c = get32x2(peer(&s.digits.cnt[2 * threadIdx.x], r));
+        const ulonglong2 w = get64x2(peer(&s.digits.mass[2 * threadIdx.x], r));
+        u.c[0] += c.x, u.c[1] += c.y;
+        u.m[0] += w.x, u.m[1] += w.y;
+      }
+      run_totals(u, s);
+      find_bin<BY_MASS>(u, left - (BY_MASS ? over_w : over), s);
+      over += s.above_cnt;
+      over_w += s.above_mass;
+      prefix = (prefix << 10) | (NB - 1 - s.bin);
+      cl_sync();  // every CTA has read the digits
+    }
+    if (threadIdx.x == 0) {
+      s.border = prefix;
+      const uint32_t key = (uint32_t)(prefix >> IDX_BITS);
+      s.inside = above + over_w + mass_of(p.sc.weight(__uint_as_float((key & 0x80000000u) ? key & 0x7FFFFFFFu : ~key)));
     }
     __syncthreads();
     return;
   }
-  // digit by digit, from the top
-  uint64_t prefix = 0, over = 0, over_w = 0;
-  for (int shift = 40; shift >= 0; shift -= 10) {
-    for (int i = threadIdx.x; i < NB; i += THREADS) s.digits.cnt[i] = 0, s.digits.mass[i] = 0;
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-      const float v = z[i];
-      if (sc.bin(v) != bin) continue;
-      const uint64_t w = mass_of(sc.weight(v)), c = place_of(v, base + i);
-      if (w == 0 || (c >> (shift + 10)) != prefix) continue;
-      const uint32_t d = NB - 1 - ((uint32_t)(c >> shift) & (NB - 1));
-      atomicAdd(&s.digits.cnt[d], 1u);
-      atomicAdd(&s.digits.mass[d], (unsigned long long)w);
-    }
-    cl_sync();
-    const Totals t = totals(s.digits, cl, s);
-    find_bin<BY_MASS>(t, left - (BY_MASS ? over_w : over), s);
-    over += s.above_cnt;
-    over_w += s.above_mass;
-    prefix = (prefix << 10) | (NB - 1 - s.bin);
-    cl_sync();  // every CTA has read the digits
-  }
-  if (threadIdx.x == 0) {
-    s.border = prefix;
-    const uint32_t key = (uint32_t)(prefix >> IDX_BITS);
-    s.inside = over_w + mass_of(sc.weight(__uint_as_float((key & 0x80000000u) ? key & 0x7FFFFFFFu : ~key)));
-  }
-  __syncthreads();
 }
 
 template <uint32_t DT>
@@ -319,7 +401,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     if (v > m || (v == m && i < mi)) m = v, mi = i;
   }
   if (lane == 0) s.part32[warp] = mi, s.part[warp] = __float_as_uint(m);
-  for (int i = tid; i < NB; i += THREADS) s.hist.cnt[i] = 0, s.hist.mass[i] = 0;
+  for (int i = tid; i < NB; i += THREADS) s.cnt[i] = s.mass[i] = 0;
   __syncthreads();
   if (tid < cl) {  // thread r tells CTA r
     for (int w = 0; w < WARPS; ++w) {
@@ -343,7 +425,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     }
     return;
   }
-  const Scale sc{m, __frcp_rn(temp)};
+  const Part p{z, n, base, rank, cl, Scale{m, __frcp_rn(temp)}};
 
   // ---- the border of top-k and top-p ----
   uint64_t border = 0;  // tokens with a place of at least this stay
@@ -351,66 +433,74 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
   const float top_p = a.top_p ? a.top_p[row] : 1.f;
   const bool by_k = k > 0 && (uint32_t)k < a.n_vocab, by_p = top_p < 1.f;
   if (by_k || by_p) {
-    for (uint32_t i = tid; i < n; i += THREADS) {
-      const float v = z[i];
-      const uint64_t w = mass_of(sc.weight(v));
-      if (w == 0) continue;
-      const int b = sc.bin(v);
-      atomicAdd(&s.hist.cnt[b], 1u);
-      atomicAdd(&s.hist.mass[b], (unsigned long long)w);
+    uint64_t sum = 0;  // of the whole row, then of the top-k set
+    each(p, [&](uint32_t, float v) {
+      const int b = p.sc.bin(v);
+      if (b == NB) return;
+      atomicAdd(&s.cnt[b], 1u);
+      if (!by_p) return;
+      const uint64_t w = mass_of(p.sc.weight(v));
+      sum += w;
+      atomicAdd(&s.mass[b], (uint32_t)(w >> bin_shift(b)));
+    });
+    sum = warp_sum64(sum);
+    if (lane == 0) s.part2[warp] = sum;
+    __syncthreads();
+    if (tid < cl) {
+      uint64_t v = 0;
+      for (int w = 0; w < WARPS; ++w) v += s.part2[w];
+      put64(peer(&s.xsum[rank], tid), v);
     }
     cl_sync();
-    const Totals t = totals(s.hist, cl, s);
-    uint64_t sum;  // of the top-k set
-    {
-      __syncthreads();
-      if (tid == THREADS - 1) s.inside = t.before_m + t.m[0] + t.m[1];
-      __syncthreads();
-      sum = s.inside;
+    Totals t{};
+    for (uint32_t r = 0; r < cl; ++r) {
+      const uint2 c = get32x2(peer(&s.cnt[2 * tid], r)), w = get32x2(peer(&s.mass[2 * tid], r));
+      t.c[0] += c.x, t.c[1] += c.y;
+      t.m[0] += w.x, t.m[1] += w.y;
     }
+    t.m[0] <<= bin_shift(2 * tid), t.m[1] <<= bin_shift(2 * tid + 1);
+    sum = 0;
+    for (uint32_t r = 0; r < cl; ++r) sum += s.xsum[r];
+    run_totals(t, s);
+    uint32_t turn = 0;
     if (by_k) {
       find_bin<false>(t, (uint64_t)k, s);
       if (s.bin < NB) {  // else fewer than k tokens have a weight
-        find_border<false>(z, n, base, sc, (uint64_t)k, 0, rank, cl, s);
+        find_border<false>(p, t, (uint64_t)k, turn, s);
         border = s.border;
-        // find_bin's sums may have been replaced by those of the digits: the bin's own again
         sum = s.inside;
-        find_bin<false>(t, (uint64_t)k, s);
-        sum += s.above_mass;
       }
     }
     if (by_p) {
       const double need_d = ceil((double)top_p * (double)sum);
       const uint64_t need = need_d >= 1.0 ? (uint64_t)need_d : 1;
       find_bin<true>(t, need, s);
-      if (s.bin < NB) {
-        find_border<true>(z, n, base, sc, need, 1, rank, cl, s);
-        border = max(border, s.border);
-      }
+      if (s.bin == NB) next_bin(t, NB, -1, s);  // the 16-bit sums fall short: the last bin with tokens
+      find_border<true>(p, t, need, turn, s);
+      border = max(border, s.border);
     }
+    cl_sync();  // xsum is read: it is written again below
   }
   float min_p = a.min_p ? a.min_p[row] : 0.f;
   min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;  // the largest weight, 1, always stays
 
-  // ---- weights that stay, summed over runs of the slice ----
+  // ---- weights that stay: each warp sums a run of the slice ----
   const uint32_t border_key = (uint32_t)(border >> IDX_BITS), border_idx = IDX_MASK - ((uint32_t)border & IDX_MASK);
-  auto kept = [&](uint32_t i) -> uint64_t {
-    const float v = z[i];
+  auto kept = [&](uint32_t i, float v) -> uint64_t {
     const uint32_t key = key_of(v);
     if (key < border_key || (key == border_key && base + i > border_idx)) return 0;
-    const float w = sc.weight(v);
+    const float w = p.sc.weight(v);
     return w < min_p ? 0 : mass_of(w);
   };
-  const uint32_t run = (slice + SEGS - 1) / SEGS;
+  const uint32_t run = slice / WARPS;  // a multiple of 8
+  const uint32_t lo = min(n, warp * run), hi = min(n, lo + run);
   uint64_t sum = 0;
-  for (uint32_t g = warp * (SEGS / WARPS); g < (warp + 1) * (SEGS / WARPS); ++g) {
-    uint64_t v = 0;
-    for (uint32_t i = g * run + lane; i < min(n, (g + 1) * run); i += 32) v += kept(i);
-    v = warp_sum64(v);
-    if (lane == 0) s.seg[g] = v;
-    sum += v;
+  for (uint32_t i = lo + 4 * lane; i + 3 < hi; i += 128) {
+    const float4 v = *reinterpret_cast<const float4*>(z + i);
+    sum += (kept(i, v.x) + kept(i + 1, v.y)) + (kept(i + 2, v.z) + kept(i + 3, v.w));
   }
-  __syncthreads();  // part: the scans above are done with it
+  if ((hi & ~3u) + lane < hi && hi > lo) sum += kept((hi & ~3u) + lane, z[(hi & ~3u) + lane]);
+  sum = warp_sum64(sum);
   if (lane == 0) s.part[warp] = sum;
   __syncthreads();
   if (tid < cl) {
@@ -428,18 +518,23 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
   uint64_t target = uf > 0.f ? (uint64_t)fmin((double)uf * (double)total, 1.8e19) : 0;
   if (target >= total) target = total - 1;
   if (target < before || target >= before + s.xsum[rank]) return;
+  // the warp's run, split again over the warps, then the token
+  uint32_t r = 0;
+  while (before + s.part[r] <= target) before += s.part[r++];
+  const uint32_t sub = (run / WARPS + 31) / 32 * 32;
+  const uint32_t from = r * run, end = min(n, from + run);
+  const uint32_t mine = min(end, from + warp * sub), mine_end = min(end, mine + sub);
+  uint64_t v = 0;
+  for (uint32_t i = mine + lane; i < mine_end; i += 32) v += kept(i, z[i]);
+  v = warp_sum64(v);
+  if (lane == 0) s.part2[warp] = v;
+  __syncthreads();
   if (warp != 0) return;
-  // the run, then the token
-  static_assert(SEGS == 128, "4 runs a lane");
-  uint64_t c = s.seg[4 * lane] + s.seg[4 * lane + 1] + s.seg[4 * lane + 2] + s.seg[4 * lane + 3];
-  const uint64_t upto = before + warp_scan(c, lane);
-  const uint32_t lane_hit = (uint32_t)__ffs(__ballot_sync(0xffffffffu, upto > target)) - 1;
-  before = __shfl_sync(0xffffffffu, upto - c, lane_hit);
-  uint32_t g = 4 * lane_hit;
-  while (before + s.seg[g] <= target) before += s.seg[g++];
-  for (uint32_t i0 = g * run;; i0 += 32) {
+  uint32_t g = 0;
+  while (g + 1 < WARPS && before + s.part2[g] <= target) before += s.part2[g++];
+  for (uint32_t i0 = from + g * sub; i0 < end; i0 += 32) {
     const uint32_t i = i0 + lane;
-    const uint64_t w = i < min(n, (g + 1) * run) ? kept(i) : 0;
+    const uint64_t w = i < end ? kept(i, z[i]) : 0;
     const uint64_t to = before + warp_scan(w, lane);
     const uint32_t hit = __ballot_sync(0xffffffffu, to > target);
     if (hit) {
@@ -449,7 +544,6 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
       }
       return;
     }
-    if (i0 >= (g + 1) * run) return;  // not reached: the run's sum holds the target
     before = __shfl_sync(0xffffffffu, to, 31);
   }
 }
