@@ -76,9 +76,9 @@ cudaError_t pages_init();  // kernel attributes, once per device
 cudaError_t pages_assign_launch(const AssignArgs& a, cudaStream_t st);
 cudaError_t pages_release_launch(const ReleaseArgs& a, cudaStream_t st);
 cudaError_t pages_append_launch(const PagesPool& p, uint32_t n, const void* k, const void* v, uint32_t dtype,
-                                size_t row_stride, const int32_t* slots, int* err, cudaStream_t st);
+                                size_t row_stride, const int32_t* slots, int* err, int num_sms, cudaStream_t st);
 cudaError_t pages_read_launch(const PagesPool& p, uint32_t n, const int32_t* slots, float* k, float* v, int* err,
-                              cudaStream_t st);
+                              int num_sms, cudaStream_t st);
 size_t pages_attend_ws_bytes(uint32_t n_rows, uint32_t n_heads, uint32_t n_kv, uint32_t hd);
 cudaError_t pages_attend_init();
 cudaError_t pages_attend_launch(const PagesAttnArgs& a, int num_sms, cudaStream_t st);

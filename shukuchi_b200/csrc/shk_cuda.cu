@@ -971,7 +971,8 @@ int shk_cuda_pages_append(shk_ctx* c, const shk_pages* p, uint32_t n_tokens, con
   if (!k || !v || !slots || !aligned(k, es) || !aligned(v, es) || n_tokens > 0x7FFFFFFFu ||
       (row_stride && row_stride < width))
     return SHK_EINVAL;
-  CK(pages_append_launch(g, n_tokens, k, v, dtype, row_stride ? row_stride : width, slots, c->d_err, pick(c, s)));
+  CK(pages_append_launch(g, n_tokens, k, v, dtype, row_stride ? row_stride : width, slots, c->d_err, c->num_sms,
+                         pick(c, s)));
   return SHK_OK;
 }
 
@@ -983,7 +984,7 @@ int shk_cuda_pages_read(shk_ctx* c, const shk_pages* p, uint32_t n_tokens, const
   if (rc) return rc;
   if (n_tokens == 0) return SHK_OK;
   if (!k || !v || !slots || !aligned(k, 4) || !aligned(v, 4) || n_tokens > 0x7FFFFFFFu) return SHK_EINVAL;
-  CK(pages_read_launch(g, n_tokens, slots, k, v, c->d_err, pick(c, s)));
+  CK(pages_read_launch(g, n_tokens, slots, k, v, c->d_err, c->num_sms, pick(c, s)));
   return SHK_OK;
 }
 
