@@ -17,7 +17,8 @@
 // some hundred in a row of 128k, go to every CTA of the cluster, which ranks them
 // by comparison.  Where the exact sums disagree with the 16-bit ones the next bin
 // is taken.  A bin with more than CAP tokens (equal logits, mostly) is searched
-// by the digits of c instead.
+// by the digits of c instead.  Where top-k leaves few tokens, all that may stay go
+// to one CTA, which does the rest with them alone.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -48,13 +49,16 @@ __device__ __forceinline__ float logit(const void* p, size_t i) {
   if constexpr (DT == DT_F16) return __half2float(static_cast<const __half*>(p)[i]);
   return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
 }
-// As the row is held: NaN as -inf, and -0 as +0 (the two compare equal).
-__device__ __forceinline__ float clean(float z) { return z == z ? z + 0.f : -INFINITY; }
+// As the row is held: NaN as -inf.
+__device__ __forceinline__ float clean(float z) { return fmaxf(z, -INFINITY); }
 
-// Larger logits have larger keys.
+// Larger logits have larger keys; -0 and +0 compare equal and have one.
 __device__ __forceinline__ uint32_t key_of(float z) {
-  const uint32_t u = __float_as_uint(z);
+  const uint32_t u = __float_as_uint(z + 0.f);
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t key) {
+  return __uint_as_float((key & 0x80000000u) ? key & 0x7FFFFFFFu : ~key);
 }
 __device__ __forceinline__ uint64_t place_of(float z, uint32_t i) {
   return ((uint64_t)key_of(z) << IDX_BITS) | (IDX_MASK - i);
@@ -62,27 +66,39 @@ __device__ __forceinline__ uint64_t place_of(float z, uint32_t i) {
 
 struct Scale {
   float zmax, inv_t;
-  __device__ __forceinline__ float x(float z) const { return (z - zmax) * inv_t; }
-  __device__ __forceinline__ float weight(float z) const {
-    const float v = x(z);
-    if (z == zmax) return 1.f;
-    return v <= 0.f ? expf(v) : 0.f;  // NaN (a masked token at an infinite T): 0
+  bool odd;  // an infinite maximum or factor: differences and products may be NaN
+  __device__ __forceinline__ float x(float z) const {
+    float v = (z - zmax) * inv_t;
+    if (odd) v = z == zmax ? 0.f : v <= 0.f ? v : -INFINITY;
+    return v;
   }
-  // Rises as z falls, from bin 0 on; NB for a token without weight.
-  __device__ __forceinline__ int bin(float z) const {
-    const float v = x(z);
-    return z == zmax ? 0 : v > X_MIN ? (int)(v * (NB / X_MIN)) : NB;
-  }
+  __device__ __forceinline__ float weight(float z) const { return expf(x(z)); }
 };
-static_assert(X_MIN * (NB / X_MIN) <= NB, "a weight's bin is below NB");
-// floor(w * 2^40) for w in [0, 1], from its mantissa and exponent (the
-// conversion instruction for 64-bit integers runs at a fraction of the rate).
-__device__ __forceinline__ uint64_t mass_of(float w) {
-  const uint32_t u = __float_as_uint(w);
-  return ((uint64_t)((u & 0x7FFFFFu) | 0x800000u) << 17) >> min(63u, 127u - (u >> 23));
+// Rises as x falls, from bin 0 on; NB for a token without weight.
+__device__ __forceinline__ int bin_of(float x) {
+  return x > X_MIN ? (int)(__float_as_uint(__fmaf_rd(x, NB / X_MIN, 8388608.f)) - 0x4B000000u) : NB;
 }
-// Weights of bin b shifted by this fit 16 bits and a bit over.
-__device__ __forceinline__ int bin_shift(int b) { return max(0, 24 - ((b * 2562) >> 16)); }
+
+// floor(w * 2^40) for w in [0, 1] as two numbers of 20 bits, rounded down by
+// additions of 2^23 (conversions to 64-bit integers run at a fraction of their
+// rate), and sums of up to 4096 of them.
+struct Mass {
+  uint32_t hi = 0, lo = 0;
+  __device__ __forceinline__ void add(float w) {
+    const float h = __fmaf_rd(w, 1048576.f, 8388608.f);
+    const float rest = __fmaf_rn(w, 1048576.f, 8388608.f - h);  // exact
+    hi += __float_as_uint(h) - 0x4B000000u;
+    lo += __float_as_uint(__fmaf_rd(rest, 1048576.f, 8388608.f)) - 0x4B000000u;
+  }
+  __device__ __forceinline__ uint64_t value() const { return ((uint64_t)hi << 20) + lo; }
+};
+__device__ __forceinline__ uint64_t mass_of(float w) {
+  Mass m;
+  m.add(w);
+  return m.value();
+}
+// Weights of bin b times 2^(16 + bin_scale) fit 16 bits and a bit over.
+__device__ __forceinline__ int bin_scale(int b) { return min(24, (b * 2562) >> 16); }
 
 __device__ __forceinline__ uint64_t warp_sum64(uint64_t v) {
 #pragma unroll
@@ -152,6 +168,10 @@ struct Shared {
       unsigned long long mass[NB];
       uint32_t cnt[NB];
     } digits;
+    struct {  // CTA 0: all the tokens that may stay
+      uint64_t place[CAP], mass[CAP];
+      float w[CAP];
+    } few;
   };
   uint64_t part[WARPS], part2[WARPS];
   uint64_t xsum[MAX_CL], xabove[2][MAX_CL], xin[2][MAX_CL];
@@ -161,7 +181,7 @@ struct Shared {
   // what one thread found
   uint64_t border, inside, above_mass;
   uint32_t above_cnt, bin, in_bin;
-  uint32_t taken;
+  uint32_t taken, n_few;
 };
 
 // A cluster's totals at this thread's two bins (bin 0 holds the largest
@@ -256,25 +276,26 @@ __device__ void find_border(const Part& p, const Totals& t, uint64_t need, uint3
       s.taken = off;
     }
     __syncthreads();
-    uint64_t above = 0, in = 0;
+    Mass above_m, in_m;
     each(p, [&](uint32_t i, float v) {
-      const int b = p.sc.bin(v);
+      const float x = p.sc.x(v);
+      const int b = bin_of(x);
       if (b > bin) return;
-      const uint64_t w = mass_of(p.sc.weight(v));
+      const float e = expf(x);
       if (b < bin) {
-        above += w;
+        above_m.add(e);
         return;
       }
-      in += w;
+      in_m.add(e);
       if (m > CAP) return;
+      const uint64_t w = mass_of(e);
       const uint32_t at = atomicAdd(&s.taken, 1);
       for (uint32_t r = 0; r < p.cl; ++r) {
         put64(peer(&s.cand.place[list][at], r), place_of(v, p.base + i));
         put64(peer(&s.cand.mass[list][at], r), w);
       }
     });
-    above = warp_sum64(above);
-    in = warp_sum64(in);
+    uint64_t above = warp_sum64(above_m.value()), in = warp_sum64(in_m.value());
     if (lane == 0) s.part[warp] = above, s.part2[warp] = in;
     __syncthreads();
     if (threadIdx.x < p.cl) {
@@ -316,7 +337,7 @@ __device__ void find_border(const Part& p, const Totals& t, uint64_t need, uint3
       for (int i = threadIdx.x; i < NB; i += THREADS) s.digits.cnt[i] = 0, s.digits.mass[i] = 0;
       __syncthreads();
       each(p, [&](uint32_t i, float v) {
-        if (p.sc.bin(v) != bin) return;
+        if (bin_of(p.sc.x(v)) != bin) return;
         const uint64_t c = place_of(v, p.base + i);
         if ((c >> (shift + 10)) != prefix) return;
         const uint32_t d = NB - 1 - ((uint32_t)(c >> shift) & (NB - 1));
@@ -340,8 +361,7 @@ __device__ void find_border(const Part& p, const Totals& t, uint64_t need, uint3
     }
     if (threadIdx.x == 0) {
       s.border = prefix;
-      const uint32_t key = (uint32_t)(prefix >> IDX_BITS);
-      s.inside = above + over_w + mass_of(p.sc.weight(__uint_as_float((key & 0x80000000u) ? key & 0x7FFFFFFFu : ~key)));
+      s.inside = above + over_w + mass_of(p.sc.weight(value_of((uint32_t)(prefix >> IDX_BITS))));
     }
     __syncthreads();
     return;
@@ -361,10 +381,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
   constexpr int PER = DT == DT_F32 ? 4 : 8;  // logits in 16 bytes
   const uint8_t* src = static_cast<const uint8_t*>(a.logits) + ((size_t)row * a.row_stride + base) * (16 / PER);
   float m = -INFINITY;
-  uint32_t mi = 0xFFFFFFFFu;
-  auto take = [&](uint32_t i, float v) {
+  auto take = [&](float v) {
     v = clean(v);
-    if (v > m) m = v, mi = i;
+    m = fmaxf(m, v);
     return v;
   };
   uint32_t done = 0;
@@ -387,45 +406,57 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
           f = make_float4(__uint_as_float(w[e / 2] << 16), __uint_as_float(w[e / 2] & 0xFFFF0000u),
                           __uint_as_float(w[e / 2 + 1] << 16), __uint_as_float(w[e / 2 + 1] & 0xFFFF0000u));
         const uint32_t at = i * PER + e;
-        f.x = take(at, f.x), f.y = take(at + 1, f.y), f.z = take(at + 2, f.z), f.w = take(at + 3, f.w);
+        f.x = take(f.x), f.y = take(f.y), f.z = take(f.z), f.w = take(f.w);
         *reinterpret_cast<float4*>(z + at) = f;
       }
     }
   }
-  for (uint32_t i = done + tid; i < n; i += THREADS) z[i] = take(i, logit<DT>(src, i));
-  if (mi != 0xFFFFFFFFu) mi += base;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float v = __shfl_xor_sync(0xffffffffu, m, o);
-    const uint32_t i = __shfl_xor_sync(0xffffffffu, mi, o);
-    if (v > m || (v == m && i < mi)) m = v, mi = i;
-  }
-  if (lane == 0) s.part32[warp] = mi, s.part[warp] = __float_as_uint(m);
+  for (uint32_t i = done + tid; i < n; i += THREADS) z[i] = take(logit<DT>(src, i));
+  m = warp_max(m);
+  if (lane == 0) s.part32[warp] = __float_as_uint(m);
   for (int i = tid; i < NB; i += THREADS) s.cnt[i] = s.mass[i] = 0;
+  if (tid == 0) s.n_few = 0;
   __syncthreads();
   if (tid < cl) {  // thread r tells CTA r
-    for (int w = 0; w < WARPS; ++w) {
-      const float v = __uint_as_float((uint32_t)s.part[w]);
-      const uint32_t i = s.part32[w];
-      if (v > m || (v == m && i < mi)) m = v, mi = i;
-    }
+    for (int w = 0; w < WARPS; ++w) m = fmaxf(m, __uint_as_float(s.part32[w]));
     put32(peer(&s.xmax[rank], tid), __float_as_uint(m));
-    put32(peer(&s.xidx[rank], tid), mi);
   }
   cl_sync();
-  m = s.xmax[0], mi = s.xidx[0];
-  for (uint32_t r = 1; r < cl; ++r)
-    if (s.xmax[r] > m || (s.xmax[r] == m && s.xidx[r] < mi)) m = s.xmax[r], mi = s.xidx[r];
+  m = s.xmax[0];
+  for (uint32_t r = 1; r < cl; ++r) m = fmaxf(m, s.xmax[r]);
 
   const float temp = a.temperature ? a.temperature[row] : 1.f;
-  if (mi == 0xFFFFFFFFu || !(temp > 0.f)) {
-    if (rank == 0 && tid == 0) {
-      a.out[row] = mi;
-      if (a.prob) a.prob[row] = mi == 0xFFFFFFFFu ? 0.f : 1.f;
+  if (m == -INFINITY || !(temp > 0.f)) {  // nothing, or the first maximum: in the first CTA that has one
+    uint32_t r = 0;
+    while (r + 1 < cl && s.xmax[r] < m) ++r;
+    if (rank != r) return;
+    uint32_t first = 0xFFFFFFFFu;
+    if (m > -INFINITY)
+      for (uint32_t i = tid; i < n && first == 0xFFFFFFFFu; i += THREADS)
+        if (z[i] == m) first = base + i;
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0) s.part32[warp] = first;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 0; w < WARPS; ++w) first = min(first, s.part32[w]);
+      a.out[row] = first;
+      if (a.prob) a.prob[row] = m > -INFINITY ? 1.f : 0.f;
     }
     return;
   }
-  const Part p{z, n, base, rank, cl, Scale{m, __frcp_rn(temp)}};
+  const float inv_t = __frcp_rn(temp);
+  const Part p{z, n, base, rank, cl, Scale{m, inv_t, !(m < INFINITY && inv_t < INFINITY && inv_t > 0.f)}};
+  const float uf = a.u[row];
+  float min_p = a.min_p ? a.min_p[row] : 0.f;
+  min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;  // the largest weight, 1, always stays
+  auto target_of = [&](uint64_t total) {
+    const uint64_t t = uf > 0.f ? (uint64_t)fmin((double)uf * (double)total, 1.8e19) : 0;
+    return t < total ? t : total - 1;
+  };
+  auto need_of = [](float top_p, uint64_t sum) {
+    const double d = ceil((double)top_p * (double)sum);
+    return d >= 1.0 ? (uint64_t)d : 1;
+  };
 
   // ---- the border of top-k and top-p ----
   uint64_t border = 0;  // tokens with a place of at least this stay
@@ -433,35 +464,106 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
   const float top_p = a.top_p ? a.top_p[row] : 1.f;
   const bool by_k = k > 0 && (uint32_t)k < a.n_vocab, by_p = top_p < 1.f;
   if (by_k || by_p) {
+    const bool with_mass = by_p && !(by_k && k <= CAP);  // else most likely not needed, and made up for below
+    Mass sum_m;
+    auto count = [&](bool counts, bool masses) {
+      each(p, [&](uint32_t, float v) {
+        const float x = p.sc.x(v);
+        const int b = bin_of(x);
+        if (b == NB) return;
+        if (counts) atomicAdd(&s.cnt[b], 1u);
+        if (!masses) return;
+        const float w = expf(x);
+        sum_m.add(w);
+        const float scale = __uint_as_float((uint32_t)(127 + 16 + bin_scale(b)) << 23);
+        atomicAdd(&s.mass[b], __float_as_uint(__fmaf_rd(w, scale, 8388608.f)) - 0x4B000000u);
+      });
+    };
+    count(true, with_mass);
     uint64_t sum = 0;  // of the whole row, then of the top-k set
-    each(p, [&](uint32_t, float v) {
-      const int b = p.sc.bin(v);
-      if (b == NB) return;
-      atomicAdd(&s.cnt[b], 1u);
-      if (!by_p) return;
-      const uint64_t w = mass_of(p.sc.weight(v));
-      sum += w;
-      atomicAdd(&s.mass[b], (uint32_t)(w >> bin_shift(b)));
-    });
-    sum = warp_sum64(sum);
-    if (lane == 0) s.part2[warp] = sum;
-    __syncthreads();
-    if (tid < cl) {
-      uint64_t v = 0;
-      for (int w = 0; w < WARPS; ++w) v += s.part2[w];
-      put64(peer(&s.xsum[rank], tid), v);
-    }
-    cl_sync();
     Totals t{};
-    for (uint32_t r = 0; r < cl; ++r) {
-      const uint2 c = get32x2(peer(&s.cnt[2 * tid], r)), w = get32x2(peer(&s.mass[2 * tid], r));
-      t.c[0] += c.x, t.c[1] += c.y;
-      t.m[0] += w.x, t.m[1] += w.y;
+    auto gather = [&]() {
+      sum = warp_sum64(sum_m.value());
+      if (lane == 0) s.part2[warp] = sum;
+      __syncthreads();
+      if (tid < cl) {
+        uint64_t v = 0;
+        for (int w = 0; w < WARPS; ++w) v += s.part2[w];
+        put64(peer(&s.xsum[rank], tid), v);
+      }
+      cl_sync();
+      t = Totals{};
+      for (uint32_t r = 0; r < cl; ++r) {
+        const uint2 c = get32x2(peer(&s.cnt[2 * tid], r)), w = get32x2(peer(&s.mass[2 * tid], r));
+        t.c[0] += c.x, t.c[1] += c.y;
+        t.m[0] += w.x, t.m[1] += w.y;
+      }
+      t.m[0] <<= 24 - bin_scale(2 * tid), t.m[1] <<= 24 - bin_scale(2 * tid + 1);
+      sum = 0;
+      for (uint32_t r = 0; r < cl; ++r) sum += s.xsum[r];
+      run_totals(t, s);
+    };
+    gather();
+    if (by_k && k <= CAP) {
+      find_bin<false>(t, (uint64_t)k, s);
+      const uint32_t bin = s.bin, m_few = bin < NB ? s.above_cnt + s.in_bin : 0;
+      if (bin < NB && m_few <= CAP) {
+        // every token that may stay, to CTA 0
+        each(p, [&](uint32_t i, float v) {
+          const float x = p.sc.x(v);
+          if (bin_of(x) > (int)bin) return;
+          uint32_t at;
+          asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(peer(&s.n_few, 0)) : "memory");
+          const float w = expf(x);
+          put64(peer(&s.few.place[at], 0), place_of(v, base + i));
+          put64(peer(&s.few.mass[at], 0), mass_of(w));
+          put32(peer(&s.few.w[at], 0), __float_as_uint(w));
+        });
+        cl_sync();
+        if (rank != 0) return;
+        uint64_t me = 0, mine = 0, over_w = 0;
+        uint32_t over = 0;
+        if (tid < m_few) {
+          me = s.few.place[tid];
+          mine = s.few.mass[tid];
+          for (uint32_t j = 0; j < m_few; ++j)
+            if (s.few.place[j] > me) over += 1, over_w += s.few.mass[j];
+        }
+        auto block_sum = [&](uint64_t v) {
+          v = warp_sum64(v);
+          __syncthreads();
+          if (lane == 0) s.part[warp] = v;
+          __syncthreads();
+          v = 0;
+          for (int w = 0; w < WARPS; ++w) v += s.part[w];
+          return v;
+        };
+        bool stays = tid < m_few && over < (uint32_t)k;
+        if (by_p) {
+          const uint64_t need = need_of(top_p, block_sum(stays ? mine : 0));
+          stays = stays && over_w < need;
+        }
+        stays = stays && !(s.few.w[tid] < min_p);
+        mine = stays ? mine : 0;
+        const uint64_t total = block_sum(mine), target = target_of(total);
+        if (tid < m_few) s.few.mass[tid] = mine;
+        __syncthreads();
+        if (mine == 0) return;
+        uint64_t before = 0;  // of the tokens of lower index
+        for (uint32_t j = 0; j < m_few; ++j)
+          if ((s.few.place[j] & IDX_MASK) > (me & IDX_MASK)) before += s.few.mass[j];
+        if (before <= target && target < before + mine) {
+          a.out[row] = IDX_MASK - (uint32_t)(me & IDX_MASK);
+          if (a.prob) a.prob[row] = (float)((double)mine / (double)total);
+        }
+        return;
+      }
+      if (by_p) {  // too many: the weights after all
+        cl_sync();
+        count(false, true);
+        gather();
+      }
     }
-    t.m[0] <<= bin_shift(2 * tid), t.m[1] <<= bin_shift(2 * tid + 1);
-    sum = 0;
-    for (uint32_t r = 0; r < cl; ++r) sum += s.xsum[r];
-    run_totals(t, s);
     uint32_t turn = 0;
     if (by_k) {
       find_bin<false>(t, (uint64_t)k, s);
@@ -472,8 +574,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
       }
     }
     if (by_p) {
-      const double need_d = ceil((double)top_p * (double)sum);
-      const uint64_t need = need_d >= 1.0 ? (uint64_t)need_d : 1;
+      const uint64_t need = need_of(top_p, sum);
       find_bin<true>(t, need, s);
       if (s.bin == NB) next_bin(t, NB, -1, s);  // the 16-bit sums fall short: the last bin with tokens
       find_border<true>(p, t, need, turn, s);
@@ -481,26 +582,24 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     }
     cl_sync();  // xsum is read: it is written again below
   }
-  float min_p = a.min_p ? a.min_p[row] : 0.f;
-  min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;  // the largest weight, 1, always stays
-
   // ---- weights that stay: each warp sums a run of the slice ----
-  const uint32_t border_key = (uint32_t)(border >> IDX_BITS), border_idx = IDX_MASK - ((uint32_t)border & IDX_MASK);
-  auto kept = [&](uint32_t i, float v) -> uint64_t {
-    const uint32_t key = key_of(v);
-    if (key < border_key || (key == border_key && base + i > border_idx)) return 0;
+  const float border_z = border ? value_of((uint32_t)(border >> IDX_BITS)) : -INFINITY;
+  const uint32_t border_idx = IDX_MASK - ((uint32_t)border & IDX_MASK);
+  auto kept = [&](uint32_t i, float v) -> float {
+    if (v < border_z || (v == border_z && base + i > border_idx)) return 0.f;
     const float w = p.sc.weight(v);
-    return w < min_p ? 0 : mass_of(w);
+    return w < min_p ? 0.f : w;
   };
   const uint32_t run = slice / WARPS;  // a multiple of 8
   const uint32_t lo = min(n, warp * run), hi = min(n, lo + run);
-  uint64_t sum = 0;
+  Mass sum_m;
+#pragma unroll 2
   for (uint32_t i = lo + 4 * lane; i + 3 < hi; i += 128) {
     const float4 v = *reinterpret_cast<const float4*>(z + i);
-    sum += (kept(i, v.x) + kept(i + 1, v.y)) + (kept(i + 2, v.z) + kept(i + 3, v.w));
+    sum_m.add(kept(i, v.x)), sum_m.add(kept(i + 1, v.y)), sum_m.add(kept(i + 2, v.z)), sum_m.add(kept(i + 3, v.w));
   }
-  if ((hi & ~3u) + lane < hi && hi > lo) sum += kept((hi & ~3u) + lane, z[(hi & ~3u) + lane]);
-  sum = warp_sum64(sum);
+  if ((hi & ~3u) + lane < hi && hi > lo) sum_m.add(kept((hi & ~3u) + lane, z[(hi & ~3u) + lane]));
+  const uint64_t sum = warp_sum64(sum_m.value());
   if (lane == 0) s.part[warp] = sum;
   __syncthreads();
   if (tid < cl) {
@@ -514,9 +613,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     if (r == rank) before = total;
     total += s.xsum[r];
   }
-  const float uf = a.u[row];
-  uint64_t target = uf > 0.f ? (uint64_t)fmin((double)uf * (double)total, 1.8e19) : 0;
-  if (target >= total) target = total - 1;
+  const uint64_t target = target_of(total);
   if (target < before || target >= before + s.xsum[rank]) return;
   // the warp's run, split again over the warps, then the token
   uint32_t r = 0;
@@ -524,9 +621,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
   const uint32_t sub = (run / WARPS + 31) / 32 * 32;
   const uint32_t from = r * run, end = min(n, from + run);
   const uint32_t mine = min(end, from + warp * sub), mine_end = min(end, mine + sub);
-  uint64_t v = 0;
-  for (uint32_t i = mine + lane; i < mine_end; i += 32) v += kept(i, z[i]);
-  v = warp_sum64(v);
+  Mass mine_m;
+  for (uint32_t i = mine + lane; i < mine_end; i += 32) mine_m.add(kept(i, z[i]));
+  const uint64_t v = warp_sum64(mine_m.value());
   if (lane == 0) s.part2[warp] = v;
   __syncthreads();
   if (warp != 0) return;
@@ -534,7 +631,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
   while (g + 1 < WARPS && before + s.part2[g] <= target) before += s.part2[g++];
   for (uint32_t i0 = from + g * sub; i0 < end; i0 += 32) {
     const uint32_t i = i0 + lane;
-    const uint64_t w = i < end ? kept(i, z[i]) : 0;
+    const uint64_t w = i < end ? mass_of(kept(i, z[i])) : 0;
     const uint64_t to = before + warp_scan(w, lane);
     const uint32_t hit = __ballot_sync(0xffffffffu, to > target);
     if (hit) {
