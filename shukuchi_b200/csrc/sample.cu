@@ -64,12 +64,13 @@ __device__ __forceinline__ uint64_t place_of(float z, uint32_t i) {
   return ((uint64_t)key_of(z) << IDX_BITS) | (IDX_MASK - i);
 }
 
+// ODD: an infinite maximum or factor, so that differences and products may be NaN.
+template <bool ODD>
 struct Scale {
   float zmax, inv_t;
-  bool odd;  // an infinite maximum or factor: differences and products may be NaN
   __device__ __forceinline__ float x(float z) const {
-    float v = (z - zmax) * inv_t;
-    if (odd) v = z == zmax ? 0.f : v <= 0.f ? v : -INFINITY;
+    const float v = (z - zmax) * inv_t;
+    if constexpr (ODD) return z == zmax ? 0.f : v <= 0.f ? v : -INFINITY;
     return v;
   }
   __device__ __forceinline__ float weight(float z) const { return expf(x(z)); }
@@ -243,14 +244,15 @@ __device__ __forceinline__ void next_bin(const Totals& t, int b, int step, Share
   __syncthreads();
 }
 
+template <bool ODD>
 struct Part {  // one CTA's part of a row
   const float* z;
   uint32_t n, base, rank, cl;
-  Scale sc;
+  Scale<ODD> sc;
 };
 
-template <typename F>
-__device__ __forceinline__ void each(const Part& p, F f) {
+template <bool ODD, typename F>
+__device__ __forceinline__ void each(const Part<ODD>& p, F f) {
   for (uint32_t i = 4 * threadIdx.x; i + 3 < p.n; i += 4 * THREADS) {
     const float4 v = *reinterpret_cast<const float4*>(p.z + i);
     f(i, v.x), f(i + 1, v.y), f(i + 2, v.z), f(i + 3, v.w);
@@ -262,8 +264,8 @@ __device__ __forceinline__ void each(const Part& p, F f) {
 // The border token, from s.bin of find_bin on: s.border = its place, and the
 // weight of the tokens down to it in s.inside.  need: by rank (BY_MASS false)
 // or by weight.  `turn` alternates between the candidate lists.
-template <bool BY_MASS>
-__device__ void find_border(const Part& p, const Totals& t, uint64_t need, uint32_t& turn, Shared& s) {
+template <bool BY_MASS, bool ODD>
+__device__ void find_border(const Part<ODD>& p, const Totals& t, uint64_t need, uint32_t& turn, Shared& s) {
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (;;) {
     const int bin = (int)s.bin;
@@ -368,84 +370,12 @@ __device__ void find_border(const Part& p, const Totals& t, uint64_t need, uint3
   }
 }
 
-template <uint32_t DT>
-__global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constant__ SampleArgs a, uint32_t slice) {
-  extern __shared__ __align__(16) uint8_t sample_smem[];
-  float* z = reinterpret_cast<float*>(sample_smem);
-  Shared& s = *reinterpret_cast<Shared*>(sample_smem + sizeof(float) * slice);
-  const uint32_t rank = cl_rank(), cl = cl_size(), row = blockIdx.x / cl;
+// The draw, from the row's slices in shared memory and its maximum on.
+template <bool ODD>
+__device__ __forceinline__ void draw(const SampleArgs& a, const Part<ODD>& p, uint32_t row, uint32_t slice, Shared& s) {
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t base = min(a.n_vocab, rank * slice), n = min(a.n_vocab - base, slice);
-
-  // ---- the slice, and its first maximum ----
-  constexpr int PER = DT == DT_F32 ? 4 : 8;  // logits in 16 bytes
-  const uint8_t* src = static_cast<const uint8_t*>(a.logits) + ((size_t)row * a.row_stride + base) * (16 / PER);
-  float m = -INFINITY;
-  auto take = [&](float v) {
-    v = clean(v);
-    m = fmaxf(m, v);
-    return v;
-  };
-  uint32_t done = 0;
-  if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-    done = n / PER * PER;
-#pragma unroll 4
-    for (uint32_t i = tid; i < n / PER; i += THREADS) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int e = 0; e < PER; e += 4) {
-        float4 f;
-        if constexpr (DT == DT_F32)
-          f = make_float4(__uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]), __uint_as_float(w[3]));
-        else if constexpr (DT == DT_F16) {
-          const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[e / 2]));
-          const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&w[e / 2 + 1]));
-          f = make_float4(x.x, x.y, y.x, y.y);
-        } else
-          f = make_float4(__uint_as_float(w[e / 2] << 16), __uint_as_float(w[e / 2] & 0xFFFF0000u),
-                          __uint_as_float(w[e / 2 + 1] << 16), __uint_as_float(w[e / 2 + 1] & 0xFFFF0000u));
-        const uint32_t at = i * PER + e;
-        f.x = take(f.x), f.y = take(f.y), f.z = take(f.z), f.w = take(f.w);
-        *reinterpret_cast<float4*>(z + at) = f;
-      }
-    }
-  }
-  for (uint32_t i = done + tid; i < n; i += THREADS) z[i] = take(logit<DT>(src, i));
-  m = warp_max(m);
-  if (lane == 0) s.part32[warp] = __float_as_uint(m);
-  for (int i = tid; i < NB; i += THREADS) s.cnt[i] = s.mass[i] = 0;
-  if (tid == 0) s.n_few = 0;
-  __syncthreads();
-  if (tid < cl) {  // thread r tells CTA r
-    for (int w = 0; w < WARPS; ++w) m = fmaxf(m, __uint_as_float(s.part32[w]));
-    put32(peer(&s.xmax[rank], tid), __float_as_uint(m));
-  }
-  cl_sync();
-  m = s.xmax[0];
-  for (uint32_t r = 1; r < cl; ++r) m = fmaxf(m, s.xmax[r]);
-
-  const float temp = a.temperature ? a.temperature[row] : 1.f;
-  if (m == -INFINITY || !(temp > 0.f)) {  // nothing, or the first maximum: in the first CTA that has one
-    uint32_t r = 0;
-    while (r + 1 < cl && s.xmax[r] < m) ++r;
-    if (rank != r) return;
-    uint32_t first = 0xFFFFFFFFu;
-    if (m > -INFINITY)
-      for (uint32_t i = tid; i < n && first == 0xFFFFFFFFu; i += THREADS)
-        if (z[i] == m) first = base + i;
-    first = __reduce_min_sync(0xffffffffu, first);
-    if (lane == 0) s.part32[warp] = first;
-    __syncthreads();
-    if (tid == 0) {
-      for (int w = 0; w < WARPS; ++w) first = min(first, s.part32[w]);
-      a.out[row] = first;
-      if (a.prob) a.prob[row] = m > -INFINITY ? 1.f : 0.f;
-    }
-    return;
-  }
-  const float inv_t = __frcp_rn(temp);
-  const Part p{z, n, base, rank, cl, Scale{m, inv_t, !(m < INFINITY && inv_t < INFINITY && inv_t > 0.f)}};
+  const uint32_t n = p.n, base = p.base, rank = p.rank, cl = p.cl;
+  const float* z = p.z;
   const float uf = a.u[row];
   float min_p = a.min_p ? a.min_p[row] : 0.f;
   min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;  // the largest weight, 1, always stays
@@ -568,7 +498,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     if (by_k) {
       find_bin<false>(t, (uint64_t)k, s);
       if (s.bin < NB) {  // else fewer than k tokens have a weight
-        find_border<false>(p, t, (uint64_t)k, turn, s);
+        find_border<false, ODD>(p, t, (uint64_t)k, turn, s);
         border = s.border;
         sum = s.inside;
       }
@@ -577,7 +507,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
       const uint64_t need = need_of(top_p, sum);
       find_bin<true>(t, need, s);
       if (s.bin == NB) next_bin(t, NB, -1, s);  // the 16-bit sums fall short: the last bin with tokens
-      find_border<true>(p, t, need, turn, s);
+      find_border<true, ODD>(p, t, need, turn, s);
       border = max(border, s.border);
     }
     cl_sync();  // xsum is read: it is written again below
@@ -643,6 +573,89 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     }
     before = __shfl_sync(0xffffffffu, to, 31);
   }
+}
+
+template <uint32_t DT>
+__global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constant__ SampleArgs a, uint32_t slice) {
+  extern __shared__ __align__(16) uint8_t sample_smem[];
+  float* z = reinterpret_cast<float*>(sample_smem);
+  Shared& s = *reinterpret_cast<Shared*>(sample_smem + sizeof(float) * slice);
+  const uint32_t rank = cl_rank(), cl = cl_size(), row = blockIdx.x / cl;
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t base = min(a.n_vocab, rank * slice), n = min(a.n_vocab - base, slice);
+
+  // ---- the slice, and its first maximum ----
+  constexpr int PER = DT == DT_F32 ? 4 : 8;  // logits in 16 bytes
+  const uint8_t* src = static_cast<const uint8_t*>(a.logits) + ((size_t)row * a.row_stride + base) * (16 / PER);
+  float m = -INFINITY;
+  auto take = [&](float v) {
+    v = clean(v);
+    m = fmaxf(m, v);
+    return v;
+  };
+  uint32_t done = 0;
+  if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+    done = n / PER * PER;
+#pragma unroll 4
+    for (uint32_t i = tid; i < n / PER; i += THREADS) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < PER; e += 4) {
+        float4 f;
+        if constexpr (DT == DT_F32)
+          f = make_float4(__uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]), __uint_as_float(w[3]));
+        else if constexpr (DT == DT_F16) {
+          const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[e / 2]));
+          const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&w[e / 2 + 1]));
+          f = make_float4(x.x, x.y, y.x, y.y);
+        } else
+          f = make_float4(__uint_as_float(w[e / 2] << 16), __uint_as_float(w[e / 2] & 0xFFFF0000u),
+                          __uint_as_float(w[e / 2 + 1] << 16), __uint_as_float(w[e / 2 + 1] & 0xFFFF0000u));
+        const uint32_t at = i * PER + e;
+        f.x = take(f.x), f.y = take(f.y), f.z = take(f.z), f.w = take(f.w);
+        *reinterpret_cast<float4*>(z + at) = f;
+      }
+    }
+  }
+  for (uint32_t i = done + tid; i < n; i += THREADS) z[i] = take(logit<DT>(src, i));
+  m = warp_max(m);
+  if (lane == 0) s.part32[warp] = __float_as_uint(m);
+  for (int i = tid; i < NB; i += THREADS) s.cnt[i] = s.mass[i] = 0;
+  if (tid == 0) s.n_few = 0;
+  __syncthreads();
+  if (tid < cl) {  // thread r tells CTA r
+    for (int w = 0; w < WARPS; ++w) m = fmaxf(m, __uint_as_float(s.part32[w]));
+    put32(peer(&s.xmax[rank], tid), __float_as_uint(m));
+  }
+  cl_sync();
+  m = s.xmax[0];
+  for (uint32_t r = 1; r < cl; ++r) m = fmaxf(m, s.xmax[r]);
+
+  const float temp = a.temperature ? a.temperature[row] : 1.f;
+  if (m == -INFINITY || !(temp > 0.f)) {  // nothing, or the first maximum: in the first CTA that has one
+    uint32_t r = 0;
+    while (r + 1 < cl && s.xmax[r] < m) ++r;
+    if (rank != r) return;
+    uint32_t first = 0xFFFFFFFFu;
+    if (m > -INFINITY)
+      for (uint32_t i = tid; i < n && first == 0xFFFFFFFFu; i += THREADS)
+        if (z[i] == m) first = base + i;
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0) s.part32[warp] = first;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 0; w < WARPS; ++w) first = min(first, s.part32[w]);
+      a.out[row] = first;
+      if (a.prob) a.prob[row] = m > -INFINITY ? 1.f : 0.f;
+    }
+    return;
+  }
+  const float inv_t = __frcp_rn(temp);
+  if (m < INFINITY && inv_t < INFINITY && inv_t > 0.f)
+    draw(a, Part<false>{z, n, base, rank, cl, {m, inv_t}}, row, slice, s);
+  else
+    draw(a, Part<true>{z, n, base, rank, cl, {m, inv_t}}, row, slice, s);
 }
 
 template <uint32_t DT>
