@@ -10,15 +10,18 @@
 // another (maximum, histograms, sums) goes over distributed shared memory.
 // Nothing is sorted.  Tokens are ordered by (logit, lower index), each one's
 // place being one 50-bit number c, and top-k and top-p together keep c >= C.
-// C is found from a histogram over x, 1024 bins down to the x whose weight is 0:
-// counts, and for top-p weights in 16 bits (two 32-bit atomics a token; sums in
-// 64 bits there took three times as long).  That names the bin of the border
-// token; what lies above it is then summed exactly, and the bin's own tokens,
-// some hundred in a row of 128k, go to every CTA of the cluster, which ranks them
-// by comparison.  Where the exact sums disagree with the 16-bit ones the next bin
+// C is found from a histogram over x, 2048 bins down to the x whose weight is 0:
+// of counts for top-k, of weights in 16 bits for top-p (one 32-bit atomic a token;
+// sums in 64 bits there took three times as long).  That names the bin of the
+// border token; what lies above it is then summed exactly, and the bin's own
+// tokens, a hundred or so in a row of 128k, go to every CTA of the cluster, which
+// ranks them by comparison.  Where the exact sums disagree with the 16-bit ones the next bin
 // is taken.  A bin with more than CAP tokens (equal logits, mostly) is searched
-// by the digits of c instead.  Where top-k leaves few tokens, all that may stay go
-// to one CTA, which does the rest with them alone.
+// by the digits of c instead.
+//
+// A small top-k takes a shorter way: the k-th largest of the threads' own maxima
+// is at most the k-th largest logit, so the tokens from its bin up, not many more
+// than k, go to one CTA, which does the rest with them alone.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -35,7 +38,9 @@ namespace {
 constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
 constexpr int MAX_CL = 8;
-constexpr int NB = 2 * THREADS;      // bins; thread t owns 2t and 2t + 1
+constexpr int OWN = 4;               // bins a thread: 16 bytes of a peer's histogram, whole lines to a warp
+constexpr int NB = OWN * THREADS;
+constexpr int DIGITS = 2 * THREADS;  // of the search by digits, 10 bits each
 constexpr int CAP = 512;             // candidates that are ranked by comparison
 constexpr float X_MIN = -27.75f;     // exp(x) * 2^40 < 1 below
 constexpr int IDX_BITS = 18;
@@ -99,7 +104,7 @@ __device__ __forceinline__ uint64_t mass_of(float w) {
   return m.value();
 }
 // Weights of bin b times 2^(16 + bin_scale) fit 16 bits and a bit over.
-__device__ __forceinline__ int bin_scale(int b) { return min(24, (b * 2562) >> 16); }
+__device__ __forceinline__ int bin_scale(int b) { return min(24, (b * 1281) >> 16); }
 
 __device__ __forceinline__ uint64_t warp_sum64(uint64_t v) {
 #pragma unroll
@@ -142,9 +147,9 @@ __device__ __forceinline__ void put32(uint32_t a, uint32_t v) {
 __device__ __forceinline__ void put64(uint32_t a, uint64_t v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
 }
-__device__ __forceinline__ uint32_t get32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+__device__ __forceinline__ uint4 get32x4(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
   return v;
 }
 __device__ __forceinline__ uint2 get32x2(uint32_t a) {
@@ -159,15 +164,14 @@ __device__ __forceinline__ ulonglong2 get64x2(uint32_t a) {
 }
 
 struct Shared {
-  uint32_t cnt[NB];   // tokens of the slice per bin
-  uint32_t mass[NB];  // their weights >> bin_shift
+  uint32_t hist[NB];  // of the slice's tokens: how many, or their weights times 2^(16 + bin_scale)
   union {
     struct {  // the border bin's tokens; two lists in turn, so that one can be written while a peer reads the other
       uint64_t place[2][CAP], mass[2][CAP];
     } cand;
     struct {
-      unsigned long long mass[NB];
-      uint32_t cnt[NB];
+      unsigned long long mass[DIGITS];
+      uint32_t cnt[DIGITS];
     } digits;
     struct {  // CTA 0: all the tokens that may stay
       uint64_t place[CAP], mass[CAP];
@@ -175,72 +179,73 @@ struct Shared {
     } few;
   };
   uint64_t part[WARPS], part2[WARPS];
+  unsigned long long kept[WARPS];  // weights that stay of each warp's run
   uint64_t xsum[MAX_CL], xabove[2][MAX_CL], xin[2][MAX_CL];
-  uint32_t part32[WARPS];
+  uint32_t part32[WARPS], xcnt[2][MAX_CL];
   float xmax[MAX_CL];
-  uint32_t xidx[MAX_CL];
   // what one thread found
-  uint64_t border, inside, above_mass;
-  uint32_t above_cnt, bin, in_bin;
-  uint32_t taken, n_few;
+  uint64_t border, inside, above, above_mass;
+  uint32_t bin;
+  uint32_t next[3];  // CTA 0: places given out in the lists, three counters in turn
+  uint32_t own;      // tokens of this CTA in the list
 };
 
-// A cluster's totals at this thread's two bins (bin 0 holds the largest
-// tokens), and the running totals before them.
+__device__ __forceinline__ uint32_t take_place(uint32_t* counter) {  // of CTA 0's copy
+  uint32_t at;
+  asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(peer(counter, 0)) : "memory");
+  return at;
+}
+
+// A cluster's totals at this thread's bins (bin 0 holds the largest tokens),
+// and the running total before them.
+template <int N>
 struct Totals {
-  uint32_t c[2], before_c;
-  uint64_t m[2], before_m;
+  uint64_t v[N], before;
 };
 
-__device__ __forceinline__ void run_totals(Totals& t, Shared& s) {
+template <int N>
+__device__ __forceinline__ void run_totals(Totals<N>& t, uint64_t* part) {
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t sc = warp_scan(t.c[0] + t.c[1], lane);
-  const uint64_t sm = warp_scan(t.m[0] + t.m[1], lane);
+  uint64_t own = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) own += t.v[i];
+  const uint64_t upto = warp_scan(own, lane);
   __syncthreads();
-  if (lane == 31) s.part32[warp] = sc, s.part[warp] = sm;
+  if (lane == 31) part[warp] = upto;
   __syncthreads();
-  t.before_c = sc - t.c[0] - t.c[1];
-  t.before_m = sm - t.m[0] - t.m[1];
-  for (uint32_t w = 0; w < warp; ++w) t.before_c += s.part32[w], t.before_m += s.part[w];
+  t.before = upto - own;
+  for (uint32_t w = 0; w < warp; ++w) t.before += part[w];
 }
 
-// The bin at which the running total reaches `need`: s.bin, s.above_cnt,
-// s.above_mass, s.in_bin; s.bin == NB where it does not.
-template <bool BY_MASS>
-__device__ __forceinline__ void find_bin(const Totals& t, uint64_t need, Shared& s) {
+// The bin at which the running total reaches `need` (s.bin; N * THREADS where it
+// does not) and the total before it (s.above).
+template <int N>
+__device__ __forceinline__ void find_bin(const Totals<N>& t, uint64_t need, Shared& s) {
   __syncthreads();
-  if (threadIdx.x == 0) s.bin = NB;
+  if (threadIdx.x == 0) s.bin = N * THREADS;
   __syncthreads();
-  uint32_t c = t.before_c;
-  uint64_t m = t.before_m;
+  uint64_t c = t.before;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint64_t lo = BY_MASS ? m : c, hi = BY_MASS ? m + t.m[i] : c + t.c[i];
-    if (lo < need && need <= hi) s.bin = 2 * threadIdx.x + i, s.above_cnt = c, s.above_mass = m, s.in_bin = t.c[i];
-    c += t.c[i];
-    m += t.m[i];
+  for (int i = 0; i < N; ++i) {
+    if (c < need && need <= c + t.v[i]) s.bin = N * threadIdx.x + i, s.above = c;
+    c += t.v[i];
   }
   __syncthreads();
 }
 
-// The nearest bin with tokens before (step -1) or after (1) bin b: s.bin and
-// s.in_bin; s.bin == NB if there is none.
-__device__ __forceinline__ void next_bin(const Totals& t, int b, int step, Shared& s) {
+// The nearest bin with tokens before (step -1) or after (1) bin b to s.bin; NB if there is none.
+__device__ __forceinline__ void next_bin(const Totals<OWN>& t, int b, int step, Shared& s) {
   __syncthreads();
-  if (threadIdx.x == 0) s.taken = step > 0 ? NB : 0;
+  if (threadIdx.x == 0) s.own = step > 0 ? NB : 0;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int mine = 2 * (int)threadIdx.x + i;
-    if (t.c[i] && step > 0 && mine > b) atomicMin(&s.taken, (uint32_t)mine);
-    if (t.c[i] && step < 0 && mine < b) atomicMax(&s.taken, (uint32_t)mine + 1);
+  for (int i = 0; i < OWN; ++i) {
+    const int mine = OWN * (int)threadIdx.x + i;
+    if (t.v[i] && step > 0 && mine > b) atomicMin(&s.own, (uint32_t)mine);
+    if (t.v[i] && step < 0 && mine < b) atomicMax(&s.own, (uint32_t)mine + 1);
   }
   __syncthreads();
-  const uint32_t to = step > 0 ? s.taken : s.taken - 1;
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (to == 2 * threadIdx.x + i) s.in_bin = t.c[i];
-  if (threadIdx.x == 0) s.bin = to < (uint32_t)NB ? to : NB;
+  if (threadIdx.x == 0) s.bin = step > 0 ? s.own : s.own ? s.own - 1 : NB;
   __syncthreads();
 }
 
@@ -248,7 +253,9 @@ template <bool ODD>
 struct Part {  // one CTA's part of a row
   const float* z;
   uint32_t n, base, rank, cl;
+  uint32_t run;  // of a warp, a multiple of 4
   Scale<ODD> sc;
+  float min_p;
 };
 
 template <bool ODD, typename F>
@@ -261,54 +268,75 @@ __device__ __forceinline__ void each(const Part<ODD>& p, F f) {
   if (i < p.n) f(i, p.z[i]);
 }
 
+// Each warp over its run of the slice.
+template <bool ODD, typename F>
+__device__ __forceinline__ void each_of_run(const Part<ODD>& p, F f) {
+  const uint32_t lane = threadIdx.x & 31;
+  const uint32_t lo = min(p.n, (threadIdx.x >> 5) * p.run), hi = min(p.n, lo + p.run);
+#pragma unroll 2
+  for (uint32_t i = lo + 4 * lane; i + 3 < hi; i += 128) {
+    const float4 v = *reinterpret_cast<const float4*>(p.z + i);
+    f(i, v.x), f(i + 1, v.y), f(i + 2, v.z), f(i + 3, v.w);
+  }
+  const uint32_t i = (hi & ~3u) + lane;
+  if (i < hi && hi > lo) f(i, p.z[i]);
+}
+
 // The border token, from s.bin of find_bin on: s.border = its place, and the
 // weight of the tokens down to it in s.inside.  need: by rank (BY_MASS false)
-// or by weight.  `turn` alternates between the candidate lists.
+// or by weight.  `turn` alternates between the candidate lists.  Returns whether
+// s.kept has the weights that stay of each warp's run (it has not where the
+// digits were searched).
 template <bool BY_MASS, bool ODD>
-__device__ void find_border(const Part<ODD>& p, const Totals& t, uint64_t need, uint32_t& turn, Shared& s) {
+__device__ bool find_border(const Part<ODD>& p, const Totals<OWN>& t, uint64_t need, uint32_t& turn, Shared& s) {
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (;;) {
     const int bin = (int)s.bin;
-    const uint32_t m = s.in_bin, list = turn & 1;
-    const uint64_t above_cnt = s.above_cnt;
-    ++turn;
+    const uint32_t list = turn & 1;
+    uint32_t* place = &s.next[turn % 3];
+    const uint64_t above_cnt = s.above;
     if (threadIdx.x == 0) {
-      uint32_t off = 0;  // of this CTA's tokens in the list
-      for (uint32_t r = 0; r < p.rank; ++r) off += get32(peer(&s.cnt[bin], r));
-      s.taken = off;
+      s.own = 0;
+      s.next[(turn + 1) % 3] = 0;  // last used two turns ago
     }
+    ++turn;
     __syncthreads();
-    Mass above_m, in_m;
-    each(p, [&](uint32_t i, float v) {
+    Mass above_m, in_m, kept_m;
+    each_of_run(p, [&](uint32_t i, float v) {
       const float x = p.sc.x(v);
       const int b = bin_of(x);
       if (b > bin) return;
       const float e = expf(x);
       if (b < bin) {
         above_m.add(e);
+        if (p.min_p > 0.f && e >= p.min_p) kept_m.add(e);
         return;
       }
       in_m.add(e);
-      if (m > CAP) return;
+      atomicAdd(&s.own, 1u);
+      const uint32_t at = take_place(place);
+      if (at >= CAP) return;
       const uint64_t w = mass_of(e);
-      const uint32_t at = atomicAdd(&s.taken, 1);
       for (uint32_t r = 0; r < p.cl; ++r) {
         put64(peer(&s.cand.place[list][at], r), place_of(v, p.base + i));
         put64(peer(&s.cand.mass[list][at], r), w);
       }
     });
     uint64_t above = warp_sum64(above_m.value()), in = warp_sum64(in_m.value());
-    if (lane == 0) s.part[warp] = above, s.part2[warp] = in;
+    const uint64_t kept = p.min_p > 0.f ? warp_sum64(kept_m.value()) : above;
+    if (lane == 0) s.part[warp] = above, s.part2[warp] = in, s.kept[warp] = kept;
     __syncthreads();
     if (threadIdx.x < p.cl) {
       uint64_t x = 0, y = 0;
       for (int w = 0; w < WARPS; ++w) x += s.part[w], y += s.part2[w];
       put64(peer(&s.xabove[list][p.rank], threadIdx.x), x);
       put64(peer(&s.xin[list][p.rank], threadIdx.x), y);
+      put32(peer(&s.xcnt[list][p.rank], threadIdx.x), s.own);
     }
     cl_sync();
     above = in = 0;
-    for (uint32_t r = 0; r < p.cl; ++r) above += s.xabove[list][r], in += s.xin[list][r];
+    uint32_t m = 0;
+    for (uint32_t r = 0; r < p.cl; ++r) above += s.xabove[list][r], in += s.xin[list][r], m += s.xcnt[list][r];
     if (BY_MASS && need <= above) {
       next_bin(t, bin, -1, s);
       continue;
@@ -318,7 +346,7 @@ __device__ void find_border(const Part<ODD>& p, const Totals& t, uint64_t need, 
       if (s.bin < NB) continue;
       if (threadIdx.x == 0) s.border = 0, s.inside = above + in;  // not reached: every token stays
       __syncthreads();
-      return;
+      return false;
     }
     const uint64_t left = BY_MASS ? need - above : need - above_cnt;  // of the bin's own
     if (m <= CAP) {
@@ -331,34 +359,45 @@ __device__ void find_border(const Part<ODD>& p, const Totals& t, uint64_t need, 
         if (o < left && left <= o + own) s.border = me, s.inside = above + over_w + mine;
       }
       __syncthreads();
-      return;
+      if (threadIdx.x < m) {  // the bin's tokens that stay, to the runs of this slice
+        const uint64_t me = s.cand.place[list][threadIdx.x];
+        const uint32_t i = IDX_MASK - (uint32_t)(me & IDX_MASK) - p.base;  // huge where it is before the slice
+        if (me >= s.border && i < p.n && !(p.sc.weight(value_of((uint32_t)(me >> IDX_BITS))) < p.min_p))
+          atomicAdd(&s.kept[i / p.run], (unsigned long long)s.cand.mass[list][threadIdx.x]);
+      }
+      __syncthreads();
+      return true;
     }
     // digit by digit, from the top
     uint64_t prefix = 0, over = 0, over_w = 0;
     for (int shift = 40; shift >= 0; shift -= 10) {
-      for (int i = threadIdx.x; i < NB; i += THREADS) s.digits.cnt[i] = 0, s.digits.mass[i] = 0;
+      for (int i = threadIdx.x; i < DIGITS; i += THREADS) s.digits.cnt[i] = 0, s.digits.mass[i] = 0;
       __syncthreads();
       each(p, [&](uint32_t i, float v) {
         if (bin_of(p.sc.x(v)) != bin) return;
         const uint64_t c = place_of(v, p.base + i);
         if ((c >> (shift + 10)) != prefix) return;
-        const uint32_t d = NB - 1 - ((uint32_t)(c >> shift) & (NB - 1));
+        const uint32_t d = DIGITS - 1 - ((uint32_t)(c >> shift) & (DIGITS - 1));
         atomicAdd(&s.digits.cnt[d], 1u);
         atomicAdd(&s.digits.mass[d], (unsigned long long)mass_of(p.sc.weight(v)));
       });
       cl_sync();
-      Totals u{};
+      Totals<2> c{}, w{};
       for (uint32_t r = 0; r < p.cl; ++r) {
-        const uint2 c = get32x2(peer(&s.digits.cnt[2 * threadIdx.x], r));
-        const ulonglong2 w = get64x2(peer(&s.digits.mass[2 * threadIdx.x], r));
-        u.c[0] += c.x, u.c[1] += c.y;
-        u.m[0] += w.x, u.m[1] += w.y;
+        const uint2 x = get32x2(peer(&s.digits.cnt[2 * threadIdx.x], r));
+        const ulonglong2 y = get64x2(peer(&s.digits.mass[2 * threadIdx.x], r));
+        c.v[0] += x.x, c.v[1] += x.y;
+        w.v[0] += y.x, w.v[1] += y.y;
       }
-      run_totals(u, s);
-      find_bin<BY_MASS>(u, left - (BY_MASS ? over_w : over), s);
-      over += s.above_cnt;
+      run_totals(c, s.part);
+      run_totals(w, s.part2);
+      find_bin(BY_MASS ? w : c, left - (BY_MASS ? over_w : over), s);
+      const uint32_t d = s.bin;
+      if (d / 2 == threadIdx.x) s.above = c.before + (d & 1 ? c.v[0] : 0), s.above_mass = w.before + (d & 1 ? w.v[0] : 0);
+      __syncthreads();
+      over += s.above;
       over_w += s.above_mass;
-      prefix = (prefix << 10) | (NB - 1 - s.bin);
+      prefix = (prefix << 10) | (DIGITS - 1 - d);
       cl_sync();  // every CTA has read the digits
     }
     if (threadIdx.x == 0) {
@@ -366,19 +405,18 @@ __device__ void find_border(const Part<ODD>& p, const Totals& t, uint64_t need, 
       s.inside = above + over_w + mass_of(p.sc.weight(value_of((uint32_t)(prefix >> IDX_BITS))));
     }
     __syncthreads();
-    return;
+    return false;
   }
 }
 
 // The draw, from the row's slices in shared memory and its maximum on.
 template <bool ODD>
-__device__ __forceinline__ void draw(const SampleArgs& a, const Part<ODD>& p, uint32_t row, uint32_t slice, Shared& s) {
+__device__ __forceinline__ void draw(const SampleArgs& a, const Part<ODD>& p, uint32_t row, float own_max, Shared& s) {
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t n = p.n, base = p.base, rank = p.rank, cl = p.cl;
   const float* z = p.z;
   const float uf = a.u[row];
-  float min_p = a.min_p ? a.min_p[row] : 0.f;
-  min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;  // the largest weight, 1, always stays
+  const float min_p = p.min_p;
   auto target_of = [&](uint64_t total) {
     const uint64_t t = uf > 0.f ? (uint64_t)fmin((double)uf * (double)total, 1.8e19) : 0;
     return t < total ? t : total - 1;
@@ -390,31 +428,16 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Part<ODD>& p, ui
 
   // ---- the border of top-k and top-p ----
   uint64_t border = 0;  // tokens with a place of at least this stay
+  bool summed = false;  // s.kept has their weights
   const int32_t k = a.top_k ? a.top_k[row] : 0;
   const float top_p = a.top_p ? a.top_p[row] : 1.f;
   const bool by_k = k > 0 && (uint32_t)k < a.n_vocab, by_p = top_p < 1.f;
   if (by_k || by_p) {
-    const bool with_mass = by_p && !(by_k && k <= CAP);  // else most likely not needed, and made up for below
-    Mass sum_m;
-    auto count = [&](bool counts, bool masses) {
-      each(p, [&](uint32_t, float v) {
-        const float x = p.sc.x(v);
-        const int b = bin_of(x);
-        if (b == NB) return;
-        if (counts) atomicAdd(&s.cnt[b], 1u);
-        if (!masses) return;
-        const float w = expf(x);
-        sum_m.add(w);
-        const float scale = __uint_as_float((uint32_t)(127 + 16 + bin_scale(b)) << 23);
-        atomicAdd(&s.mass[b], __float_as_uint(__fmaf_rd(w, scale, 8388608.f)) - 0x4B000000u);
-      });
-    };
-    count(true, with_mass);
     uint64_t sum = 0;  // of the whole row, then of the top-k set
-    Totals t{};
-    auto gather = [&]() {
-      sum = warp_sum64(sum_m.value());
-      if (lane == 0) s.part2[warp] = sum;
+    Totals<OWN> t{};
+    auto gather = [&](bool masses, uint64_t mine) {  // the cluster's histogram, and the sum of what each thread has
+      mine = warp_sum64(mine);
+      if (lane == 0) s.part2[warp] = mine;
       __syncthreads();
       if (tid < cl) {
         uint64_t v = 0;
@@ -422,34 +445,48 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Part<ODD>& p, ui
         put64(peer(&s.xsum[rank], tid), v);
       }
       cl_sync();
-      t = Totals{};
+      t = Totals<OWN>{};
       for (uint32_t r = 0; r < cl; ++r) {
-        const uint2 c = get32x2(peer(&s.cnt[2 * tid], r)), w = get32x2(peer(&s.mass[2 * tid], r));
-        t.c[0] += c.x, t.c[1] += c.y;
-        t.m[0] += w.x, t.m[1] += w.y;
+        const uint4 c = get32x4(peer(&s.hist[OWN * tid], r));
+        t.v[0] += c.x, t.v[1] += c.y, t.v[2] += c.z, t.v[3] += c.w;
       }
-      t.m[0] <<= 24 - bin_scale(2 * tid), t.m[1] <<= 24 - bin_scale(2 * tid + 1);
-      sum = 0;
-      for (uint32_t r = 0; r < cl; ++r) sum += s.xsum[r];
-      run_totals(t, s);
+      if (masses)
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) t.v[i] <<= 24 - bin_scale(OWN * tid + i);
+      mine = 0;
+      for (uint32_t r = 0; r < cl; ++r) mine += s.xsum[r];
+      run_totals(t, s.part);
+      return mine;
     };
-    gather();
+    auto clear = [&]() {  // the histogram, once every CTA has read it
+      cl_sync();
+      for (int i = tid; i < NB; i += THREADS) s.hist[i] = 0;
+      __syncthreads();
+    };
     if (by_k && k <= CAP) {
-      find_bin<false>(t, (uint64_t)k, s);
-      const uint32_t bin = s.bin, m_few = bin < NB ? s.above_cnt + s.in_bin : 0;
-      if (bin < NB && m_few <= CAP) {
-        // every token that may stay, to CTA 0
-        each(p, [&](uint32_t i, float v) {
-          const float x = p.sc.x(v);
-          if (bin_of(x) > (int)bin) return;
-          uint32_t at;
-          asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(peer(&s.n_few, 0)) : "memory");
-          const float w = expf(x);
-          put64(peer(&s.few.place[at], 0), place_of(v, base + i));
-          put64(peer(&s.few.mass[at], 0), mass_of(w));
-          put32(peer(&s.few.w[at], 0), __float_as_uint(w));
-        });
-        cl_sync();
+      // the bin of the k-th largest of the threads' maxima: k tokens at least are in it or above
+      const int own_bin = bin_of(p.sc.x(own_max));
+      if (own_bin < NB) atomicAdd(&s.hist[own_bin], 1u);
+      gather(false, 0);
+      find_bin(t, (uint64_t)k, s);
+      const int bin = min((int)s.bin, NB - 1);  // else every token with a weight may stay
+      each(p, [&](uint32_t i, float v) {
+        const float x = p.sc.x(v);
+        if (bin_of(x) > bin) return;
+        atomicAdd(&s.own, 1u);
+        const uint32_t at = take_place(&s.next[2]);
+        if (at >= CAP) return;
+        const float w = expf(x);
+        put64(peer(&s.few.place[at], 0), place_of(v, base + i));
+        put64(peer(&s.few.mass[at], 0), mass_of(w));
+        put32(peer(&s.few.w[at], 0), __float_as_uint(w));
+      });
+      __syncthreads();
+      if (tid < cl) put32(peer(&s.xcnt[0][rank], tid), s.own);
+      cl_sync();
+      uint32_t m_few = 0;  // (from here on no CTA touches another's memory: all but CTA 0 may leave)
+      for (uint32_t r = 0; r < cl; ++r) m_few += s.xcnt[0][r];
+      if (m_few <= CAP) {
         if (rank != 0) return;
         uint64_t me = 0, mine = 0, over_w = 0;
         uint32_t over = 0;
@@ -488,26 +525,39 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Part<ODD>& p, ui
         }
         return;
       }
-      if (by_p) {  // too many: the weights after all
-        cl_sync();
-        count(false, true);
-        gather();
-      }
+      clear();  // more than fit: as with a large k
     }
     uint32_t turn = 0;
     if (by_k) {
-      find_bin<false>(t, (uint64_t)k, s);
+      each(p, [&](uint32_t, float v) {
+        const int b = bin_of(p.sc.x(v));
+        if (b < NB) atomicAdd(&s.hist[b], 1u);
+      });
+      gather(false, 0);
+      find_bin(t, (uint64_t)k, s);
       if (s.bin < NB) {  // else fewer than k tokens have a weight
-        find_border<false, ODD>(p, t, (uint64_t)k, turn, s);
+        summed = find_border<false, ODD>(p, t, (uint64_t)k, turn, s);
         border = s.border;
         sum = s.inside;
       }
+      if (by_p) clear();
     }
     if (by_p) {
-      const uint64_t need = need_of(top_p, sum);
-      find_bin<true>(t, need, s);
+      Mass all;
+      each(p, [&](uint32_t, float v) {
+        const float x = p.sc.x(v);
+        const int b = bin_of(x);
+        if (b == NB) return;
+        const float w = expf(x);
+        all.add(w);
+        const float scale = __uint_as_float((uint32_t)(127 + 16 + bin_scale(b)) << 23);
+        atomicAdd(&s.hist[b], __float_as_uint(__fmaf_rd(w, scale, 8388608.f)) - 0x4B000000u);
+      });
+      const uint64_t row_sum = gather(true, all.value());
+      const uint64_t need = need_of(top_p, border ? sum : row_sum);
+      find_bin(t, need, s);
       if (s.bin == NB) next_bin(t, NB, -1, s);  // the 16-bit sums fall short: the last bin with tokens
-      find_border<true, ODD>(p, t, need, turn, s);
+      summed = find_border<true, ODD>(p, t, need, turn, s);  // (top-p's border is not below top-k's)
       border = max(border, s.border);
     }
     cl_sync();  // xsum is read: it is written again below
@@ -520,21 +570,17 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Part<ODD>& p, ui
     const float w = p.sc.weight(v);
     return w < min_p ? 0.f : w;
   };
-  const uint32_t run = slice / WARPS;  // a multiple of 8
-  const uint32_t lo = min(n, warp * run), hi = min(n, lo + run);
-  Mass sum_m;
-#pragma unroll 2
-  for (uint32_t i = lo + 4 * lane; i + 3 < hi; i += 128) {
-    const float4 v = *reinterpret_cast<const float4*>(z + i);
-    sum_m.add(kept(i, v.x)), sum_m.add(kept(i + 1, v.y)), sum_m.add(kept(i + 2, v.z)), sum_m.add(kept(i + 3, v.w));
+  if (!summed) {
+    Mass sum_m;
+    each_of_run(p, [&](uint32_t i, float v) { sum_m.add(kept(i, v)); });
+    const uint64_t sum = warp_sum64(sum_m.value());
+    if (lane == 0) s.kept[warp] = sum;
+    __syncthreads();
   }
-  if ((hi & ~3u) + lane < hi && hi > lo) sum_m.add(kept((hi & ~3u) + lane, z[(hi & ~3u) + lane]));
-  const uint64_t sum = warp_sum64(sum_m.value());
-  if (lane == 0) s.part[warp] = sum;
-  __syncthreads();
+  const uint32_t run = p.run;
   if (tid < cl) {
     uint64_t v = 0;
-    for (int w = 0; w < WARPS; ++w) v += s.part[w];
+    for (int w = 0; w < WARPS; ++w) v += s.kept[w];
     put64(peer(&s.xsum[rank], tid), v);
   }
   cl_sync();
@@ -547,7 +593,7 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Part<ODD>& p, ui
   if (target < before || target >= before + s.xsum[rank]) return;
   // the warp's run, split again over the warps, then the token
   uint32_t r = 0;
-  while (before + s.part[r] <= target) before += s.part[r++];
+  while (before + s.kept[r] <= target) before += s.kept[r++];
   const uint32_t sub = (run / WARPS + 31) / 32 * 32;
   const uint32_t from = r * run, end = min(n, from + run);
   const uint32_t mine = min(end, from + warp * sub), mine_end = min(end, mine + sub);
@@ -619,10 +665,12 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     }
   }
   for (uint32_t i = done + tid; i < n; i += THREADS) z[i] = take(logit<DT>(src, i));
+  const float own_max = m;
   m = warp_max(m);
   if (lane == 0) s.part32[warp] = __float_as_uint(m);
-  for (int i = tid; i < NB; i += THREADS) s.cnt[i] = s.mass[i] = 0;
-  if (tid == 0) s.n_few = 0;
+  for (int i = tid; i < NB; i += THREADS) s.hist[i] = 0;
+  if (tid < 3) s.next[tid] = 0;
+  if (tid == 0) s.own = 0;
   __syncthreads();
   if (tid < cl) {  // thread r tells CTA r
     for (int w = 0; w < WARPS; ++w) m = fmaxf(m, __uint_as_float(s.part32[w]));
@@ -652,10 +700,12 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     return;
   }
   const float inv_t = __frcp_rn(temp);
+  float min_p = a.min_p ? a.min_p[row] : 0.f;
+  min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;  // the largest weight, 1, always stays
   if (m < INFINITY && inv_t < INFINITY && inv_t > 0.f)
-    draw(a, Part<false>{z, n, base, rank, cl, {m, inv_t}}, row, slice, s);
+    draw(a, Part<false>{z, n, base, rank, cl, slice / WARPS, {m, inv_t}, min_p}, row, own_max, s);
   else
-    draw(a, Part<true>{z, n, base, rank, cl, {m, inv_t}}, row, slice, s);
+    draw(a, Part<true>{z, n, base, rank, cl, slice / WARPS, {m, inv_t}, min_p}, row, own_max, s);
 }
 
 template <uint32_t DT>
