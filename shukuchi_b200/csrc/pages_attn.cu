@@ -46,9 +46,8 @@ constexpr int STEP = 2 * SUB;   // positions of a warp's step
 constexpr int UNIT = STEP * WARPS;
 constexpr int CTAS_PER_SM = 4;  // 128 registers a thread
 constexpr int MAX_CTAS = 640;   // 4 x the SMs of a B200 (148), rounded up
-constexpr int ITEM_UNITS = 1;   // what an item costs besides its positions, in units
+constexpr int ITEM_UNITS = 2;   // what an item costs besides its positions, in units (0: 32 ragged rows 78 us, 1: 66, 2: 66; 64 x 4: 62, 47, 45)
 constexpr int MIN_UNITS = 2;    // a CTA's part: shorter ones cost more in joining than they save
-constexpr int JOIN_THREADS = 512;
 
 template <int HD>
 struct Lay {
@@ -577,17 +576,18 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
   }
 }
 
-// Joins the pieces of the item that begins in CTA blockIdx.x's part: first
-// every piece's (max, sum) at once, then the outputs, 4 dims per thread and
-// the pieces dealt to the thread groups.
-template <int HD>
-__global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const __grid_constant__ PagesAttnArgs a) {
+// Joins the pieces of the item that begins in CTA blockIdx.x's part.  Its time
+// is that of loads that wait on one another, so there are two such waits: for the
+// header, then for the pieces' (max, sum) together with their outputs (4 dims a
+// thread, the pieces dealt to the thread groups, the first 8 of a group held in
+// registers meanwhile).
+template <int HD, int THREADS_J>
+__global__ void __launch_bounds__(THREADS_J) attend_join_kernel(const __grid_constant__ PagesAttnArgs a) {
   using L = Lay<HD>;
-  constexpr int PER_GROUP = HEADS * HD / 4, GROUPS = JOIN_THREADS / PER_GROUP;
-  __shared__ __align__(16) float st[2][HEADS][MAX_CTAS + 1];
+  constexpr uint32_t PER_GROUP = HEADS * HD / 4, GROUPS = THREADS_J / PER_GROUP, HELD = 8;
+  __shared__ float weight[HEADS][MAX_CTAS + 1];  // of a piece's outputs
   __shared__ float fin[HEADS];
-  float4* sum = reinterpret_cast<float4*>(st[0]);  // the maxima are done with by then
-  static_assert(sizeof(st[0]) >= JOIN_THREADS * sizeof(float4), "outputs fit where the maxima were");
+  __shared__ float4 sum[THREADS_J];
   const uint32_t c = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
   pdl_wait();
   const Header hd = static_cast<const Header*>(a.ws)[c];
@@ -596,42 +596,48 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const __grid_
   const uint32_t n_kv = a.pool.n_kv, G = a.n_heads / n_kv, nsub = (G + HEADS - 1) / HEADS;
   const uint32_t kvh = hd.item / nsub, sub = hd.item % nsub, n = (uint32_t)hd.last - c + 1;
   auto rec = [&](uint32_t i) { return records + (size_t)(2 * (c + i) + (i == 0 ? hd.slot : 0)) * L::REC; };
-  for (uint32_t i = tid; i < n * 2 * HEADS; i += JOIN_THREADS) {
-    const uint32_t p = i / (2 * HEADS), k = i % (2 * HEADS);
-    st[k / HEADS][k % HEADS][p] = rec(p)[HEADS * HD + k];
-  }
-  __syncthreads();
-  if (tid < 32 * HEADS) {
-    const uint32_t h = tid >> 5;
-    float m = -INFINITY, M = -INFINITY, l = 0.f;
-    for (uint32_t i = lane; i < n; i += 32) m = fmaxf(m, st[0][h][i]), M = fmaxf(M, st[1][h][i]);
-    m = warp_max(m);
-    M = warp_max(M);
-    for (uint32_t i = lane; i < n; i += 32) {
-      const float x = rec(i)[HEADS * (HD + 2) + h];
-      const bool some = x != 0.f;  // else a piece without positions
-      l += some ? x * ex2(st[0][h][i] - m) : 0.f;
-      st[1][h][i] = some ? ex2(st[1][h][i] - M) : 0.f;
-    }
-    l = warp_sum(l);
-    if (lane == 0) fin[h] = l == 0.f ? 0.f : ex2(M - m - 14.f) / l;
-  }
-  __syncthreads();
   const uint32_t grp = tid / PER_GROUP, e = tid % PER_GROUP, h = e / (HD / 4);
-  float4 o{};
-#pragma unroll 8
-  for (uint32_t i = grp; i < n; i += GROUPS) {
-    const float4 x = reinterpret_cast<const float4*>(rec(i))[e];
-    const float f = st[1][h][i];
-    o.x += x.x * f, o.y += x.y * f, o.z += x.z * f, o.w += x.w * f;
+  float4 x[HELD];
+#pragma unroll
+  for (uint32_t k = 0; k < HELD; ++k)
+    if (grp + k * GROUPS < n) x[k] = reinterpret_cast<const float4*>(rec(grp + k * GROUPS))[e];
+  if (tid < 32 * HEADS) {  // warp h: head h
+    const uint32_t hh = tid >> 5;
+    float m = -INFINITY, M = -INFINITY, l = 0.f;
+    for (uint32_t i = lane; i < n; i += 32) {  // running maxima, and the sum that goes with them
+      const float* r = rec(i) + HEADS * HD + hh;
+      const float rm = r[0], rM = r[HEADS], rl = r[2 * HEADS];
+      weight[hh][i] = rl == 0.f ? -INFINITY : rM;  // no positions: no weight
+      if (rl == 0.f) continue;
+      const float mn = fmaxf(m, rm);
+      l = (m == mn ? l : l * ex2(m - mn)) + (rm == mn ? rl : rl * ex2(rm - mn));
+      m = mn;
+      M = fmaxf(M, rM);
+    }
+    const float mm = warp_max(m);
+    M = warp_max(M);
+    l = warp_sum(l == 0.f ? 0.f : l * ex2(m - mm));
+    for (uint32_t i = lane; i < n; i += 32) weight[hh][i] = weight[hh][i] == -INFINITY ? 0.f : ex2(weight[hh][i] - M);
+    if (lane == 0) fin[hh] = l == 0.f ? 0.f : ex2(M - mm - 14.f) / l;
   }
+  __syncthreads();
+  float4 o{};
+  auto add = [&](const float4& v, uint32_t i) {
+    const float f = weight[h][i];
+    o.x += v.x * f, o.y += v.y * f, o.z += v.z * f, o.w += v.w * f;
+  };
+#pragma unroll
+  for (uint32_t k = 0; k < HELD; ++k)
+    if (grp + k * GROUPS < n) add(x[k], grp + k * GROUPS);
+#pragma unroll 4
+  for (uint32_t i = grp + HELD * GROUPS; i < n; i += GROUPS) add(reinterpret_cast<const float4*>(rec(i))[e], i);
   sum[tid] = o;
   __syncthreads();
   if (grp || sub * HEADS + h >= G) return;
 #pragma unroll
-  for (int k = 1; k < GROUPS; ++k) {
-    const float4 x = sum[k * PER_GROUP + e];
-    o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+  for (uint32_t k = 1; k < GROUPS; ++k) {
+    const float4 v = sum[k * PER_GROUP + e];
+    o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
   }
   const float f = fin[h];
   const size_t at = (uint32_t)hd.row * a.out_stride + (size_t)((sub * HEADS + h) * n_kv + kvh) * HD + 4 * (e % (HD / 4));
@@ -647,16 +653,21 @@ cudaError_t attend_go(const PagesAttnArgs& a, int num_sms, cudaStream_t st) {
   cudaError_t e = launch_k(attend_kernel<HD, TYPE>, dim3(ctas), dim3(THREADS), Lay<HD>::BYTES, st, a);
   if (e != cudaSuccess) return e;
   // the join waits for the kernel above by itself (griddepcontrol.wait)
+  // Few items are cut into many pieces each, and only their first CTAs have any
+  // to join: large blocks (1 x 8192, 32 pieces an item: 8.4 us against 11).  Many
+  // items are cut in two or three, by almost every CTA: small ones.
+  const uint32_t G = a.n_heads / a.pool.n_kv;
+  const bool many = (uint64_t)a.n_rows * a.pool.n_kv * ((G + HEADS - 1) / HEADS) * 4 > ctas;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(JOIN_THREADS);
+  cfg.blockDim = dim3(many ? 256 : 1024);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attend_join_kernel<HD>, a);
+  return many ? cudaLaunchKernelEx(&cfg, attend_join_kernel<HD, 256>, a) : cudaLaunchKernelEx(&cfg, attend_join_kernel<HD, 1024>, a);
 }
 
 }  // namespace
