@@ -190,10 +190,20 @@ struct Shared {
   uint32_t own;      // tokens of this CTA in the list
 };
 
-__device__ __forceinline__ uint32_t take_place(uint32_t* counter) {  // of CTA 0's copy
-  uint32_t at;
-  asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(peer(counter, 0)) : "memory");
-  return at;
+// Places for a warp's `mine` tokens (of 4 a lane) in a list whose counter is CTA
+// 0's: one atomic for all of them, as it takes as long as a hundred
+// instructions.  A lane's first place; its tokens follow one another.
+__device__ __forceinline__ uint32_t take_places(uint32_t* counter, uint32_t mine, Shared& s) {
+  const uint32_t lane = threadIdx.x & 31, upto = warp_scan(mine, lane);
+  uint32_t at = 0;
+  if (lane == 31) {
+    atomicAdd(&s.own, upto);
+    asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;"
+                 : "=r"(at)
+                 : "r"(peer(counter, 0)), "r"(upto)
+                 : "memory");
+  }
+  return __shfl_sync(0xffffffffu, at, 31) + upto - mine;
 }
 
 // A cluster's totals at this thread's bins (bin 0 holds the largest tokens),
@@ -258,28 +268,39 @@ struct Part {  // one CTA's part of a row
   float min_p;
 };
 
+// Four tokens at a time (those behind the slice's last are -inf).  What is done
+// with each of them has no branch, so that their chains of dependent
+// instructions run side by side (top-p's pass over 16k tokens: 7.6k cycles; one
+// token after the other, each with a branch, 9.2k).
+template <bool ODD, typename F>
+__device__ __forceinline__ void each4(const Part<ODD>& p, F f) {
+  for (uint32_t i0 = 128 * (threadIdx.x >> 5); i0 < p.n; i0 += 4 * THREADS) {  // whole warps stay together
+    const uint32_t i = i0 + 4 * (threadIdx.x & 31);
+    float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    if (i < p.n) v = *reinterpret_cast<const float4*>(p.z + i);
+    const float w[4] = {v.x, v.y, v.z, v.w};
+    f(i, w);
+  }
+}
+// The same, each warp over its run of the slice.
+template <bool ODD, typename F>
+__device__ __forceinline__ void each4_of_run(const Part<ODD>& p, F f) {
+  const uint32_t lo = min(p.n, (threadIdx.x >> 5) * p.run), hi = min(p.n, lo + p.run);
+  for (uint32_t i0 = lo; i0 < hi; i0 += 128) {
+    const uint32_t i = i0 + 4 * (threadIdx.x & 31);
+    float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    if (i < hi) v = *reinterpret_cast<const float4*>(p.z + i);
+    const float w[4] = {v.x, v.y, v.z, v.w};
+    f(i, w);
+  }
+}
+// One token after the other, for what concerns few of them.
 template <bool ODD, typename F>
 __device__ __forceinline__ void each(const Part<ODD>& p, F f) {
-  for (uint32_t i = 4 * threadIdx.x; i + 3 < p.n; i += 4 * THREADS) {
+  for (uint32_t i = 4 * threadIdx.x; i < p.n; i += 4 * THREADS) {
     const float4 v = *reinterpret_cast<const float4*>(p.z + i);
     f(i, v.x), f(i + 1, v.y), f(i + 2, v.z), f(i + 3, v.w);
   }
-  const uint32_t i = (p.n & ~3u) + threadIdx.x;
-  if (i < p.n) f(i, p.z[i]);
-}
-
-// Each warp over its run of the slice.
-template <bool ODD, typename F>
-__device__ __forceinline__ void each_of_run(const Part<ODD>& p, F f) {
-  const uint32_t lane = threadIdx.x & 31;
-  const uint32_t lo = min(p.n, (threadIdx.x >> 5) * p.run), hi = min(p.n, lo + p.run);
-#pragma unroll 2
-  for (uint32_t i = lo + 4 * lane; i + 3 < hi; i += 128) {
-    const float4 v = *reinterpret_cast<const float4*>(p.z + i);
-    f(i, v.x), f(i + 1, v.y), f(i + 2, v.z), f(i + 3, v.w);
-  }
-  const uint32_t i = (hi & ~3u) + lane;
-  if (i < hi && hi > lo) f(i, p.z[i]);
 }
 
 // The border token, from s.bin of find_bin on: s.border = its place, and the
@@ -302,24 +323,33 @@ __device__ bool find_border(const Part<ODD>& p, const Totals<OWN>& t, uint64_t n
     ++turn;
     __syncthreads();
     Mass above_m, in_m, kept_m;
-    each_of_run(p, [&](uint32_t i, float v) {
-      const float x = p.sc.x(v);
-      const int b = bin_of(x);
-      if (b > bin) return;
-      const float e = expf(x);
-      if (b < bin) {
-        above_m.add(e);
-        if (p.min_p > 0.f && e >= p.min_p) kept_m.add(e);
-        return;
+    each4_of_run(p, [&](uint32_t i, const float (&v)[4]) {
+      int b[4];
+      float e[4];
+      uint32_t mine = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x = p.sc.x(v[j]);
+        b[j] = bin_of(x);
+        e[j] = expf(x);
+        above_m.add(b[j] < bin ? e[j] : 0.f);
+        mine += b[j] == bin;
       }
-      in_m.add(e);
-      atomicAdd(&s.own, 1u);
-      const uint32_t at = take_place(place);
-      if (at >= CAP) return;
-      const uint64_t w = mass_of(e);
-      for (uint32_t r = 0; r < p.cl; ++r) {
-        put64(peer(&s.cand.place[list][at], r), place_of(v, p.base + i));
-        put64(peer(&s.cand.mass[list][at], r), w);
+      if (p.min_p > 0.f)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kept_m.add(b[j] < bin && e[j] >= p.min_p ? e[j] : 0.f);
+      if (!__any_sync(0xffffffffu, mine)) return;
+      uint32_t at = take_places(place, mine, s);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (b[j] != bin) continue;
+        in_m.add(e[j]);
+        if (at < CAP)
+          for (uint32_t r = 0; r < p.cl; ++r) {
+            put64(peer(&s.cand.place[list][at], r), place_of(v[j], p.base + i + j));
+            put64(peer(&s.cand.mass[list][at], r), mass_of(e[j]));
+          }
+        ++at;
       }
     });
     uint64_t above = warp_sum64(above_m.value()), in = warp_sum64(in_m.value());
@@ -337,12 +367,8 @@ __device__ bool find_border(const Part<ODD>& p, const Totals<OWN>& t, uint64_t n
     above = in = 0;
     uint32_t m = 0;
     for (uint32_t r = 0; r < p.cl; ++r) above += s.xabove[list][r], in += s.xin[list][r], m += s.xcnt[list][r];
-    if (BY_MASS && need <= above) {
-      next_bin(t, bin, -1, s);
-      continue;
-    }
-    if (BY_MASS && need > above + in) {
-      next_bin(t, bin, 1, s);
+    if (BY_MASS && (need <= above || need > above + in)) {
+      next_bin(t, bin, need <= above ? -1 : 1, s);
       if (s.bin < NB) continue;
       if (threadIdx.x == 0) s.border = 0, s.inside = above + in;  // not reached: every token stays
       __syncthreads();
@@ -446,10 +472,11 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Part<ODD>& p, ui
       }
       cl_sync();
       t = Totals<OWN>{};
-      for (uint32_t r = 0; r < cl; ++r) {
-        const uint4 c = get32x4(peer(&s.hist[OWN * tid], r));
-        t.v[0] += c.x, t.v[1] += c.y, t.v[2] += c.z, t.v[3] += c.w;
-      }
+      uint4 c[MAX_CL];  // all on their way at once
+#pragma unroll
+      for (uint32_t r = 0; r < MAX_CL; ++r) c[r] = r < cl ? get32x4(peer(&s.hist[OWN * tid], r)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (uint32_t r = 0; r < MAX_CL; ++r) t.v[0] += c[r].x, t.v[1] += c[r].y, t.v[2] += c[r].z, t.v[3] += c[r].w;
       if (masses)
 #pragma unroll
         for (int i = 0; i < OWN; ++i) t.v[i] <<= 24 - bin_scale(OWN * tid + i);
@@ -474,7 +501,8 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Part<ODD>& p, ui
         const float x = p.sc.x(v);
         if (bin_of(x) > bin) return;
         atomicAdd(&s.own, 1u);
-        const uint32_t at = take_place(&s.next[2]);
+        uint32_t at;
+        asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(peer(&s.next[2], 0)) : "memory");
         if (at >= CAP) return;
         const float w = expf(x);
         put64(peer(&s.few.place[at], 0), place_of(v, base + i));
@@ -529,9 +557,12 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Part<ODD>& p, ui
     }
     uint32_t turn = 0;
     if (by_k) {
-      each(p, [&](uint32_t, float v) {
-        const int b = bin_of(p.sc.x(v));
-        if (b < NB) atomicAdd(&s.hist[b], 1u);
+      each4(p, [&](uint32_t, const float (&v)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int b = bin_of(p.sc.x(v[j]));
+          if (b < NB) atomicAdd(&s.hist[b], 1u);
+        }
       });
       gather(false, 0);
       find_bin(t, (uint64_t)k, s);
@@ -544,14 +575,20 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Part<ODD>& p, ui
     }
     if (by_p) {
       Mass all;
-      each(p, [&](uint32_t, float v) {
-        const float x = p.sc.x(v);
-        const int b = bin_of(x);
-        if (b == NB) return;
-        const float w = expf(x);
-        all.add(w);
-        const float scale = __uint_as_float((uint32_t)(127 + 16 + bin_scale(b)) << 23);
-        atomicAdd(&s.hist[b], __float_as_uint(__fmaf_rd(w, scale, 8388608.f)) - 0x4B000000u);
+      each4(p, [&](uint32_t, const float (&v)[4]) {
+        int b[4];
+        uint32_t part[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x = p.sc.x(v[j]), w = expf(x);
+          b[j] = bin_of(x);
+          all.add(w);
+          const float scale = __uint_as_float((uint32_t)(127 + 16 + bin_scale(b[j])) << 23);
+          part[j] = __float_as_uint(__fmaf_rd(w, scale, 8388608.f)) - 0x4B000000u;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (b[j] < NB) atomicAdd(&s.hist[b[j]], part[j]);
       });
       const uint64_t row_sum = gather(true, all.value());
       const uint64_t need = need_of(top_p, border ? sum : row_sum);
@@ -566,13 +603,15 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Part<ODD>& p, ui
   const float border_z = border ? value_of((uint32_t)(border >> IDX_BITS)) : -INFINITY;
   const uint32_t border_idx = IDX_MASK - ((uint32_t)border & IDX_MASK);
   auto kept = [&](uint32_t i, float v) -> float {
-    if (v < border_z || (v == border_z && base + i > border_idx)) return 0.f;
     const float w = p.sc.weight(v);
-    return w < min_p ? 0.f : w;
+    return (v < border_z) | ((v == border_z) & (base + i > border_idx)) | (w < min_p) ? 0.f : w;
   };
   if (!summed) {
     Mass sum_m;
-    each_of_run(p, [&](uint32_t i, float v) { sum_m.add(kept(i, v)); });
+    each4_of_run(p, [&](uint32_t i, const float (&v)[4]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum_m.add(kept(i + j, v[j]));
+    });
     const uint64_t sum = warp_sum64(sum_m.value());
     if (lane == 0) s.kept[warp] = sum;
     __syncthreads();
@@ -665,6 +704,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     }
   }
   for (uint32_t i = done + tid; i < n; i += THREADS) z[i] = take(logit<DT>(src, i));
+  if (tid < ((4 - n) & 3)) z[n + tid] = -INFINITY;  // whole fours
   const float own_max = m;
   m = warp_max(m);
   if (lane == 0) s.part32[warp] = __float_as_uint(m);
