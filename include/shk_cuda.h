@@ -408,6 +408,19 @@ int shk_cuda_model_embed(shk_model *m, uint32_t token, void *stream);
 /* lm_head on the raw residual (no final norm, engine/src/engine.c:403-422) and
  * first-index argmax.  logits_host may be NULL. */
 int shk_cuda_model_lm_head(shk_model *m, uint32_t *token_host, float *logits_host, void *stream);
+/* A token drawn from the logits of the model's last output head (shk_cuda_token_step
+ * or shk_cuda_prefill with the next token wanted, shk_cuda_model_lm_head), as
+ * shk_cuda_sample draws one, in place of that call's argmax.  u in [0, 1);
+ * temperature <= 0 gives the argmax, top_k <= 0, top_p >= 1 and min_p <= 0 are
+ * off.  *prob_host (may be NULL): the token's share of the weights that stayed.
+ * Synchronous.  Single GPU (a tensor-parallel rank: SHK_EUNSUPPORTED). */
+struct shk_sampling {
+    float temperature;
+    int32_t top_k;
+    float top_p, min_p;
+};
+int shk_cuda_model_sample(shk_model *m, const struct shk_sampling *s, float u, uint32_t *token_host,
+                          float *prob_host, void *stream);
 float *shk_cuda_model_hidden(shk_model *m); /* device pointer to hidden[n_embd] */
 /* One whole token through embed -> all layers (-> lm_head -> argmax when
  * want_next) as one captured CUDA graph.  token and pos come from the host;

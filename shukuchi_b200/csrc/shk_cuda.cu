@@ -212,8 +212,8 @@ struct shk_model {
   shk_kv* kv = nullptr;
   float *hidden = nullptr, *q = nullptr, *k = nullptr, *v = nullptr, *att = nullptr,
         *act = nullptr, *logits = nullptr;
-  uint32_t* d_tok = nullptr;  // [0] token, [1] position
-  uint32_t* h_tok = nullptr;  // pinned: [0] token in, [1] pos in, [2] token out
+  uint32_t* d_tok = nullptr;  // [0] token, [1] position; [8..14] shk_cuda_model_sample
+  uint32_t* h_tok = nullptr;  // pinned: [0] token in, [1] pos in, [2] token out; [8..14] as d_tok
   float* am_v = nullptr;
   uint32_t* am_i = nullptr;
   int* am_cnt = nullptr;
@@ -1589,9 +1589,9 @@ shk_model* shk_cuda_model_create(shk_ctx* c, const shk_model_desc* d, shk_kv* kv
   ok = ok && cudaMalloc(&m->am_i, 256 * sizeof(uint32_t)) == cudaSuccess;
   ok = ok && cudaMalloc(&m->am_cnt, sizeof(int)) == cudaSuccess;
   ok = ok && cudaMemset(m->am_cnt, 0, sizeof(int)) == cudaSuccess;
-  ok = ok && cudaMalloc(&m->d_tok, 4 * sizeof(uint32_t)) == cudaSuccess;
-  ok = ok && cudaMemset(m->d_tok, 0, 4 * sizeof(uint32_t)) == cudaSuccess;
-  ok = ok && cudaMallocHost(&m->h_tok, 4 * sizeof(uint32_t)) == cudaSuccess;
+  ok = ok && cudaMalloc(&m->d_tok, 16 * sizeof(uint32_t)) == cudaSuccess;
+  ok = ok && cudaMemset(m->d_tok, 0, 16 * sizeof(uint32_t)) == cudaSuccess;
+  ok = ok && cudaMallocHost(&m->h_tok, 16 * sizeof(uint32_t)) == cudaSuccess;
   if (ok) ok = cudaMemset(m->hidden, 0, d->n_embd * sizeof(float)) == cudaSuccess;
   if (!ok) {
     shk_cuda_model_destroy(m);
@@ -1709,6 +1709,31 @@ int shk_cuda_model_lm_head(shk_model* m, uint32_t* token, float* logits, void* s
   if (logits) CK(cudaMemcpyAsync(logits, m->logits, (size_t)m->d.n_vocab * 4, cudaMemcpyDeviceToHost, st));
   CK(cudaStreamSynchronize(st));
   if (token) *token = m->h_tok[2];
+  return ctx_err_check(m->ctx);
+}
+
+int shk_cuda_model_sample(shk_model* m, const shk_sampling* p, float u, uint32_t* token, float* prob, void* s) {
+  if (m) on_dev(m->ctx);
+  if (!m || !p || !token || !(u >= 0.f && u < 1.f)) return SHK_EINVAL;
+  // (a tensor-parallel rank holds a slice of the logits)
+  if (m->ctx->tp_world > 1 || m->d.n_vocab > SHK_SAMPLE_MAX_VOCAB) return SHK_EUNSUPPORTED;
+  cudaStream_t st = pick(m->ctx, s);
+  CK(cudaStreamSynchronize(st));  // h_tok is reused below
+  uint32_t *h = m->h_tok + 8, *d = m->d_tok + 8;
+  memcpy(h, &p->temperature, 4);
+  memcpy(h + 1, &p->top_k, 4);
+  memcpy(h + 2, &p->top_p, 4);
+  memcpy(h + 3, &p->min_p, 4);
+  memcpy(h + 4, &u, 4);
+  CK(cudaMemcpyAsync(d, h, 20, cudaMemcpyHostToDevice, st));
+  auto f = [&](int i) { return reinterpret_cast<float*>(d + i); };
+  const SampleArgs a{m->logits, DT_F32, 1, m->d.n_vocab, m->d.n_vocab, f(0), reinterpret_cast<int32_t*>(d + 1), f(2),
+                     f(3),      f(4),   d + 5, f(6)};
+  CK(sample_launch(a, m->ctx->num_sms, st));
+  CK(cudaMemcpyAsync(h + 5, d + 5, 8, cudaMemcpyDeviceToHost, st));
+  CK(cudaStreamSynchronize(st));
+  *token = h[5];
+  if (prob) memcpy(prob, h + 6, 4);
   return ctx_err_check(m->ctx);
 }
 

@@ -76,6 +76,10 @@ class PagesRows(C.Structure):
                 ("table_stride", C.c_uint32), ("scale", C.c_float), ("ws_dev", C.c_void_p), ("ws_bytes", C.c_size_t)]
 
 
+class Sampling(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float)]
+
+
 P, U32, U64, I, F, SZ = C.c_void_p, C.c_uint32, C.c_uint64, C.c_int, C.c_float, C.c_size_t
 _SIGS = {
     "shk_cuda_init": (P, [C.POINTER(CudaConfig)]),
@@ -144,6 +148,7 @@ _SIGS = {
     "shk_cuda_forward_layer": (I, [P, C.POINTER(LayerDesc), U32, U32, P, P]),
     "shk_cuda_model_embed": (I, [P, U32, P]),
     "shk_cuda_model_lm_head": (I, [P, C.POINTER(U32), P, P]),
+    "shk_cuda_model_sample": (I, [P, C.POINTER(Sampling), F, C.POINTER(U32), C.POINTER(F), P]),
     "shk_cuda_model_hidden": (P, [P]),
     "shk_cuda_token_step": (I, [P, U32, U32, I, C.POINTER(U32), P]),
     "shk_cuda_decode_steps": (I, [P, U32, U32, U32, P]),
@@ -473,6 +478,13 @@ class DeviceModel:
         t = C.c_uint32(0)
         _call("shk_cuda_model_lm_head", self.h, C.byref(t), logits_host_ptr, None)
         return t.value
+
+    def sample(self, u: float, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, stream=None):
+        """(token, probability) drawn from the last output head's logits with the random number u."""
+        t, pr = C.c_uint32(0), C.c_float(0)
+        s = Sampling(temperature, top_k, top_p, min_p)
+        _call("shk_cuda_model_sample", self.h, C.byref(s), u, C.byref(t), C.byref(pr), stream)
+        return t.value, pr.value
 
     @property
     def hidden(self) -> int:

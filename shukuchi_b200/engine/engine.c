@@ -114,6 +114,8 @@ struct engine_handle {
     char *text;
     size_t text_len, text_cap;
     volatile int cancel;
+    struct shk_sampling sampling; /* temperature 0: greedy */
+    uint64_t seed, rng;           /* of the draws; rng starts at seed in every generation */
     uint32_t pos;      /* next KV position */
     uint64_t ring_next; /* ring mode: next loader request to consume */
 };
@@ -688,6 +690,28 @@ static int step(struct engine_handle *h, uint32_t tok, int want_next, uint32_t *
     return 0;
 }
 
+/* The next random number in [0, 1), 24 bits: SplitMix64 (Steele, Lea and
+ * Flood, "Fast splittable pseudorandom number generators", 2014). */
+static float next_uniform(uint64_t *state) {
+    uint64_t z = *state += 0x9E3779B97F4A7C15ull;
+    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+    z ^= z >> 31;
+    return (float)(z >> 40) * 0x1p-24f;
+}
+
+/* With engine_set_sampling: a draw in place of the greedy token that the last
+ * step returned. */
+static int draw(struct engine_handle *h, uint32_t *next) {
+    if (!(h->sampling.temperature > 0.f)) return 0;
+    const int e = shk_cuda_model_sample(h->m, &h->sampling, next_uniform(&h->rng), next, NULL, NULL);
+    if (e != SHK_OK || *next >= h->n_vocab) {
+        fprintf(stderr, "engine: position %u: sampling failed (%d)\n", h->pos, e);
+        return -1;
+    }
+    return 0;
+}
+
 /* engine/src/engine.c:306-501 token schedule. */
 static int generate(struct engine_handle *h, const uint32_t *prompt, uint32_t n_prompt, uint32_t n_decode,
                     token_callback cb, void *user, int print, float *logits_out) {
@@ -701,6 +725,11 @@ static int generate(struct engine_handle *h, const uint32_t *prompt, uint32_t n_
     if (h->text) h->text[0] = '\0';
     h->cancel = 0;
     h->pos = 0; /* each generation starts a new sequence */
+    h->rng = h->seed;
+    if (h->tp > 1 && h->sampling.temperature > 0.f) {
+        fprintf(stderr, "engine: sampling needs SHUKUCHI_TP=1\n");
+        return -1;
+    }
     shk_cuda_kv_clear(h->kv);
     if (!h->resident) {
         /* the ring streams exactly the passes this generation runs, like the
@@ -755,6 +784,7 @@ static int generate(struct engine_handle *h, const uint32_t *prompt, uint32_t n_
         const int last = i + 1 == n_prompt;
         rc = step(h, prompt[i], last, &next, last ? logits_out : NULL);
     }
+    if (!rc) rc = draw(h, &next);
     /* cancellation ends a generation between tokens; tensor-parallel ranks
      * run every step in lockstep, so there it takes effect at the end */
     for (uint32_t j = 0; j < n_decode && !rc && (h->tp > 1 || !h->cancel); ++j) {
@@ -763,6 +793,7 @@ static int generate(struct engine_handle *h, const uint32_t *prompt, uint32_t n_
         float *lg = (want && logits_out) ? logits_out + (size_t)(j + 1) * h->n_vocab : NULL;
         uint32_t nx = 0;
         if (!rc) rc = step(h, next, want, &nx, lg);
+        if (!rc && want) rc = draw(h, &nx);
         if (want) next = nx;
         note_rss(h);
     }
@@ -1308,6 +1339,16 @@ int engine_generate_ids(engine_handle_t *h, const uint32_t *prompt, uint32_t n_p
     const int rc = generate(h, prompt, n_prompt, n_decode, NULL, NULL, 0, out_logits);
     if (!rc && out_ids) memcpy(out_ids, h->out_ids, h->n_out * sizeof(uint32_t));
     return rc ? rc : (int)h->n_out;
+}
+
+int engine_set_sampling(engine_handle_t *h, float temperature, int top_k, float top_p, float min_p, uint64_t seed) {
+    if (!h || !(temperature >= 0.f) || temperature > 3.0e38f || top_p != top_p || min_p != min_p) return -1;
+    h->sampling.temperature = temperature;
+    h->sampling.top_k = top_k;
+    h->sampling.top_p = top_p;
+    h->sampling.min_p = min_p;
+    h->seed = seed;
+    return 0;
 }
 
 const char *engine_get_output(engine_handle_t *h) { return (h && h->text) ? h->text : ""; }

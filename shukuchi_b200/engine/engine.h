@@ -90,6 +90,13 @@ int engine_get_streaming_stats(engine_handle_t *h, struct streaming_stats *out);
 int engine_generate_ids(engine_handle_t *h, const uint32_t *prompt, uint32_t n_prompt,
                         uint32_t n_decode, uint32_t *out_ids, float *out_logits);
 uint32_t engine_vocab_size(engine_handle_t *h);
+/* Tokens drawn at random instead of the greedy ones (an addition: the
+ * reference only takes the argmax): temperature 0 (the default) is greedy, top_k
+ * <= 0, top_p >= 1 and min_p <= 0 are off (shk_cuda_sample says what each does).
+ * Every generation's draws start from `seed`: the same seed and prompt give the
+ * same tokens.  0, or -1 for a negative or NaN argument; with SHUKUCHI_TP > 1
+ * a generation with a temperature above 0 returns -1. */
+int engine_set_sampling(engine_handle_t *h, float temperature, int top_k, float top_p, float min_p, uint64_t seed);
 /* The GPU backend's counters on stderr (matvec calls, layer forwards, token
  * steps, staged copies and bytes): the CLI's closing report, as the
  * reference's main prints metal_ops_report() (engine/src/main.c:106). */

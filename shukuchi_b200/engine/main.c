@@ -2,7 +2,8 @@
  *   shukuchi <model.gguf> [--prompt "..."] [--max-tokens N] [--tokens 1,2,3]
  * SHUKUCHI_PREFETCH_DEPTH sets the loader depth (default 3; 0 -> 2).  Tokens
  * are printed as "<id>text"; the streaming statistics line follows on stderr.
- * --tokens (an addition) feeds token ids instead of prompt text. */
+ * --tokens (an addition) feeds token ids instead of prompt text; --temperature,
+ * --top-k, --top-p, --min-p and --seed (additions) draw the tokens at random. */
 #include <stdio.h>
 #include <stdlib.h>
 #include <string.h>
@@ -12,15 +13,26 @@
 
 int main(int argc, char **argv) {
     if (argc < 2) {
-        fprintf(stderr, "Usage: %s <model.gguf> [--prompt \"...\"] [--max-tokens N] [--tokens 1,2,3]\n", argv[0]);
+        fprintf(stderr,
+                "Usage: %s <model.gguf> [--prompt \"...\"] [--max-tokens N] [--tokens 1,2,3]\n"
+                "       [--temperature T] [--top-k K] [--top-p P] [--min-p P] [--seed S]\n",
+                argv[0]);
         return 1;
     }
     uint32_t max_tokens = 16;
     const char *prompt = NULL, *tokens = NULL;
+    float temperature = 0.f, top_p = 1.f, min_p = 0.f;
+    int top_k = 0;
+    uint64_t seed = 0;
     for (int i = 2; i + 1 < argc; ++i) {
         if (strcmp(argv[i], "--max-tokens") == 0) max_tokens = (uint32_t)strtoul(argv[++i], NULL, 10);
         else if (strcmp(argv[i], "--prompt") == 0) prompt = argv[++i];
         else if (strcmp(argv[i], "--tokens") == 0) tokens = argv[++i];
+        else if (strcmp(argv[i], "--temperature") == 0) temperature = strtof(argv[++i], NULL);
+        else if (strcmp(argv[i], "--top-k") == 0) top_k = (int)strtol(argv[++i], NULL, 10);
+        else if (strcmp(argv[i], "--top-p") == 0) top_p = strtof(argv[++i], NULL);
+        else if (strcmp(argv[i], "--min-p") == 0) min_p = strtof(argv[++i], NULL);
+        else if (strcmp(argv[i], "--seed") == 0) seed = strtoull(argv[++i], NULL, 10);
     }
     uint32_t depth = 3;
     const char *env = getenv("SHUKUCHI_PREFETCH_DEPTH");
@@ -37,6 +49,11 @@ int main(int argc, char **argv) {
     engine_handle_t *h = engine_open(argv[1], &cfg);
     if (!h) {
         fprintf(stderr, "engine: failed to open model\n");
+        return 1;
+    }
+    if (engine_set_sampling(h, temperature, top_k, top_p, min_p, seed) != 0) {
+        fprintf(stderr, "engine: bad sampling settings\n");
+        engine_close(h);
         return 1;
     }
     int rc;
