@@ -1008,6 +1008,10 @@ int shk_cuda_pages_attend(shk_ctx* c, const shk_pages* p, const shk_pages_rows* 
       (!r->seq_dev && r->n_rows > r->n_seq) || r->n_rows > SHK_PAGES_MAX_ROWS ||
       (uint64_t)r->table_stride * p->block_tokens > 0x7FFFFFFFull)
     return SHK_EINVAL;
+  // a row's q may be read again after its neighbours have been written
+  const size_t qs = r->q_stride ? r->q_stride : width, os = r->out_stride ? r->out_stride : width;
+  const uintptr_t q0 = reinterpret_cast<uintptr_t>(r->q_dev), o0 = reinterpret_cast<uintptr_t>(r->out_dev);
+  if (q0 < o0 + ((r->n_rows - 1) * os + width) * es && o0 < q0 + ((r->n_rows - 1) * qs + width) * es) return SHK_EINVAL;
   if (!r->ws_dev || !aligned(r->ws_dev, 16) ||
       r->ws_bytes < pages_attend_ws_bytes(r->n_rows, r->n_heads, g.pool.n_kv, g.pool.hd))
     return SHK_EINVAL;
@@ -1017,8 +1021,8 @@ int shk_cuda_pages_attend(shk_ctx* c, const shk_pages* p, const shk_pages_rows* 
   g.dtype = r->dtype;
   g.q = r->q_dev;
   g.out = r->out_dev;
-  g.q_stride = r->q_stride ? r->q_stride : width;
-  g.out_stride = r->out_stride ? r->out_stride : width;
+  g.q_stride = qs;
+  g.out_stride = os;
   g.row_seq = r->seq_dev;
   g.row_pos = r->pos_dev;
   g.table = r->table_dev;

@@ -614,7 +614,7 @@ def test_attend_arguments(ctx):
     for bad in (dict(q=None), dict(out=None), dict(n_heads=0), dict(n_heads=7), dict(n_heads=8192), dict(row_pos=None),
                 dict(table=None), dict(table_stride=0), dict(n_seq=0), dict(n_seq=1), dict(ws=None), dict(ws=p(ws) + 4),
                 dict(ws_bytes=n - 1), dict(dtype=2), dict(q_stride=511), dict(out_stride=100), dict(n_rows=65536),
-                dict(q=p(q) + 2), dict(table_stride=1 << 28)):
+                dict(q=p(q) + 2), dict(table_stride=1 << 28), dict(out=p(q)), dict(out=p(q) + 2048)):
         with pytest.raises(sc.ShkError):
             pool.pages.attend(**{**good, **bad})
     pool.pages.attend(**{**good, "n_rows": 0})
