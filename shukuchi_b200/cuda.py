@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import re
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libshk_cuda.so")
@@ -76,6 +77,13 @@ class PagesRows(C.Structure):
                 ("table_stride", C.c_uint32), ("scale", C.c_float), ("ws_dev", C.c_void_p), ("ws_bytes", C.c_size_t)]
 
 
+# The argument structs of calls that a server makes in every step are packed by
+# struct, which takes a third of the time of filling a ctypes.Structure.
+_ASSIGN = struct.Struct("@5I11P")
+_ROWS = struct.Struct("@3I2P2N3P2IfPN")
+assert _ASSIGN.size == C.sizeof(PagesAssign) and _ROWS.size == C.sizeof(PagesRows)
+
+
 class Sampling(C.Structure):
     _fields_ = [("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float)]
 
@@ -133,12 +141,12 @@ _SIGS = {
     "shk_cuda_kv_read_blocks": (I, [P, U32, U32, U32, P, P, P]),
     "shk_cuda_kv_attend": (I, [P, U32, P, P, P, P, U32, U32, F, P]),
     "shk_cuda_kv_attend_batch": (I, [P, U32, U32, P, P, P, P, U32, U32, F, P]),
-    "shk_cuda_pages_assign": (I, [P, C.POINTER(PagesAssign), P]),
+    "shk_cuda_pages_assign": (I, [P, P, P]),
     "shk_cuda_pages_release": (I, [P, U32, U32, U32, U32, P, P, P, P, P, P, P, P]),
-    "shk_cuda_pages_append": (I, [P, C.POINTER(PagesDesc), U32, P, P, U32, SZ, P, P]),
-    "shk_cuda_pages_read": (I, [P, C.POINTER(PagesDesc), U32, P, P, P, P]),
+    "shk_cuda_pages_append": (I, [P, P, U32, P, P, U32, SZ, P, P]),
+    "shk_cuda_pages_read": (I, [P, P, U32, P, P, P, P]),
     "shk_cuda_pages_attend_ws": (SZ, [U32, U32, U32, U32]),
-    "shk_cuda_pages_attend": (I, [P, C.POINTER(PagesDesc), C.POINTER(PagesRows), P]),
+    "shk_cuda_pages_attend": (I, [P, P, P, P]),
     "shk_cuda_sample": (I, [P, P, U32, U32, U32, SZ, P, P, P, P, P, P, P, P]),
     "shk_cuda_kv_clear": (None, [P]),
     "shk_cuda_kv_seq_len": (U32, [P, U32]),
@@ -299,21 +307,27 @@ class Context:
     def pages_assign(self, n_seq, block_tokens, n_blocks, table_stride, n_rows, have, add, table, free, n_free, lens,
                      counts, slots, pos, seq, last, stream=None):
         """Block tables, slots and positions of every request's new tokens (shk_cuda_pages_assign)."""
-        a = PagesAssign(n_seq, block_tokens, n_blocks, table_stride, n_rows, have, add, table, free, n_free, lens,
-                        counts, slots, pos, seq, last)
-        _call("shk_cuda_pages_assign", self.h, C.byref(a), stream)
+        a = _ASSIGN.pack(n_seq, block_tokens, n_blocks, table_stride, n_rows, have or 0, add or 0, table or 0, free or 0,
+                         n_free or 0, lens or 0, counts or 0, slots or 0, pos or 0, seq or 0, last or 0)
+        rc = (_lib or lib()).shk_cuda_pages_assign(self.h, a, stream)
+        if rc:
+            check("shk_cuda_pages_assign", rc)
 
     def pages_release(self, n_seq, block_tokens, n_blocks, table_stride, table, done, have, lens, free, n_free,
                       n_free_out, stream=None):
         """Blocks of the requests that are done, back on the free stack."""
-        _call("shk_cuda_pages_release", self.h, n_seq, block_tokens, n_blocks, table_stride, table, done, have, lens,
-              free, n_free, n_free_out, stream)
+        rc = (_lib or lib()).shk_cuda_pages_release(self.h, n_seq, block_tokens, n_blocks, table_stride, table, done,
+                                                    have, lens, free, n_free, n_free_out, stream)
+        if rc:
+            check("shk_cuda_pages_release", rc)
 
     def sample(self, logits, n_rows, n_vocab, u, out, prob=None, temperature=None, top_k=None, top_p=None,
                min_p=None, dtype=0, row_stride=0, stream=None):
         """One token per row of logits (shk_cuda_sample); settings are device arrays or None for off."""
-        _call("shk_cuda_sample", self.h, logits, dtype, n_rows, n_vocab, row_stride, temperature, top_k, top_p, min_p,
-              u, out, prob, stream)
+        rc = (_lib or lib()).shk_cuda_sample(self.h, logits, dtype, n_rows, n_vocab, row_stride, temperature, top_k,
+                                             top_p, min_p, u, out, prob, stream)
+        if rc:
+            check("shk_cuda_sample", rc)
 
     # staging
     def layer_stage(self, slot, dst_dev, src_host_ptr, nbytes):
@@ -410,17 +424,24 @@ class Pages:
         self.desc = PagesDesc(k, v, k_scale, v_scale, type_, n_blocks, n_kv_heads, head_dim, block_tokens)
 
     def append(self, n_tokens, k, v, slots, dtype=DTYPE_F32, row_stride=0, stream=None):
-        _call("shk_cuda_pages_append", self.ctx.h, C.byref(self.desc), n_tokens, k, v, dtype, row_stride, slots, stream)
+        rc = (_lib or lib()).shk_cuda_pages_append(self.ctx.h, C.byref(self.desc), n_tokens, k, v, dtype,
+                                               row_stride, slots, stream)
+        if rc:
+            check("shk_cuda_pages_append", rc)
 
     def read(self, n_tokens, slots, k, v, stream=None):
-        _call("shk_cuda_pages_read", self.ctx.h, C.byref(self.desc), n_tokens, slots, k, v, stream)
+        rc = (_lib or lib()).shk_cuda_pages_read(self.ctx.h, C.byref(self.desc), n_tokens, slots, k, v, stream)
+        if rc:
+            check("shk_cuda_pages_read", rc)
 
     def attend(self, n_rows, q, out, n_heads, row_pos, table, table_stride, n_seq, scale, ws, ws_bytes, row_seq=None,
                dtype=DTYPE_F32, q_stride=0, out_stride=0, stream=None):
         """Rows of q over the positions 0 .. row_pos of their requests; ws_bytes >= pages_attend_ws(...)."""
-        r = PagesRows(n_rows, n_heads, dtype, q, out, q_stride, out_stride, row_seq, row_pos, table, n_seq,
-                      table_stride, scale, ws, ws_bytes)
-        _call("shk_cuda_pages_attend", self.ctx.h, C.byref(self.desc), C.byref(r), stream)
+        r = _ROWS.pack(n_rows, n_heads, dtype, q or 0, out or 0, q_stride, out_stride, row_seq or 0, row_pos or 0,
+                       table or 0, n_seq, table_stride, scale, ws or 0, ws_bytes)
+        rc = (_lib or lib()).shk_cuda_pages_attend(self.ctx.h, C.byref(self.desc), r, stream)
+        if rc:
+            check("shk_cuda_pages_attend", rc)
 
 
 class DeviceModel:
