@@ -136,6 +136,13 @@ __device__ __forceinline__ void cl_sync() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// Another CTA's memory may be touched once that CTA has begun: each says so at
+// its start, and waits for the others' word before its first store to them.
+__device__ __forceinline__ void cl_begun() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cl_all_begun() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ uint32_t peer(const void* p, uint32_t rank) {
   uint32_t a;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
@@ -663,6 +670,7 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Part<ODD>& p, ui
 template <uint32_t DT>
 __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constant__ SampleArgs a, uint32_t slice) {
   extern __shared__ __align__(16) uint8_t sample_smem[];
+  cl_begun();
   float* z = reinterpret_cast<float*>(sample_smem);
   Shared& s = *reinterpret_cast<Shared*>(sample_smem + sizeof(float) * slice);
   const uint32_t rank = cl_rank(), cl = cl_size(), row = blockIdx.x / cl;
@@ -712,6 +720,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
   if (tid < 3) s.next[tid] = 0;
   if (tid == 0) s.own = 0;
   __syncthreads();
+  cl_all_begun();
   if (tid < cl) {  // thread r tells CTA r
     for (int w = 0; w < WARPS; ++w) m = fmaxf(m, __uint_as_float(s.part32[w]));
     put32(peer(&s.xmax[rank], tid), __float_as_uint(m));
