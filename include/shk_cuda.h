@@ -333,7 +333,11 @@ int shk_cuda_pages_read(shk_ctx *ctx, const struct shk_pages *pages, uint32_t n_
  * (engine/src/ops.c:423).  pos < 0: the row sees nothing and becomes zeros;
  * seq < 0: no row (padding), out left as it was.  q and out are dtype F32, F16
  * or BF16 rows of n_heads * head_dim, q_stride / out_stride elements apart (0 =
- * dense); out may not overlap q.  Sums and softmax in fp32.  ws_dev:
+ * dense); out may not overlap q.  Sums and softmax in fp32.  Rows of one request
+ * that follow one another read its blocks together.  What no row of the call
+ * sees may hold anything; between a row's last position and that of a
+ * neighbour in its request, E4M3 bytes have to be numbers, as shk_cuda_pages_append
+ * writes them.  ws_dev:
  * shk_cuda_pages_attend_ws bytes, 16-byte aligned, contents of no account
  * before and after; calls that may run at the same time need one each. */
 struct shk_pages_rows {

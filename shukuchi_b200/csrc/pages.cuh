@@ -70,6 +70,11 @@ struct PagesAttnArgs {
   float scale;
   void* ws;
   int* err;
+  // set by the launcher
+  uint32_t group;      // query heads of a KV head
+  uint32_t subs;       // items of a KV head and row
+  uint32_t window;     // rows whose heads fit one item
+  uint32_t inv_group;  // 2^16 / group + 1: x * inv_group >> 16 is x / group for x < 16
 };
 
 cudaError_t pages_init();  // kernel attributes, once per device

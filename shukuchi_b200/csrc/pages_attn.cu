@@ -2,8 +2,9 @@
 //
 // A row reads its request's keys and values once and does 4 hd flops per
 // position and query head with them: bound by memory.  So the work is laid out
-// by bytes.  An item is one row's positions for up to 8 query heads of one KV
-// head; items are cut into units of 128 positions, all units of all items are
+// by bytes.  An item is the positions that one row reads for up to 8 or 16 query
+// heads of one KV head, or that several rows of one request read together, where
+// their heads fit; items are cut into units of 128 positions, all units of all items are
 // put in one line, and each CTA takes an equal part of it, whatever the
 // lengths.  A CTA's part may begin and end inside an item: its (max, sum,
 // output) for that piece goes to the workspace and a second, small kernel joins
@@ -40,16 +41,16 @@ namespace {
 
 constexpr int WARPS = 4;
 constexpr int THREADS = 32 * WARPS;
-constexpr int HEADS = 8;        // query heads of an item: the MMA's rows g
+constexpr int HEADS = 8;        // slots (a row's query head each) of a set: the MMA's rows g
 constexpr int SUB = 16;         // positions under one pair of scales
 constexpr int STEP = 2 * SUB;   // positions of a warp's step
 constexpr int UNIT = STEP * WARPS;
-constexpr int CTAS_PER_SM = 4;  // 128 registers a thread
+constexpr int CTAS_PER_SM = 4;  // 128 registers a thread (two sets: 3, 168)
 constexpr int MAX_CTAS = 640;   // 4 x the SMs of a B200 (148), rounded up
 constexpr int ITEM_UNITS = 2;   // what an item costs besides its positions, in units (0: 32 ragged rows 78 us, 1: 66, 2: 66; 64 x 4: 62, 47, 45)
 constexpr int MIN_UNITS = 2;    // a CTA's part: shorter ones cost more in joining than they save
 
-template <int HD>
+template <int HD, int SETS>
 struct Lay {
   static constexpr int NP = HD / 64;            // 16-byte pieces of a K row per lane
   static constexpr int NW = HD / 32;            // words of a V row per lane
@@ -57,15 +58,17 @@ struct Lay {
   static constexpr int HALF = SUB * HD;         // bytes of 16 positions of K or V
   static constexpr int KBUF = 2 * HALF;         // a step's K; V has two such buffers behind it
   static constexpr int RING = 3 * KBUF;         // per warp
-  static constexpr int QF = STEPS * 32 * 16;    // q fragments
+  static constexpr int CTAS = SETS == 2 ? 3 : CTAS_PER_SM;
+  static constexpr int QF = STEPS * 32 * 16;    // a set's q fragments
   static constexpr int HROW = HD + 4;           // floats of a head's outputs in shared memory, padded
-  static constexpr int BYTES = WARPS * RING + QF;
-  static constexpr int REC = HEADS * (HD + 3);  // floats of a piece's record: O, m, M, l
+  static constexpr int BYTES = WARPS * RING + SETS * QF;
+  static constexpr int REC = HEADS * (HD + 3);  // floats of a piece's record of one set: O, m, M, l
   static_assert(HEADS * HROW * 4 <= RING, "a warp's output fits its ring");
 };
 
 struct Header {  // the item that begins in a CTA's part and ends in a later one's
-  int32_t row, item, last, slot;
+  int32_t row, item, last;
+  int32_t slot_rows;  // which of the CTA's two records, and twice the item's rows
 };
 
 __device__ __forceinline__ float load_dt(const void* p, size_t i, uint32_t dt) {
@@ -136,27 +139,39 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
 
 struct Row {
   int32_t z;
-  uint32_t len, units;
+  uint32_t len, units, rows;  // of the item: the longest row's positions, units of them, and its rows
 };
 
-// A live row has at least one unit, so that a row which sees nothing is
-// written (zeros); a padding row has none.
-__device__ __forceinline__ Row row_of(const PagesAttnArgs& a, uint32_t r) {
-  Row w;
-  w.z = a.row_seq ? a.row_seq[r] : (int32_t)r;
-  const int32_t p = a.row_pos[r];
-  w.len = 0;
-  w.units = 0;
-  if (w.z < 0) return w;
-  if (p >= 0) {
-    if ((uint32_t)w.z >= a.n_seq || (uint64_t)p >= ((uint64_t)a.stride << a.pool.block_shift))
-      set_error(a.err, DERR_BAD_POS);
-    else
-      w.len = (uint32_t)p + 1;
-  } else if ((uint32_t)w.z >= a.n_seq) {
-    set_error(a.err, DERR_BAD_POS);
+// Positions of row r of request z.
+__device__ __forceinline__ uint32_t row_len(const PagesAttnArgs& a, int32_t z, int32_t p) {
+  if ((uint32_t)z >= a.n_seq || (p >= 0 && (uint64_t)p >= ((uint64_t)a.stride << a.pool.block_shift))) {
+    if (z >= 0) set_error(a.err, DERR_BAD_POS);
+    return 0;
   }
-  w.units = w.len ? (w.len + UNIT - 1) / UNIT : 1;
+  return z >= 0 && p >= 0 ? (uint32_t)p + 1 : 0;
+}
+
+// The item that begins at row r.  MANY: up to a.window rows of one request, one
+// behind the other, that begin at a multiple of a.window or where the request
+// changes; other rows have no units.  A padding row has none either; live rows
+// have at least one, so that rows which see nothing are written (zeros).
+template <bool MANY>
+__device__ __forceinline__ Row row_of(const PagesAttnArgs& a, uint32_t r) {
+  Row w{a.row_seq ? a.row_seq[r] : (int32_t)r, 0, 0, 1};
+  w.len = row_len(a, w.z, a.row_pos[r]);
+  bool leads = true;
+  if (MANY && a.window > 1) {
+    const uint32_t in = r % a.window, behind = min(a.window - in, a.n_rows - r);
+    leads = in == 0 || a.row_seq[r - 1] != w.z;
+    bool same = true;
+#pragma unroll 4
+    for (uint32_t i = 1; i < behind; ++i) {  // (loads that do not wait on one another)
+      const int32_t z = a.row_seq[r + i], p = a.row_pos[r + i];
+      same = same && z == w.z;
+      if (same) w.len = max(w.len, row_len(a, z, p)), ++w.rows;
+    }
+  }
+  if (w.z >= 0 && leads) w.units = w.len ? (w.len + UNIT - 1) / UNIT : 1;
   return w;
 }
 
@@ -194,7 +209,7 @@ template <int HD, uint32_t TYPE, bool V>
 __device__ __forceinline__ void fetch(const uint8_t* row0, uint32_t dst, uint32_t rows, uint32_t lane) {
   const uint8_t* src = row0 + 16 * lane;
 #pragma unroll
-  for (int j = 0; j < Lay<HD>::HALF / 512; ++j) {
+  for (int j = 0; j < SUB * HD / 512; ++j) {
     const uint32_t to = dst + at_piece<HD, V>(4 * j + (lane >> 3), lane & 7);
     if constexpr (V && TYPE == PAGES_E4M3)
       copy_or_zero(to, src + 512 * j, (512 * j + 16 * lane) / HD < rows);
@@ -203,16 +218,17 @@ __device__ __forceinline__ void fetch(const uint8_t* row0, uint32_t dst, uint32_
   }
 }
 
-template <int HD, uint32_t TYPE>
-__global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __grid_constant__ PagesAttnArgs a) {
-  using L = Lay<HD>;
+template <int HD, uint32_t TYPE, int SETS, bool MANY>
+__global__ void __launch_bounds__(THREADS, Lay<HD, SETS>::CTAS) attend_kernel(const __grid_constant__ PagesAttnArgs a) {
+  using L = Lay<HD, SETS>;
+  constexpr uint32_t SLOTS = SETS * HEADS;
   extern __shared__ __align__(16) uint8_t att_smem[];
   __shared__ Sums sums;
-  __shared__ int32_t qmax[HEADS];
+  __shared__ int32_t qmax[SLOTS];
   __shared__ float stat[WARPS][HEADS][3];
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const uint32_t c = blockIdx.x, bs = a.pool.block_shift, n_kv = a.pool.n_kv, G = a.n_heads / n_kv;
-  const uint32_t nsub = (G + HEADS - 1) / HEADS, NI = n_kv * nsub;
+  const uint32_t c = blockIdx.x, bs = a.pool.block_shift, n_kv = a.pool.n_kv, G = a.group;
+  const uint32_t nsub = a.subs, NI = n_kv * nsub;
   Header* headers = static_cast<Header*>(a.ws);
   float* records = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + MAX_CTAS * sizeof(Header));
   pdl_trigger();
@@ -239,13 +255,13 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
     }
     return v;
   };
-  Row rw = tid < a.n_rows ? row_of(a, tid) : Row{-1, 0, 0};
+  Row rw = tid < a.n_rows ? row_of<MANY>(a, tid) : Row{-1, 0, 0, 0};
   uint64_t total;
   uint64_t upto = scan(cost(rw), total);
   uint64_t carry = total;
   if (a.n_rows > THREADS) {
     uint64_t more = 0;
-    for (uint32_t r = THREADS + tid; r < a.n_rows; r += THREADS) more += cost(row_of(a, r));
+    for (uint32_t r = THREADS + tid; r < a.n_rows; r += THREADS) more += cost(row_of<MANY>(a, r));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
     __syncthreads();
@@ -262,7 +278,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
   for (uint32_t r0 = 0;; r0 += THREADS) {  // the row that unit s belongs to
     if (r0) {
       __syncthreads();
-      rw = r0 + tid < a.n_rows ? row_of(a, r0 + tid) : Row{-1, 0, 0};
+      rw = r0 + tid < a.n_rows ? row_of<MANY>(a, r0 + tid) : Row{-1, 0, 0, 0};
       uint64_t n;
       upto = carry + scan(cost(rw), n);
       carry += n;
@@ -302,17 +318,28 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
     const bool next_row = s < end && s == base + (uint64_t)NI * span;
     if (ub > 0) {
     const uint32_t kvh = item / nsub, sub = item % nsub;
-    const uint32_t n_heads = min(G - sub * HEADS, (uint32_t)HEADS);
+    // slot x of the item: head sub * SLOTS + x of its row, or head x % G of row x / G
+    const uint32_t slots = MANY && nsub == 1 ? rw.rows * G : min(G - sub * SLOTS, SLOTS);
+    auto slot_in = [&](uint32_t x) { return MANY && nsub == 1 ? x * a.inv_group >> 16 : 0; };
+    auto slot_row = [&](uint32_t x) { return row + slot_in(x); };
+    auto slot_dim = [&](uint32_t x) { return (size_t)((sub * SLOTS + x - slot_in(x) * G) * n_kv + kvh) * HD; };
     const int32_t* table = a.table + (size_t)rw.z * a.stride;  // z is in range where len > 0
 
     // q of this lane's fragments: k-step st covers, for lane (g, t), the 4 dims of word st % 4 of its piece st / 4
-    float q[L::STEPS / WARPS][4];
+    float q[SETS][L::STEPS / WARPS][4];
+    uint32_t len[SETS];  // of the rows of this lane's slots
 #pragma unroll
-    for (int i = 0; i < L::STEPS / WARPS; ++i) {
-      const uint32_t st = warp + WARPS * i, d = 64 * (st >> 2) + 16 * t + 4 * (st & 3);
-      const size_t at = row * a.q_stride + (size_t)((sub * HEADS + g) * n_kv + kvh) * HD + d;
+    for (int x = 0; x < SETS; ++x) {
+      const uint32_t slot = HEADS * x + g;
+      len[x] = rw.len;
+      if (MANY && rw.rows > 1 && slot < slots) len[x] = row_len(a, rw.z, a.row_pos[slot_row(slot)]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) q[i][e] = g < n_heads ? load_dt(a.q, at + e, a.dtype) : 0.f;
+      for (int i = 0; i < L::STEPS / WARPS; ++i) {
+        const uint32_t st = warp + WARPS * i, d = 64 * (st >> 2) + 16 * t + 4 * (st & 3);
+        const size_t at = slot < slots ? slot_row(slot) * a.q_stride + slot_dim(slot) + d : 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[x][i][e] = slot < slots ? load_dt(a.q, at + e, a.dtype) : 0.f;
+      }
     }
 
     // ---- this warp's steps: units ua .. ub - 1, positions UNIT u + STEP warp ----
@@ -356,10 +383,13 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
       const size_t at = (size_t)(id < 0 ? 0 : id) * n_kv + kvh;
       return make_float2(a.pool.ks[at], a.pool.vs[at]);
     };
-    float m = -INFINITY, M = -INFINITY, l = 0.f;
-    float o[HD / 16][4];
+    float m[SETS], M[SETS], l[SETS], o[SETS][HD / 16][4];
 #pragma unroll
-    for (int j = 0; j < HD / 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    for (int x = 0; x < SETS; ++x) {
+      m[x] = M[x] = -INFINITY, l[x] = 0.f;
+#pragma unroll
+      for (int j = 0; j < HD / 16; ++j) o[x][j][0] = o[x][j][1] = o[x][j][2] = o[x][j][3] = 0.f;
+    }
     int2 id0{-1, -1}, id1{-1, -1};
     float2 sx{}, sy{};
     if (n > 0) {  // the first copies are on their way before q is needed
@@ -372,28 +402,35 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
     }
 
     // q scaled by a power of two so that the largest magnitude of a head is in [2^14, 2^15)
-    if (tid < HEADS) qmax[tid] = 0;
+    if (tid < SLOTS) qmax[tid] = 0;
     __syncthreads();
-    float big = 0.f;
 #pragma unroll
-    for (int i = 0; i < L::STEPS / WARPS; ++i)
+    for (int x = 0; x < SETS; ++x) {
+      float big = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(q[i][e]));
-    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-    if (t == 0) atomicMax(&qmax[g], __float_as_int(big));
+      for (int i = 0; i < L::STEPS / WARPS; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(q[x][i][e]));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      if (t == 0) atomicMax(&qmax[HEADS * x + g], __float_as_int(big));
+    }
     __syncthreads();
-    const float top = __int_as_float(qmax[g]);
-    int ex = 0;
-    if (top > 0.f && top < INFINITY) ex = min(14 - ilogbf(top), 126);
-    const float up = ldexpf(1.f, ex);
-    const float qscale = a.scale * 1.4426950408889634f * ldexpf(1.f, -ex);
+    float qscale[SETS];
 #pragma unroll
-    for (int i = 0; i < L::STEPS / WARPS; ++i) {
-      uint4 f;
-      split2(q[i][0] * up, q[i][1] * up, f.x, f.y);
-      split2(q[i][2] * up, q[i][3] * up, f.z, f.w);
-      qf[(warp + WARPS * i) * 32 + lane] = f;
+    for (int x = 0; x < SETS; ++x) {
+      const float top = __int_as_float(qmax[HEADS * x + g]);
+      int ex = 0;
+      if (top > 0.f && top < INFINITY) ex = min(14 - ilogbf(top), 126);
+      const float up = ldexpf(1.f, ex);
+      qscale[x] = a.scale * 1.4426950408889634f * ldexpf(1.f, -ex);
+#pragma unroll
+      for (int i = 0; i < L::STEPS / WARPS; ++i) {
+        uint4 f;
+        split2(q[x][i][0] * up, q[x][i][1] * up, f.x, f.y);
+        split2(q[x][i][2] * up, q[x][i][3] * up, f.z, f.w);
+        qf[(x * L::STEPS + warp + WARPS * i) * 32 + lane] = f;
+      }
     }
     __syncthreads();
 
@@ -405,7 +442,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
       copy_wait<1>();  // this step's K and V; the next V may be on its way
       __syncwarp();
       const uint8_t* here = att_smem + warp * L::RING;
-      float acc[4][4] = {};
+      float acc[SETS][4][4] = {};
 #pragma unroll
       for (int pi = 0; pi < L::NP; ++pi) {
         uint32_t kw[4][4];
@@ -416,33 +453,20 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
         }
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const uint4 qa = qf[(4 * pi + w) * 32 + lane];
+          uint4 qa[SETS];
+#pragma unroll
+          for (int x = 0; x < SETS; ++x) qa[x] = qf[(x * L::STEPS + 4 * pi + w) * 32 + lane];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             uint32_t b0, b1;
             to_f16<TYPE>(kw[j][w], b0, b1);
-            mma_f16(acc[j], qa, b0, b1);
+#pragma unroll
+            for (int x = 0; x < SETS; ++x) mma_f16(acc[x][j], qa[x], b0, b1);
           }
         }
       }
       __syncwarp();
       issue_k(i + 1, id1);  // this step's K has been multiplied
-      // scores in powers of two; lane (g, t) holds head g at positions 8 j + 2t, 8 j + 2t + 1
-      float sv[4][2];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float f = (j < 2 ? sx.x : sy.x) * qscale;
-        sv[j][0] = (acc[j][0] + acc[j][2]) * f;
-        sv[j][1] = (acc[j][1] + acc[j][3]) * f;
-      }
-      const int32_t left = (int32_t)(rw.len - place(i, 0));
-      if (left < STEP || id0.x < 0 || id0.y < 0) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if ((int32_t)(8 * j + 2 * t + e) >= left || (j < 2 ? id0.x : id0.y) < 0) sv[j][e] = -INFINITY;
-      }
       // a V scale is 2^E * vf, vf below 2 (also for a scale of 0, an infinite one or NaN)
       float E[2], vf[2];
 #pragma unroll
@@ -452,40 +476,63 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
         E[h] = (float)(e8 - 127);
         vf[h] = e8 == 254 ? vs * 0x1p-127f : vs * __int_as_float((254 - e8) << 23);
       }
-      const float c0 = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
-      const float c1 = fmaxf(fmaxf(sv[2][0], sv[2][1]), fmaxf(sv[3][0], sv[3][1]));
-      float mn = fmaxf(c0, c1), Mn = fmaxf(c0 + E[0], c1 + E[1]);
+      // scores in powers of two; lane (g, t) holds slot g at positions 8 j + 2t, 8 j + 2t + 1
+      float sv[SETS][4][2], m0[SETS], M0[SETS];
 #pragma unroll
-      for (int x = 1; x <= 2; x <<= 1) {
-        mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, x));
-        Mn = fmaxf(Mn, __shfl_xor_sync(0xffffffffu, Mn, x));
-      }
-      mn = fmaxf(m, mn), Mn = fmaxf(M, Mn);
-      if (__any_sync(0xffffffffu, mn > m || Mn > M)) {
-        const float al = m == mn ? 1.f : ex2(m - mn), aM = M == Mn ? 1.f : ex2(M - Mn);
-        l *= al;
-        // the outputs of lane (g, t) are heads 2t and 2t + 1
-        const float a0 = __shfl_sync(0xffffffffu, aM, 8 * t), a1 = __shfl_sync(0xffffffffu, aM, 8 * t + 4);
+      for (int x = 0; x < SETS; ++x) {
 #pragma unroll
-        for (int j = 0; j < HD / 16; ++j) o[j][0] *= a0, o[j][1] *= a1, o[j][2] *= a0, o[j][3] *= a1;
-        m = mn;
-        M = Mn;
+        for (int j = 0; j < 4; ++j) {
+          const float f = (j < 2 ? sx.x : sy.x) * qscale[x];
+          sv[x][j][0] = (acc[x][j][0] + acc[x][j][2]) * f;
+          sv[x][j][1] = (acc[x][j][1] + acc[x][j][3]) * f;
+        }
+        const int32_t left = (int32_t)(len[x] - place(i, 0));
+        if (left < STEP || id0.x < 0 || id0.y < 0) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if ((int32_t)(8 * j + 2 * t + e) >= left || (j < 2 ? id0.x : id0.y) < 0) sv[x][j][e] = -INFINITY;
+        }
+        const float c0 = fmaxf(fmaxf(sv[x][0][0], sv[x][0][1]), fmaxf(sv[x][1][0], sv[x][1][1]));
+        const float c1 = fmaxf(fmaxf(sv[x][2][0], sv[x][2][1]), fmaxf(sv[x][3][0], sv[x][3][1]));
+        float mn = fmaxf(c0, c1), Mn = fmaxf(c0 + E[0], c1 + E[1]);
+#pragma unroll
+        for (int y = 1; y <= 2; y <<= 1) {
+          mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, y));
+          Mn = fmaxf(Mn, __shfl_xor_sync(0xffffffffu, Mn, y));
+        }
+        mn = fmaxf(m[x], mn), Mn = fmaxf(M[x], Mn);
+        if (__any_sync(0xffffffffu, mn > m[x] || Mn > M[x])) {
+          const float al = m[x] == mn ? 1.f : ex2(m[x] - mn), aM = M[x] == Mn ? 1.f : ex2(M[x] - Mn);
+          l[x] *= al;
+          // the outputs of lane (g, t) are slots 2t and 2t + 1
+          const float a0 = __shfl_sync(0xffffffffu, aM, 8 * t), a1 = __shfl_sync(0xffffffffu, aM, 8 * t + 4);
+#pragma unroll
+          for (int j = 0; j < HD / 16; ++j) o[x][j][0] *= a0, o[x][j][1] *= a1, o[x][j][2] *= a0, o[x][j][3] *= a1;
+          m[x] = mn;
+          M[x] = Mn;
+        }
+        // a step without positions may leave the maxima at -inf: its weights are 0
+        m0[x] = m[x] == -INFINITY ? 0.f : m[x], M0[x] = M[x] == -INFINITY ? 0.f : M[x];
       }
-      // a step without positions (its blocks are bad) may leave the maxima at -inf: its weights are 0
-      const float m0 = m == -INFINITY ? 0.f : m, M0 = M == -INFINITY ? 0.f : M;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float wt[4];
+        uint32_t hi0[SETS], lo0[SETS], hi1[SETS], lo1[SETS];
         const float vo = E[h] + 14.f;  // weights up to 2^15: their low parts stay normal f16
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = sv[2 * h + (e >> 1)][e & 1];
-          l += ex2(x - m0);
-          wt[e] = ex2((x - M0) + vo) * vf[h];
+        for (int x = 0; x < SETS; ++x) {
+          float wt[4];
+          const float f = (int32_t)(len[x] - place(i, h)) <= 0 ? 0.f : vf[h];  // (an infinite scale of positions that the slot does not see)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float y = sv[x][2 * h + (e >> 1)][e & 1];
+            l[x] += ex2(y - m0[x]);
+            wt[e] = ex2((y - M0[x]) + vo) * f;
+          }
+          split2(wt[0], wt[1], hi0[x], lo0[x]);
+          split2(wt[2], wt[3], hi1[x], lo1[x]);
         }
-        uint32_t hi0, lo0, hi1, lo1;
-        split2(wt[0], wt[1], hi0, lo0);
-        split2(wt[2], wt[3], hi1, lo1);
         const uint8_t* vp = here + L::KBUF + (i & 1) * L::KBUF + h * L::HALF;
         uint32_t vr[4][L::NW];
 #pragma unroll
@@ -506,8 +553,11 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
             uint4 va;
             to_f16<TYPE>(__byte_perm(vr[0][w], vr[1][w], e ? 0x7362 : 0x5140), va.x, va.y);
             to_f16<TYPE>(__byte_perm(vr[2][w], vr[3][w], e ? 0x7362 : 0x5140), va.z, va.w);
-            mma_f16(o[2 * w + e], va, hi0, hi1);
-            mma_f16(o[2 * w + e], va, lo0, lo1);
+#pragma unroll
+            for (int x = 0; x < SETS; ++x) {
+              mma_f16(o[x][2 * w + e], va, hi0[x], hi1[x]);
+              mma_f16(o[x][2 * w + e], va, lo0[x], lo1[x]);
+            }
           }
       }
       id0 = id1, id1 = id2;
@@ -516,23 +566,29 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
     }
     copy_wait<0>();
 
-    // ---- the warps' outputs meet in shared memory (each in its own ring) ----
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    // lane (g, t): heads 2t and 2t + 1, the HD / 8 dims from HD / 8 g
-    float* mo = reinterpret_cast<float*>(att_smem + warp * L::RING) + 2 * t * L::HROW + g * (HD / 8);
-    __syncwarp();
-#pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-      for (int j = 0; j < HD / 16; j += 2)
-        *reinterpret_cast<float4*>(mo + r * L::HROW + 2 * j) = make_float4(o[j][r], o[j][r + 2], o[j + 1][r], o[j + 1][r + 2]);
-    if (t == 0) stat[warp][g][0] = m, stat[warp][g][1] = M, stat[warp][g][2] = l;
-    __syncthreads();
+    // ---- the warps' outputs meet in shared memory (each in its own ring), a set after the other ----
     const bool whole = ua == 0 && ub == rw.units;
-    float* rec = records + (size_t)(2 * c + (start == first ? 0 : 1)) * L::REC;
-    {
-      constexpr int PER = HD * HEADS / THREADS;  // consecutive dims of one head per thread
+    const uint32_t mine = start == first ? 0 : 1;
+    if (!whole && tid == 0 && ua == 0)
+      headers[c] = Header{(int32_t)row, (int32_t)item, (int32_t)(((base + (uint64_t)(item + 1) * span) * C - 1) / U),
+                          (int32_t)(mine + 2 * (MANY ? rw.rows : 1))};
+#pragma unroll
+    for (int x = 0; x < SETS; ++x) {
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+      // lane (g, t): slots 2t and 2t + 1, the HD / 8 dims from HD / 8 g
+      float* mo = reinterpret_cast<float*>(att_smem + warp * L::RING) + 2 * t * L::HROW + g * (HD / 8);
+      __syncwarp();
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int j = 0; j < HD / 16; j += 2)
+          *reinterpret_cast<float4*>(mo + r * L::HROW + 2 * j) =
+              make_float4(o[x][j][r], o[x][j][r + 2], o[x][j + 1][r], o[x][j + 1][r + 2]);
+      if (t == 0) stat[warp][g][0] = m[x], stat[warp][g][1] = M[x], stat[warp][g][2] = l[x];
+      __syncthreads();
+      float* rec = records + ((size_t)(2 * c + mine) * SETS + x) * L::REC;
+      constexpr int PER = HD * HEADS / THREADS;  // consecutive dims of one slot per thread
       const uint32_t h = tid / (HD / PER), d = (tid % (HD / PER)) * PER;
       float mm = -INFINITY, MM = -INFINITY, ll = 0.f;
 #pragma unroll
@@ -543,16 +599,17 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
         const float lw = stat[w][h][2];
         if (lw == 0.f) continue;  // a warp without positions
         ll += lw * ex2(stat[w][h][0] - mm);
-        const float x = ex2(stat[w][h][1] - MM);
+        const float f = ex2(stat[w][h][1] - MM);
         const float* src = reinterpret_cast<const float*>(att_smem + w * L::RING) + h * L::HROW + d;
 #pragma unroll
-        for (int e = 0; e < PER; ++e) out[e] += src[e] * x;
+        for (int e = 0; e < PER; ++e) out[e] += src[e] * f;
       }
       if (whole) {
-        if (h < n_heads) {
+        const uint32_t slot = HEADS * x + h;
+        if (slot < slots) {
           // MM - mm is at most the largest exponent of a scale
           const float f = ll == 0.f ? 0.f : ex2(MM - mm - 14.f) / ll;
-          const size_t at = row * a.out_stride + (size_t)((sub * HEADS + h) * n_kv + kvh) * HD + d;
+          const size_t at = slot_row(slot) * a.out_stride + slot_dim(slot) + d;
 #pragma unroll
           for (int e = 0; e < PER; ++e) store_dt(a.out, at + e, a.dtype, ll == 0.f ? 0.f : out[e] * f);
         }
@@ -561,29 +618,27 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attend_kernel(const __gr
         for (int e = 0; e < PER; e += 4)
           *reinterpret_cast<float4*>(rec + h * HD + d + e) = make_float4(out[e], out[e + 1], out[e + 2], out[e + 3]);
         if (d == 0) rec[HEADS * HD + h] = mm, rec[HEADS * (HD + 1) + h] = MM, rec[HEADS * (HD + 2) + h] = ll;
-        if (tid == 0 && ua == 0)
-          headers[c] = Header{(int32_t)row, (int32_t)item, (int32_t)(((base + (uint64_t)(item + 1) * span) * C - 1) / U),
-                              start == first ? 0 : 1};
       }
+      __syncthreads();  // the rings and stat are free again
     }
-    __syncthreads();  // the rings and stat are free again
     }
     if (next_row) {
       base = s;
-      do rw = row_of(a, ++row);
+      do rw = row_of<MANY>(a, ++row);
       while (rw.units == 0);
     }
   }
 }
 
-// Joins the pieces of the item that begins in CTA blockIdx.x's part.  Its time
+// Joins the pieces of set blockIdx.y of the item that begins in CTA blockIdx.x's part.  Its time
 // is that of loads that wait on one another, so there are two such waits: for the
 // header, then for the pieces' (max, sum) together with their outputs (4 dims a
 // thread, the pieces dealt to the thread groups, the first 8 of a group held in
 // registers meanwhile).
-template <int HD, int THREADS_J>
+template <int HD, int SETS, int THREADS_J>
 __global__ void __launch_bounds__(THREADS_J) attend_join_kernel(const __grid_constant__ PagesAttnArgs a) {
-  using L = Lay<HD>;
+  using L = Lay<HD, SETS>;
+  constexpr uint32_t SLOTS = SETS * HEADS;
   constexpr uint32_t PER_GROUP = HEADS * HD / 4, GROUPS = THREADS_J / PER_GROUP, HELD = 8;
   __shared__ float weight[HEADS][MAX_CTAS + 1];  // of a piece's outputs
   __shared__ float fin[HEADS];
@@ -593,9 +648,9 @@ __global__ void __launch_bounds__(THREADS_J) attend_join_kernel(const __grid_con
   const Header hd = static_cast<const Header*>(a.ws)[c];
   if (hd.row < 0) return;
   const float* records = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.ws) + MAX_CTAS * sizeof(Header));
-  const uint32_t n_kv = a.pool.n_kv, G = a.n_heads / n_kv, nsub = (G + HEADS - 1) / HEADS;
+  const uint32_t n_kv = a.pool.n_kv, G = a.group, nsub = a.subs;
   const uint32_t kvh = hd.item / nsub, sub = hd.item % nsub, n = (uint32_t)hd.last - c + 1;
-  auto rec = [&](uint32_t i) { return records + (size_t)(2 * (c + i) + (i == 0 ? hd.slot : 0)) * L::REC; };
+  auto rec = [&](uint32_t i) { return records + ((size_t)(2 * (c + i) + (i == 0 ? hd.slot_rows & 1 : 0)) * SETS + blockIdx.y) * L::REC; };
   const uint32_t grp = tid / PER_GROUP, e = tid % PER_GROUP, h = e / (HD / 4);
   float4 x[HELD];
 #pragma unroll
@@ -633,33 +688,40 @@ __global__ void __launch_bounds__(THREADS_J) attend_join_kernel(const __grid_con
   for (uint32_t i = grp + HELD * GROUPS; i < n; i += GROUPS) add(reinterpret_cast<const float4*>(rec(i))[e], i);
   sum[tid] = o;
   __syncthreads();
-  if (grp || sub * HEADS + h >= G) return;
+  const uint32_t slot = HEADS * blockIdx.y + h, rows = (uint32_t)hd.slot_rows >> 1;
+  if (grp || slot >= (nsub == 1 ? rows * G : min(G - sub * SLOTS, SLOTS))) return;
 #pragma unroll
   for (uint32_t k = 1; k < GROUPS; ++k) {
     const float4 v = sum[k * PER_GROUP + e];
     o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
   }
   const float f = fin[h];
-  const size_t at = (uint32_t)hd.row * a.out_stride + (size_t)((sub * HEADS + h) * n_kv + kvh) * HD + 4 * (e % (HD / 4));
+  const uint32_t in = nsub == 1 ? slot * a.inv_group >> 16 : 0, row = (uint32_t)hd.row + in, head = sub * SLOTS + slot - in * G;
+  const size_t at = row * a.out_stride + (size_t)(head * n_kv + kvh) * HD + 4 * (e % (HD / 4));
   store_dt(a.out, at, a.dtype, o.x * f);
   store_dt(a.out, at + 1, a.dtype, o.y * f);
   store_dt(a.out, at + 2, a.dtype, o.z * f);
   store_dt(a.out, at + 3, a.dtype, o.w * f);
 }
 
-template <int HD, uint32_t TYPE>
-cudaError_t attend_go(const PagesAttnArgs& a, int num_sms, cudaStream_t st) {
-  const uint32_t ctas = (uint32_t)min(num_sms * CTAS_PER_SM, MAX_CTAS);
-  cudaError_t e = launch_k(attend_kernel<HD, TYPE>, dim3(ctas), dim3(THREADS), Lay<HD>::BYTES, st, a);
+template <int HD, uint32_t TYPE, int SETS, bool MANY>
+cudaError_t attend_sets(PagesAttnArgs a, int num_sms, cudaStream_t st) {
+  using L = Lay<HD, SETS>;
+  constexpr uint32_t SLOTS = SETS * HEADS;
+  a.group = a.n_heads / a.pool.n_kv;
+  a.subs = (a.group + SLOTS - 1) / SLOTS;
+  a.window = MANY && a.row_seq && a.group < SLOTS ? SLOTS / a.group : 1;
+  a.inv_group = 65536 / a.group + 1;
+  const uint32_t ctas = (uint32_t)min(num_sms * L::CTAS, MAX_CTAS);
+  cudaError_t e = launch_k(attend_kernel<HD, TYPE, SETS, MANY>, dim3(ctas), dim3(THREADS), L::BYTES, st, a);
   if (e != cudaSuccess) return e;
   // the join waits for the kernel above by itself (griddepcontrol.wait)
   // Few items are cut into many pieces each, and only their first CTAs have any
   // to join: large blocks (1 x 8192, 32 pieces an item: 8.4 us against 11).  Many
   // items are cut in two or three, by almost every CTA: small ones.
-  const uint32_t G = a.n_heads / a.pool.n_kv;
-  const bool many = (uint64_t)a.n_rows * a.pool.n_kv * ((G + HEADS - 1) / HEADS) * 4 > ctas;
+  const bool many = (uint64_t)a.n_rows * a.pool.n_kv * a.subs * 4 > ctas;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas);
+  cfg.gridDim = dim3(ctas, SETS);
   cfg.blockDim = dim3(many ? 256 : 1024);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -667,22 +729,45 @@ cudaError_t attend_go(const PagesAttnArgs& a, int num_sms, cudaStream_t st) {
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return many ? cudaLaunchKernelEx(&cfg, attend_join_kernel<HD, 256>, a) : cudaLaunchKernelEx(&cfg, attend_join_kernel<HD, 1024>, a);
+  return many ? cudaLaunchKernelEx(&cfg, attend_join_kernel<HD, SETS, 256>, a)
+              : cudaLaunchKernelEx(&cfg, attend_join_kernel<HD, SETS, 1024>, a);
+}
+
+template <int HD, uint32_t TYPE>
+cudaError_t attend_go(const PagesAttnArgs& a, int num_sms, cudaStream_t st) {
+  // Where a request's rows have more than 8 heads for a KV head, two sets of slots
+  // share what is read and converted, and three CTAs fit an SM instead of four:
+  // 32 requests of 2000 positions, 4 rows of 64 heads over 8 of 128: 84 us with
+  // one set, 76 with two; 24 heads over 2, one row: 29 and 27; 64 x 4 rows of 32
+  // heads over 4 of 64, 2048 positions: 70 and 62; at 8 heads one set is all it takes.
+  // Rows of one request share an item of one set as well: 5 rows of 16 heads over 16:
+  // 111 us apart, 51 together.  The search for such rows costs other calls 0.5 us
+  // of instruction fetches, so they go without.
+  const uint64_t G = a.n_heads / a.pool.n_kv;
+  if (a.n_rows * G > (uint64_t)HEADS * min(a.n_seq, a.n_rows)) return attend_sets<HD, TYPE, 2, true>(a, num_sms, st);
+  return a.row_seq && a.n_rows > a.n_seq ? attend_sets<HD, TYPE, 1, true>(a, num_sms, st)
+                                         : attend_sets<HD, TYPE, 1, false>(a, num_sms, st);
+}
+
+template <int HD, uint32_t TYPE>
+cudaError_t attend_attributes() {
+  const auto big = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  cudaError_t e = cudaFuncSetAttribute(attend_kernel<HD, TYPE, 1, false>, big, Lay<HD, 1>::BYTES);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(attend_kernel<HD, TYPE, 1, true>, big, Lay<HD, 1>::BYTES);
+  return e == cudaSuccess ? cudaFuncSetAttribute(attend_kernel<HD, TYPE, 2, true>, big, Lay<HD, 2>::BYTES) : e;
 }
 
 }  // namespace
 
 size_t pages_attend_ws_bytes(uint32_t, uint32_t, uint32_t, uint32_t hd) {
-  return MAX_CTAS * (sizeof(Header) + 2 * 4 * (size_t)(hd == 64 ? Lay<64>::REC : Lay<128>::REC));
+  return MAX_CTAS * (sizeof(Header) + 2 * 2 * 4 * (size_t)(hd == 64 ? Lay<64, 2>::REC : Lay<128, 2>::REC));
 }
 
 cudaError_t pages_attend_init() {
-  const auto big = cudaFuncAttributeMaxDynamicSharedMemorySize;
-  cudaError_t e = cudaFuncSetAttribute(attend_kernel<64, PAGES_I8>, big, Lay<64>::BYTES);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(attend_kernel<64, PAGES_E4M3>, big, Lay<64>::BYTES);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(attend_kernel<128, PAGES_I8>, big, Lay<128>::BYTES);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(attend_kernel<128, PAGES_E4M3>, big, Lay<128>::BYTES);
-  return e;
+  cudaError_t e = attend_attributes<64, PAGES_I8>();
+  if (e == cudaSuccess) e = attend_attributes<64, PAGES_E4M3>();
+  if (e == cudaSuccess) e = attend_attributes<128, PAGES_I8>();
+  return e == cudaSuccess ? attend_attributes<128, PAGES_E4M3>() : e;
 }
 
 cudaError_t pages_attend_launch(const PagesAttnArgs& a, int num_sms, cudaStream_t st) {

@@ -443,8 +443,9 @@ def attend_reference(q, K, V, table, seq, pos, block, n_heads, scale):
     return out, lim
 
 
-def run_attend(ctx, pool, rng, lens, rows, n_heads, dtype, pad=0, qgain=1.0, poison=True, stream=None):
-    """Attention of `rows` rows per request against the reference; returns the device arrays.  Everything that no row may
+def run_attend(ctx, pool, rng, lens, rows, n_heads, dtype, pad=0, qgain=1.0, poison=True, stream=None, plan=None):
+    """Attention of `rows` rows per request, or of plan's (request, position) rows in their order, against the
+    reference; returns the device arrays.  Everything that no row may
     see is poisoned: places behind each request's end, and blocks of nobody."""
     blocks, n_kv, block, hd = pool.shape
     stride = max(1, max(-(-n // block) for n in lens)) + 1
@@ -468,7 +469,7 @@ def run_attend(ctx, pool, rng, lens, rows, n_heads, dtype, pad=0, qgain=1.0, poi
     seq = [z for z in range(len(lens)) for _ in range(rows)] + [-1] * pad
     pos = [n - rows + j for n in lens for j in range(rows)] + [5] * pad
     order = rng.permutation(len(seq))
-    seq, pos = np.array(seq)[order], np.array(pos)[order]
+    seq, pos = (np.array(x) for x in zip(*plan)) if plan else (np.array(seq)[order], np.array(pos)[order])
     w = n_heads * hd
     q = to_dev((rng.normal(0, 1, (len(seq), w + 24)) * qgain).astype(np.float32)).to(TORCH[dtype])
     out = torch.full((len(seq), w + 16), 7.0, device="cuda", dtype=TORCH[dtype])
@@ -518,6 +519,52 @@ def test_attend_long_and_many(ctx, dtype, rows, block, lens):
     rng = np.random.default_rng(rows + block)
     pool = Pool(ctx, rng, sum(-(-n // block) for n in lens) + 2, 2, block, 128, sc.PAGES_E4M3 if rows == 3 else sc.PAGES_I8)
     run_attend(ctx, pool, rng, lens, rows, 16, dtype, pad=3)
+
+
+@gpu
+@pytest.mark.parametrize("kind", [sc.PAGES_I8, sc.PAGES_E4M3])
+@pytest.mark.parametrize("H,KV,hd", [(8, 8, 64), (16, 8, 128), (6, 2, 64), (32, 8, 128), (10, 2, 128), (16, 2, 64),
+                                     (24, 2, 128), (16, 1, 128), (40, 1, 64)])
+@pytest.mark.parametrize("block,lens,most", [(16, [40, 1, 0, 150], 7), (64, [70, 2500], 20), (16, [33] * 60, 5)])
+def test_attend_rows_of_one_request(ctx, kind, H, KV, hd, block, lens, most):
+    """Rows of one request side by side, in any number and order: other positions, the same one twice, ones that see
+    nothing, padding between them, requests that come again."""
+    rng = np.random.default_rng(H * hd + most)
+    pool = Pool(ctx, rng, sum(-(-n // block) for n in lens) + 2, KV, block, hd, kind)
+    plan = []
+    for z in [*range(len(lens)), *rng.permutation(len(lens))[:3]]:
+        top = lens[z]
+        at = rng.integers(-1, top, rng.integers(0, most + 1)) if top else np.full(rng.integers(0, 3), -1)
+        plan += [(z, int(t)) for t in at] + [(-1, 3)] * int(rng.random() < 0.2)
+    plan += [(0, lens[0] - 1)] * 3
+    run_attend(ctx, pool, rng, lens, 0, H, 30 if kind else 0, plan=plan)
+
+
+@gpu
+@pytest.mark.parametrize("scale", [np.inf, np.nan])
+def test_attend_hidden_scales(ctx, scale):
+    """A block that only the longer row of a request sees, with a scale that is no number: nothing to the others."""
+    rng = np.random.default_rng(6)
+    plan, lens, block = [(0, 10), (0, 39), (0, 31), (0, 7)], [40], 16
+    for kind, H, KV, hd in ((sc.PAGES_I8, 8, 4, 64), (sc.PAGES_E4M3, 32, 4, 64), (sc.PAGES_I8, 8, 2, 128)):
+        pool = Pool(ctx, rng, 6, KV, block, hd, kind)
+        table = rng.permutation(6)[:3].reshape(1, 3)
+        K, V = pool.values()
+        for i in range(2):
+            pool.hs[i][table[0, 2]] = scale
+            pool.ds[i].copy_(torch.from_numpy(pool.hs[i]))
+        seq, pos = (np.array(x) for x in zip(*plan))
+        q = rng.normal(0, 1, (4, H, hd)).astype(np.float32)
+        qd, out = to_dev(q), torch.full((4, H * hd), 7.0, device="cuda")
+        ws = torch.empty(sc.pages_attend_ws(4, H, KV, hd), dtype=torch.uint8, device="cuda")
+        td, sd, pd = dev(table), dev(seq), dev(pos)
+        pool.pages.attend(4, p(qd), p(out), H, p(pd), p(td), 3, 1, 0.125, p(ws), ws.numel(), row_seq=p(sd))
+        ctx.check()
+        ref, lim = attend_reference(q, K, V, table, seq, pos, block, H, 0.125)
+        got = out.double().cpu().numpy().reshape(ref.shape)
+        see = [0, 2, 3]
+        assert np.all(np.abs(got - ref)[see] <= lim[see])
+        assert not np.isfinite(got[1]).any()
 
 
 @gpu
