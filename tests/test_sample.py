@@ -145,6 +145,21 @@ def test_sample_many_ties(ctx, vocab, settings):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("spread,vocab", [(1.6, 128256), (2.2, 100003), (0.5, 32000), (1.0, 40000)])
+@pytest.mark.parametrize("settings", [(1.0, None, 0.97, None), (1.0, None, 0.83, 0.02), (1.0, 30011, None, None),
+                                      (1.0, 20001, 0.9, None)])
+def test_sample_crowded_border(ctx, dtype, spread, vocab, settings):
+    """Flat rows: some hundred tokens and more share the border's bin, in 16 bits many with the same logit."""
+    rng = np.random.default_rng(vocab + dtype)
+    z = rng.normal(0, spread, (5, vocab)).astype(np.float32)
+    u = rng.random(5)
+    first = check(ctx, z, u, settings, dtype)
+    again = check(ctx, z, u, settings, dtype)
+    assert all((x == y).all() for x, y in zip(first, again))
+
+
+@gpu
 def test_sample_masked(ctx):
     """-inf, the type's lowest value, NaN and +inf among the logits; a row with nothing left; one token left."""
     rng = np.random.default_rng(2)
