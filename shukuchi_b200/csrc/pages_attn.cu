@@ -236,64 +236,58 @@ __global__ void __launch_bounds__(THREADS, Lay<HD, SETS>::CTAS) attend_kernel(co
 
   // ---- this CTA's part of the line of units ----
   if (tid == 0) headers[c] = Header{-1, 0, 0, 0};
-  // cost of this thread's row (the first THREADS rows), running sums over the warp and the CTA
+  // Its first unit's row: each thread sums what its share of the rows cost, the
+  // sums are summed over the CTA, and the share that has the unit is dealt out
+  // again until it is one row (65535 rows: three times).
   auto cost = [](const Row& r) -> uint32_t { return r.units ? r.units + ITEM_UNITS : 0; };
-  auto scan = [&](uint32_t n, uint64_t& total) -> uint64_t {  // inclusive; one barrier before the next call
-    uint64_t v = n;
+  Row rw{-1, 0, 0, 0};
+  uint64_t s = 0, end = 0, U = 0, before = 0;
+  uint32_t C = 0, row = 0;
+  for (uint32_t left = a.n_rows;;) {
+    const uint32_t per = (left + THREADS - 1) / THREADS;
+    const uint32_t r0 = row + tid * per, r1 = min(row + left, r0 + per);
+    uint64_t mine = 0, upto;
+#pragma unroll 2
+    for (uint32_t r = r0; r < r1; ++r) {
+      rw = row_of<MANY>(a, r);
+      mine += cost(rw);
+    }
+    upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t u = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= (uint32_t)o) v += u;
+      const uint64_t u = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= (uint32_t)o) upto += u;
     }
-    if (lane == 31) sums.warp[warp] = v;
+    if (lane == 31) sums.warp[warp] = upto;
     __syncthreads();
-    total = 0;
+    uint64_t total = 0;
 #pragma unroll
     for (uint32_t w = 0; w < WARPS; ++w) {
-      if (w < warp) v += sums.warp[w];
+      if (w < warp) upto += sums.warp[w];
       total += sums.warp[w];
     }
-    return v;
-  };
-  Row rw = tid < a.n_rows ? row_of<MANY>(a, tid) : Row{-1, 0, 0, 0};
-  uint64_t total;
-  uint64_t upto = scan(cost(rw), total);
-  uint64_t carry = total;
-  if (a.n_rows > THREADS) {
-    uint64_t more = 0;
-    for (uint32_t r = THREADS + tid; r < a.n_rows; r += THREADS) more += cost(row_of<MANY>(a, r));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
-    __syncthreads();
-    if (lane == 0) sums.warp[warp] = more;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) total += sums.warp[w];
-  }
-  const uint64_t U = NI * total, want = U / MIN_UNITS;
-  const uint32_t C = want < 1 ? 1 : want < gridDim.x ? (uint32_t)want : gridDim.x;
-  if (c >= C || U == 0) return;
-  uint64_t s = c * U / C;
-  const uint64_t first = s, end = (c + 1) * U / C;
-  for (uint32_t r0 = 0;; r0 += THREADS) {  // the row that unit s belongs to
-    if (r0) {
-      __syncthreads();
-      rw = r0 + tid < a.n_rows ? row_of<MANY>(a, r0 + tid) : Row{-1, 0, 0, 0};
-      uint64_t n;
-      upto = carry + scan(cost(rw), n);
-      carry += n;
+    if (left == a.n_rows) {
+      U = NI * total;
+      const uint64_t want = U / MIN_UNITS;
+      C = want < 1 ? 1 : want < gridDim.x ? (uint32_t)want : gridDim.x;
+      if (c >= C || U == 0) return;
+      s = c * U / C;
+      end = (c + 1) * U / C;
     }
-    const uint64_t lo = NI * (upto - cost(rw));
-    if (rw.units && s >= lo && s < NI * upto) {
-      sums.row = r0 + tid;
-      sums.base = lo;
+    upto += before;
+    if (mine && s >= NI * (upto - mine) && s < NI * upto) {
+      sums.row = r0;
+      sums.base = upto - mine;
       sums.at = rw;
     }
-    if (s < NI * carry || r0 + THREADS >= a.n_rows) break;
+    __syncthreads();
+    row = sums.row;
+    before = sums.base;
+    if (per == 1) break;
+    left = min(per, a.n_rows - row);
   }
-  __syncthreads();
-  uint32_t row = sums.row;
-  uint64_t base = sums.base;
+  const uint64_t first = s;
+  uint64_t base = NI * before;
   rw = sums.at;
 
   const uint32_t ring = smem_u32(att_smem) + warp * L::RING;

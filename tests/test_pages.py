@@ -541,6 +541,20 @@ def test_attend_rows_of_one_request(ctx, kind, H, KV, hd, block, lens, most):
 
 
 @gpu
+@pytest.mark.parametrize("n_rows,live", [(1000, [0, 127, 128, 999]), (20000, [5, 6, 7, 19999]), (65535, [511, 512, 40000, 65534]),
+                                         (65535, [])])
+def test_attend_rows_far_apart(ctx, n_rows, live):
+    """Few rows among many padding rows: the first ones, the last one, none."""
+    rng = np.random.default_rng(n_rows)
+    lens = [40, 3]
+    pool = Pool(ctx, rng, 6, 2, 16, 64, sc.PAGES_I8)
+    plan = [(-1, 3)] * n_rows
+    for i, r in enumerate(live):
+        plan[r] = (i % 2, lens[i % 2] - 1)
+    run_attend(ctx, pool, rng, lens, 0, 2, 0, plan=plan)
+
+
+@gpu
 @pytest.mark.parametrize("scale", [np.inf, np.nan])
 def test_attend_hidden_scales(ctx, scale):
     """A block that only the longer row of a request sees, with a scale that is no number: nothing to the others."""
