@@ -88,6 +88,8 @@ __global__ void __launch_bounds__(TAB_THREADS) assign_kernel(const __grid_consta
   const uint32_t bs = a.block_shift, bt = 1u << bs;
   const uint32_t rank = cluster_rank(), ctas = cluster_ctas();
   const int64_t cap = (int64_t)a.stride << bs;
+  pdl_trigger();
+  pdl_wait();
   int32_t n_free = *a.n_free;
   if (threadIdx.x < 3) tally[threadIdx.x] = 0;
   if (n_free < 0 || n_free > (int32_t)a.n_blocks) {
@@ -199,6 +201,8 @@ __global__ void __launch_bounds__(TAB_THREADS) release_kernel(const __grid_const
   int32_t* start = tab_sm;  // first freed block of each request
   const uint32_t bs = a.block_shift, bt = 1u << bs;
   const uint32_t rank = cluster_rank(), ctas = cluster_ctas();
+  pdl_trigger();
+  pdl_wait();
   const int32_t n_free = *a.n_free;
   uint64_t total = 0;
   bool bad = false;
@@ -234,20 +238,9 @@ __global__ void __launch_bounds__(TAB_THREADS) release_kernel(const __grid_const
 
 template <typename Args>
 cudaError_t tables_go(void (*kernel)(Args), const Args& a, uint32_t rows, uint32_t arrays, cudaStream_t st) {
-  const uint32_t most = a.n_seq > rows ? a.n_seq : rows;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(rows > TAB_ROWS ? TAB_CLUSTER : 1);
-  cfg.blockDim = dim3(most >= TAB_THREADS ? TAB_THREADS : (most + 127) / 128 * 128);
-  cfg.dynamicSmemBytes = arrays * 4 * a.n_seq;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cfg.gridDim.x;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, a);
+  const uint32_t most = a.n_seq > rows ? a.n_seq : rows, ctas = rows > TAB_ROWS ? TAB_CLUSTER : 1;
+  return launch_early(kernel, ctas, dim3(ctas), dim3(most >= TAB_THREADS ? TAB_THREADS : (most + 127) / 128 * 128),
+                         arrays * 4 * a.n_seq, st, a);
 }
 
 // ---- append ----
@@ -328,10 +321,10 @@ template <uint32_t DT>
 __device__ __forceinline__ uint4 load_piece(const void* x, size_t at, bool wide) {
   if constexpr (DT == DT_F32) {
     const uint32_t* u = static_cast<const uint32_t*>(x) + at;
-    return wide ? __ldg(reinterpret_cast<const uint4*>(u)) : make_uint4(u[0], u[1], u[2], u[3]);
+    return wide ? *reinterpret_cast<const uint4*>(u) : make_uint4(u[0], u[1], u[2], u[3]);
   } else {
     const unsigned short* u = static_cast<const unsigned short*>(x) + at;
-    if (wide) return __ldg(reinterpret_cast<const uint4*>(u));
+    if (wide) return *reinterpret_cast<const uint4*>(u);
     auto two = [&](int i) { return (uint32_t)u[i] | (uint32_t)u[i + 1] << 16; };
     return make_uint4(two(0), two(2), two(4), two(6));
   }
@@ -419,6 +412,8 @@ __global__ void __launch_bounds__(APP_THREADS, 4) append_kernel(PagesPool p, uin
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bs = p.block_shift, bt = 1u << bs;
   const uint32_t first_pair = blockIdx.y * pairs, n_pairs = min(pairs, 2 * p.n_kv - first_pair);
 
+  pdl_trigger();
+  pdl_wait();
   const uint64_t t_lo = (uint64_t)blockIdx.x * tokens, t_hi = min((uint64_t)n, t_lo + tokens);
   for (uint64_t t0 = t_lo; t0 < t_hi; t0 += APP_TOKENS) {
     // ---- the runs that begin here ----
@@ -471,7 +466,7 @@ __global__ void __launch_bounds__(APP_THREADS, 4) append_kernel(PagesPool p, uin
       j0 = look & ~3u;
 #pragma unroll 4
       for (uint32_t j = 4 * tid; j < j0; j += 4 * APP_THREADS) {
-        const int4 v = __ldg(reinterpret_cast<const int4*>(slots + j));
+        const int4 v = *reinterpret_cast<const int4*>(slots + j);
         if (maybe(v.x) | maybe(v.y) | maybe(v.z) | maybe(v.w)) refuse_runs(run_block, run_t, run_len, count, slots, j, 4, bs, err);
       }
     }
@@ -557,6 +552,8 @@ template <uint32_t TYPE>
 __global__ void __launch_bounds__(256) read_kernel(PagesPool p, uint32_t n, const int32_t* slots, float* k, float* v,
                                                    bool wide, int* err) {
   const uint32_t quads = p.n_kv * p.hd / 4;  // of a row
+  pdl_trigger();
+  pdl_wait();
   const uint64_t total = (uint64_t)n * quads;
   for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x) {
     const uint32_t r = (uint32_t)(i / quads), d = 4 * (uint32_t)(i % quads);
@@ -601,9 +598,8 @@ struct AppendCall {
 
 template <int HD, uint32_t TYPE, uint32_t DT>
 cudaError_t append_go(const PagesPool& p, const AppendCall& c) {
-  append_kernel<HD, TYPE, DT><<<c.grid, APP_THREADS, 0, c.st>>>(p, c.n, c.k, c.v, c.row_stride, c.wide, c.slots, c.tokens,
-                                                               c.pairs, c.err);
-  return cudaGetLastError();
+  return launch_early(append_kernel<HD, TYPE, DT>, 1, c.grid, dim3(APP_THREADS), 0, c.st, p, c.n, c.k, c.v, c.row_stride, c.wide,
+                  c.slots, c.tokens, c.pairs, c.err);
 }
 template <int HD, uint32_t TYPE>
 cudaError_t append_dt(const PagesPool& p, uint32_t dtype, const AppendCall& c) {
@@ -654,11 +650,8 @@ cudaError_t pages_read_launch(const PagesPool& p, uint32_t n, const int32_t* slo
   const uint64_t ctas = ((uint64_t)n * p.n_kv * p.hd / 4 + 255) / 256, most = (uint64_t)num_sms * 32;
   const bool wide = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
   const dim3 grid((uint32_t)(ctas < most ? ctas : most));
-  if (p.type == PAGES_I8)
-    read_kernel<PAGES_I8><<<grid, 256, 0, st>>>(p, n, slots, k, v, wide, err);
-  else
-    read_kernel<PAGES_E4M3><<<grid, 256, 0, st>>>(p, n, slots, k, v, wide, err);
-  return cudaGetLastError();
+  return launch_early(p.type == PAGES_I8 ? read_kernel<PAGES_I8> : read_kernel<PAGES_E4M3>, 1, grid, dim3(256), 0, st, p, n, slots, k,
+                  v, wide, err);
 }
 
 }  // namespace shk

@@ -707,24 +707,15 @@ cudaError_t attend_sets(PagesAttnArgs a, int num_sms, cudaStream_t st) {
   a.window = MANY && a.row_seq && a.group < SLOTS ? SLOTS / a.group : 1;
   a.inv_group = 65536 / a.group + 1;
   const uint32_t ctas = (uint32_t)min(num_sms * L::CTAS, MAX_CTAS);
-  cudaError_t e = launch_k(attend_kernel<HD, TYPE, SETS, MANY>, dim3(ctas), dim3(THREADS), L::BYTES, st, a);
+  cudaError_t e = launch_early(attend_kernel<HD, TYPE, SETS, MANY>, 1, dim3(ctas), dim3(THREADS), L::BYTES, st, a);
   if (e != cudaSuccess) return e;
   // the join waits for the kernel above by itself (griddepcontrol.wait)
   // Few items are cut into many pieces each, and only their first CTAs have any
   // to join: large blocks (1 x 8192, 32 pieces an item: 8.4 us against 11).  Many
   // items are cut in two or three, by almost every CTA: small ones.
   const bool many = (uint64_t)a.n_rows * a.pool.n_kv * a.subs * 4 > ctas;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas, SETS);
-  cfg.blockDim = dim3(many ? 256 : 1024);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return many ? cudaLaunchKernelEx(&cfg, attend_join_kernel<HD, SETS, 256>, a)
-              : cudaLaunchKernelEx(&cfg, attend_join_kernel<HD, SETS, 1024>, a);
+  return launch_early(many ? attend_join_kernel<HD, SETS, 256> : attend_join_kernel<HD, SETS, 1024>, 1, dim3(ctas, SETS),
+                      dim3(many ? 256 : 1024), 0, st, a);
 }
 
 template <int HD, uint32_t TYPE>

@@ -743,6 +743,8 @@ template <uint32_t DT>
 __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constant__ SampleArgs a, uint32_t slice) {
   extern __shared__ __align__(16) uint8_t sample_smem[];
   cl_begun();
+  pdl_trigger();
+  pdl_wait();
   float* z = reinterpret_cast<float*>(sample_smem);
   Shared& s = *reinterpret_cast<Shared*>(sample_smem + sizeof(float) * slice);
   const uint32_t rank = cl_rank(), cl = cl_size(), row = blockIdx.x / cl;
@@ -763,7 +765,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     done = n / PER * PER;
 #pragma unroll 4
     for (uint32_t i = tid; i < n / PER; i += THREADS) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
+      const uint4 v = reinterpret_cast<const uint4*>(src)[i];
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int e = 0; e < PER; e += 4) {
@@ -836,19 +838,7 @@ cudaError_t sample_go(const SampleArgs& a, int num_sms, cudaStream_t st) {
   while (cl < MAX_CL && (a.n_vocab > cl * 16384 || (a.n_rows * cl * 2 <= (uint32_t)num_sms && a.n_vocab > cl * 2048))) cl *= 2;
   const uint32_t slice = ((a.n_vocab + cl - 1) / cl + 127) / 128 * 128;
   const size_t smem = sizeof(float) * slice + sizeof(Shared);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.n_rows * cl);
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cl;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sample_kernel<DT>, a, slice);
+  return launch_early(sample_kernel<DT>, cl, dim3(a.n_rows * cl), dim3(THREADS), smem, st, a, slice);
 }
 
 }  // namespace
