@@ -8,6 +8,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <mutex>
 #include <new>
 #include <unordered_map>
@@ -889,6 +890,13 @@ static bool act_dtype(uint32_t dt) { return dt == DT_F32 || dt == DT_F16 || dt =
 
 static bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
+// Arrays of 32-bit words, null ones included.
+static bool words(std::initializer_list<const void*> all) {
+  for (const void* p : all)
+    if (!aligned(p, 4)) return false;
+  return true;
+}
+
 static int pages_pool(const shk_pages* p, PagesPool* out) {
   if (!p || !p->k_dev || !p->v_dev || !p->k_scale_dev || !p->v_scale_dev || !p->n_kv_heads) return SHK_EINVAL;
   if (!aligned(p->k_dev, 16) || !aligned(p->v_dev, 16) || !aligned(p->k_scale_dev, 4) || !aligned(p->v_scale_dev, 4))
@@ -913,6 +921,9 @@ int shk_cuda_pages_assign(shk_ctx* c, const shk_pages_assign* a, void* s) {
       !a->counts_dev || !a->last_dev)
     return SHK_EINVAL;
   if (a->n_rows && (!a->slots_dev || !a->pos_dev || !a->seq_dev)) return SHK_EINVAL;
+  if (!words({a->have_dev, a->add_dev, a->table_dev, a->free_dev, a->n_free_dev, a->lens_dev, a->counts_dev, a->last_dev,
+              a->slots_dev, a->pos_dev, a->seq_dev}))
+    return SHK_EINVAL;
   AssignArgs g{};
   if (!pages_dims(a->n_blocks, a->block_tokens, &g.block_shift)) return SHK_EINVAL;
   if (!a->n_seq || a->n_seq > SHK_PAGES_MAX_SEQ || !a->table_stride || a->n_rows > 0x3FFFFFFFu) return SHK_EINVAL;
@@ -941,6 +952,7 @@ int shk_cuda_pages_release(shk_ctx* c, uint32_t n_seq, uint32_t block_tokens, ui
                            int32_t* free_ids, const int32_t* n_free, int32_t* n_free_out, void* s) {
   if (c) on_dev(c);
   if (!c || !table || !done || !have || !lens || !free_ids || !n_free || !n_free_out) return SHK_EINVAL;
+  if (!words({table, done, have, lens, free_ids, n_free, n_free_out})) return SHK_EINVAL;
   ReleaseArgs g{};
   if (!pages_dims(n_blocks, block_tokens, &g.block_shift)) return SHK_EINVAL;
   if (!n_seq || n_seq > SHK_PAGES_MAX_SEQ || !table_stride) return SHK_EINVAL;
@@ -968,7 +980,7 @@ int shk_cuda_pages_append(shk_ctx* c, const shk_pages* p, uint32_t n_tokens, con
   if (n_tokens == 0) return SHK_OK;
   if (!act_dtype(dtype)) return SHK_EUNSUPPORTED;
   const size_t width = (size_t)g.n_kv * g.hd, es = dtype == DT_F32 ? 4 : 2;
-  if (!k || !v || !slots || !aligned(k, es) || !aligned(v, es) || n_tokens > 0x7FFFFFFFu ||
+  if (!k || !v || !slots || !aligned(k, es) || !aligned(v, es) || !words({slots}) || n_tokens > 0x7FFFFFFFu ||
       (row_stride && row_stride < width))
     return SHK_EINVAL;
   CK(pages_append_launch(g, n_tokens, k, v, dtype, row_stride ? row_stride : width, slots, c->d_err, c->num_sms,
@@ -983,7 +995,7 @@ int shk_cuda_pages_read(shk_ctx* c, const shk_pages* p, uint32_t n_tokens, const
   const int rc = c ? pages_pool(p, &g) : SHK_EINVAL;
   if (rc) return rc;
   if (n_tokens == 0) return SHK_OK;
-  if (!k || !v || !slots || !aligned(k, 4) || !aligned(v, 4) || n_tokens > 0x7FFFFFFFu) return SHK_EINVAL;
+  if (!k || !v || !slots || !words({k, v, slots}) || n_tokens > 0x7FFFFFFFu) return SHK_EINVAL;
   CK(pages_read_launch(g, n_tokens, slots, k, v, c->d_err, c->num_sms, pick(c, s)));
   return SHK_OK;
 }
@@ -1004,6 +1016,7 @@ int shk_cuda_pages_attend(shk_ctx* c, const shk_pages* p, const shk_pages_rows* 
   const size_t width = (size_t)r->n_heads * g.pool.hd, es = r->dtype == DT_F32 ? 4 : 2;
   if (!r->n_heads || r->n_heads % g.pool.n_kv || r->n_heads > 4096 || !r->q_dev || !r->out_dev || !r->pos_dev ||
       !r->table_dev || !r->table_stride || !r->n_seq || !aligned(r->q_dev, es) || !aligned(r->out_dev, es) ||
+      !words({r->seq_dev, r->pos_dev, r->table_dev}) ||
       (r->q_stride && r->q_stride < width) || (r->out_stride && r->out_stride < width) ||
       (!r->seq_dev && r->n_rows > r->n_seq) || r->n_rows > SHK_PAGES_MAX_ROWS ||
       (uint64_t)r->table_stride * p->block_tokens > 0x7FFFFFFFull)
@@ -1041,7 +1054,8 @@ int shk_cuda_sample(shk_ctx* c, const void* logits, uint32_t dtype, uint32_t n_r
   if (!c || !n_vocab || (row_stride && row_stride < n_vocab)) return SHK_EINVAL;
   if (n_rows == 0) return SHK_OK;
   if (!act_dtype(dtype) || n_vocab > SHK_SAMPLE_MAX_VOCAB) return SHK_EUNSUPPORTED;
-  if (!logits || !u || !out || !aligned(logits, dtype == DT_F32 ? 4 : 2) || n_rows > SHK_PAGES_MAX_ROWS)
+  if (!logits || !u || !out || !aligned(logits, dtype == DT_F32 ? 4 : 2) || n_rows > SHK_PAGES_MAX_ROWS ||
+      !words({temperature, top_k, top_p, min_p, u, out, prob}))
     return SHK_EINVAL;
   const SampleArgs g{logits, dtype, n_rows, n_vocab, row_stride ? row_stride : n_vocab, temperature, top_k, top_p,
                      min_p,  u,     out,    prob};

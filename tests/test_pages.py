@@ -213,6 +213,37 @@ def test_table_arguments(ctx):
     ctx.check()
 
 
+@gpu
+def test_arrays_of_words_are_aligned(ctx):
+    """Every int32 and float array two bytes off: refused before any launch."""
+    t = Tables([1], [1], [[0]], [0] * 4, 1, 1)
+    x = torch.zeros(4096, device="cuda")
+    i = p(t.have)
+    for at in range(11):
+        with pytest.raises(sc.ShkError):
+            ctx.pages_assign(1, 16, 4, 1, 1, *[i + 2 * (j == at) for j in range(11)])
+    for at in range(7):
+        with pytest.raises(sc.ShkError):
+            ctx.pages_release(1, 16, 4, 1, *[i + 2 * (j == at) for j in range(7)])
+    pool = Pool(ctx, np.random.default_rng(1), 2, 1, 16, 64, sc.PAGES_I8)
+    with pytest.raises(sc.ShkError):
+        pool.pages.append(1, p(x), p(x), i + 2)
+    for at in range(3):
+        with pytest.raises(sc.ShkError):
+            pool.pages.read(1, *[(i if j == 0 else p(x)) + 2 * (j == at) for j in range(3)])
+    ws = torch.zeros(sc.pages_attend_ws(1, 1, 1, 64), dtype=torch.uint8, device="cuda")
+    for bad in ("row_pos", "table", "row_seq"):
+        arrays = {n: i + 2 * (n == bad) for n in ("row_pos", "table", "row_seq")}
+        with pytest.raises(sc.ShkError):
+            pool.pages.attend(1, p(x), p(x) + 4096, 1, table_stride=1, n_seq=1, scale=1.0, ws=p(ws), ws_bytes=ws.numel(), **arrays)
+    names = ("u", "out", "prob", "temperature", "top_k", "top_p", "min_p")
+    for bad in names:
+        with pytest.raises(sc.ShkError):
+            ctx.sample(p(x), 1, 8, **{n: i + 2 * (n == bad) for n in names})
+    ctx.check()
+    pool.same()
+
+
 # ---- append and read ----
 
 E4M3 = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).float().numpy()
@@ -552,6 +583,26 @@ def test_attend_rows_far_apart(ctx, n_rows, live):
     for i, r in enumerate(live):
         plan[r] = (i % 2, lens[i % 2] - 1)
     run_attend(ctx, pool, rng, lens, 0, 2, 0, plan=plan)
+
+
+@gpu
+@pytest.mark.parametrize("H,KV,hd", [(8, 4, 64), (16, 2, 64), (32, 8, 128)])
+def test_attend_bad_queries_stay_alone(ctx, H, KV, hd):
+    """Rows of one request, every other one NaN or infinite: the ones between are what they are alone."""
+    rng = np.random.default_rng(7)
+    pool = Pool(ctx, rng, 4, KV, 16, hd, sc.PAGES_E4M3)
+    table, seq, pos = rng.permutation(4)[:3].reshape(1, 3), np.zeros(6, int), np.array([47, 40, 41, 3, 20, 47])
+    q = rng.normal(0, 1, (6, H, hd)).astype(np.float32)
+    ref, lim = attend_reference(q, *pool.values(), table, seq, pos, 16, H, 0.125)
+    q[1::2, :, 5] = np.array([np.nan, np.inf, -np.inf])[:, None]
+    qd, out = to_dev(q), torch.full((6, H * hd), 7.0, device="cuda")
+    ws = torch.empty(sc.pages_attend_ws(6, H, KV, hd), dtype=torch.uint8, device="cuda")
+    td, sd, pd = dev(table), dev(seq), dev(pos)
+    pool.pages.attend(6, p(qd), p(out), H, p(pd), p(td), 3, 1, 0.125, p(ws), ws.numel(), row_seq=p(sd))
+    ctx.check()
+    got = out.double().cpu().numpy().reshape(ref.shape)
+    assert np.all(np.abs(got - ref)[::2] <= lim[::2])
+    assert not np.isfinite(got[1]).any()
 
 
 @gpu
