@@ -18,9 +18,11 @@ namespace {
 // the lengths for itself (no exchange), and the rows, each of which looks up its
 // request and its block, are dealt to all.  The cluster's barrier separates the
 // last read of the inputs from the writes to arrays that may be the same.
+// Release and assign of 1024 requests with 50k rows 14.7 us together, of 64
+// requests 8.8 (five of them the two calls' own).
 constexpr int TAB_THREADS = 1024;
 constexpr int TAB_CLUSTER = 8;
-constexpr uint32_t TAB_ROWS = 2048;  // rows that one CTA takes alone: 1024 requests' 50k rows took 57 us on one CTA, 12 on 8
+constexpr uint32_t TAB_ROWS = 2048;  // rows that one CTA takes alone (1024 requests, 50k rows: 57 us on one CTA, 12 on 8; 64 rows: the same)
 
 __device__ __forceinline__ uint64_t warp_scan64(uint64_t v, uint32_t lane) {
 #pragma unroll
@@ -397,6 +399,10 @@ __device__ __noinline__ void refuse_runs(const uint32_t* run_block, const uint32
 // A block whose rows come in two runs of one call would be written by two CTAs at
 // once: the later run is refused, so each CTA looks through the earlier tokens for
 // the blocks of its own runs (a bit per hashed block first).
+//
+// 6300 tokens of bf16 (8 heads of 128) into e4m3 blocks of 64: 21 us (1.8 TB/s) in
+// a row of calls, bound by instructions (22 an element, most of them the two
+// roundings of round4) at 0.5 a cycle and by 3 or 4 CTAs on an SM; 32 tokens 5 us.
 template <int HD, uint32_t TYPE, uint32_t DT>
 __global__ void __launch_bounds__(APP_THREADS, 4) append_kernel(PagesPool p, uint32_t n, const void* k, const void* v,
                                                                 size_t row_stride, bool wide, const int32_t* slots,
@@ -547,7 +553,8 @@ __global__ void __launch_bounds__(APP_THREADS, 4) append_kernel(PagesPool p, uin
   }
 }
 
-// Four values a thread: 4 bytes in, 16 out, both whole lines to a warp.
+// Four values a thread: 4 bytes in, 16 out, both whole lines to a warp.  Bound by
+// memory: 6300 tokens of 8 x 128 (64 MB) 11.7 us, 5.5 TB/s.
 template <uint32_t TYPE>
 __global__ void __launch_bounds__(256) read_kernel(PagesPool p, uint32_t n, const int32_t* slots, float* k, float* v,
                                                    bool wide, int* err) {
