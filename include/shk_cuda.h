@@ -250,7 +250,8 @@ uint32_t shk_cuda_kv_seq_len(shk_kv *kv, uint32_t layer);
  *      shk_cuda_sample on the logits.  All of it is stream-ordered and reads
  *      lengths on the device only, so a captured step can be replayed.
  *
- *      Lengths, slots, positions and block ids are int32.  A bad one (a block
+ *      Lengths, slots, positions and block ids are int32, and every array of
+ *      them or of floats is 4-byte aligned (else SHK_EINVAL).  A bad value (a block
  *      id outside the pool, a position outside the table, a slot outside the
  *      pool) is left out and recorded: shk_cuda_check returns SHK_EDEVICE. ---- */
 #define SHK_PAGES_I8 0u   /* signed integers -127..127 */

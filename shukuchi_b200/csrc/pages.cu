@@ -22,7 +22,9 @@ namespace {
 // requests 8.8 (five of them the two calls' own).
 constexpr int TAB_THREADS = 1024;
 constexpr int TAB_CLUSTER = 8;
-constexpr uint32_t TAB_ROWS = 2048;  // rows that one CTA takes alone (1024 requests, 50k rows: 57 us on one CTA, 12 on 8; 64 rows: the same)
+// Rows that one CTA takes alone (1024 requests, 50k rows: 57 us on one CTA, 12 on
+// 8; 64 rows: the same).
+constexpr uint32_t TAB_ROWS = 2048;
 
 __device__ __forceinline__ uint64_t warp_scan64(uint64_t v, uint32_t lane) {
 #pragma unroll

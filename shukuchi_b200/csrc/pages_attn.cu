@@ -32,7 +32,7 @@
 // 270 to 290 us, 5.6 to 6.0 TB/s; 32 of 1 to 8192, i8, 65 us, 4.3 TB/s, of which
 // the join is 9; one of 8192 16.4 us, one of 777 (32 heads) 11 us, both chains of
 // loads that wait on one another.  64 x 4 rows of 100 to 2000 positions (32 heads
-// over 4 of 64) 42 us: instructions, 770 a warp's step of 32 positions for 16
+// over 4 of 64) 41 us: instructions, 770 a warp's step of 32 positions for 16
 // slots at 0.54 a cycle.  Five and six CTAs an SM there: 47 and 52 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -54,7 +54,9 @@ constexpr int STEP = 2 * SUB;   // positions of a warp's step
 constexpr int UNIT = STEP * WARPS;
 constexpr int CTAS_PER_SM = 4;  // 128 registers a thread (two sets: 3, 168)
 constexpr int MAX_CTAS = 640;   // 4 x the SMs of a B200 (148), rounded up
-constexpr int ITEM_UNITS = 2;   // what an item costs besides its positions, in units (32 ragged rows with 0, 1, 2: 78, 66, 66 us; 64 x 4: 62, 47, 45)
+// What an item costs besides its positions, in units (32 ragged rows with 0, 1, 2:
+// 78, 66, 66 us; 64 x 4: 62, 47, 45).
+constexpr int ITEM_UNITS = 2;
 constexpr int MIN_UNITS = 2;    // a CTA's part: shorter ones cost more in joining than they save
 
 template <int HD, int SETS>
@@ -524,7 +526,8 @@ __global__ void __launch_bounds__(THREADS, Lay<HD, SETS>::CTAS) attend_kernel(co
 #pragma unroll
         for (int x = 0; x < SETS; ++x) {
           float wt[4];
-          const float f = (int32_t)(len[x] - place(i, h)) <= 0 ? 0.f : vf[h];  // (an infinite scale of positions that the slot does not see)
+          // (an infinite scale of positions that the slot does not see)
+          const float f = (int32_t)(len[x] - place(i, h)) <= 0 ? 0.f : vf[h];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float y = sv[x][2 * h + (e >> 1)][e & 1];
@@ -631,16 +634,18 @@ __global__ void __launch_bounds__(THREADS, Lay<HD, SETS>::CTAS) attend_kernel(co
   }
 }
 
-// Joins the pieces of set blockIdx.y of the item that begins in CTA blockIdx.x's part.  Its time
-// is that of loads that wait on one another, so there are two such waits: for the
-// header, then for the pieces' (max, sum) together with their outputs (4 dims a
-// thread, the pieces dealt to the thread groups, the first 8 of a group held in
+// Joins the pieces of set blockIdx.y of the item that begins in CTA blockIdx.x's
+// part.  Its time is that of loads that wait on one another, so there are two such
+// waits: for the header, then for the pieces' (max, sum) together with their outputs (4 dims a
+// thread, the pieces dealt to the thread groups, the first HELD of a group held in
 // registers meanwhile).
 template <int HD, int SETS, int THREADS_J>
 __global__ void __launch_bounds__(THREADS_J) attend_join_kernel(const __grid_constant__ PagesAttnArgs a) {
   using L = Lay<HD, SETS>;
   constexpr uint32_t SLOTS = SETS * HEADS;
-  constexpr uint32_t PER_GROUP = HEADS * HD / 4, GROUPS = THREADS_J / PER_GROUP, HELD = 8;
+  constexpr uint32_t PER_GROUP = HEADS * HD / 4, GROUPS = THREADS_J / PER_GROUP;
+  // (8 in a small block of two groups: 64 x 4 rows 42.3 us, 4: 41.0)
+  constexpr uint32_t HELD = THREADS_J == 256 ? 8 / GROUPS : 8;
   __shared__ float weight[HEADS][MAX_CTAS + 1];  // of a piece's outputs
   __shared__ float fin[HEADS];
   __shared__ float4 sum[THREADS_J];

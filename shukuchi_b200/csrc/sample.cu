@@ -91,7 +91,8 @@ struct Scale {
   __device__ __forceinline__ float weight(float z) const { return expf(x(z)); }
 };
 // Rises as x falls, from bin 0 on; NB for a token without weight.
-__device__ __forceinline__ float bin_float(float x) { return __fmaf_rd(x, NB / X_MIN, 8388608.f); }  // 2^23 + the bin, above it without weight
+// (2^23 + the bin, or more than 2^23 + NB.)
+__device__ __forceinline__ float bin_float(float x) { return __fmaf_rd(x, NB / X_MIN, 8388608.f); }
 __device__ __forceinline__ int bin_of(float x) {
   return x > X_MIN ? (int)(__float_as_uint(bin_float(x)) - 0x4B000000u) : NB;
 }
