@@ -836,9 +836,12 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
 
 template <uint32_t DT>
 cudaError_t sample_go(const SampleArgs& a, int num_sms, cudaStream_t st) {
-  // As many CTAs a row as its slice needs, more while the rows leave SMs idle.
+  // As many CTAs a row as its slice needs, more while the rows leave SMs idle: down
+  // to 8192 logits each, as below that the cluster's exchanges cost more than the
+  // shorter slices save (a row of 32000, top-p: 14.1 us with 8 CTAs, 13.6 with 4,
+  // 15.5 with 2; 128256: 22 with 4, 18.7 with 8, 21 with 16).
   uint32_t cl = 1;
-  while (cl < MAX_CL && (a.n_vocab > cl * 16384 || (a.n_rows * cl * 2 <= (uint32_t)num_sms && a.n_vocab > cl * 2048))) cl *= 2;
+  while (cl < MAX_CL && (a.n_vocab > cl * 16384 || (a.n_rows * cl * 2 <= (uint32_t)num_sms && a.n_vocab > cl * 8192))) cl *= 2;
   const uint32_t slice = ((a.n_vocab + cl - 1) / cl + 127) / 128 * 128;
   const size_t smem = sizeof(float) * slice + sizeof(Shared);
   return launch_early(sample_kernel<DT>, cl, dim3(a.n_rows * cl), dim3(THREADS), smem, st, a, slice);
