@@ -628,8 +628,10 @@ __global__ void __launch_bounds__(THREADS, Lay<HD, SETS>::CTAS) attend_kernel(co
     }
     if (next_row) {
       base = s;
-      do rw = row_of<MANY>(a, ++row);
-      while (rw.units == 0);
+      do {
+        if (++row >= a.n_rows) return;  // (positions that were changed during the call)
+        rw = row_of<MANY>(a, row);
+      } while (rw.units == 0);
     }
   }
 }
