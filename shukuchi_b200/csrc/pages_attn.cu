@@ -32,7 +32,7 @@
 // 270 to 290 us, 5.6 to 6.0 TB/s; 32 of 1 to 8192, i8, 65 us, 4.3 TB/s, of which
 // the join is 9; one of 8192 16.4 us, one of 777 (32 heads) 11 us, both chains of
 // loads that wait on one another.  64 x 4 rows of 100 to 2000 positions (32 heads
-// over 4 of 64) 41 us: instructions, 770 a warp's step of 32 positions for 16
+// over 4 of 64) 40 us: instructions, 770 a warp's step of 32 positions for 16
 // slots at 0.54 a cycle.  Five and six CTAs an SM there: 47 and 52 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -72,7 +72,7 @@ struct Lay {
   static constexpr int HROW = HD + 4;           // floats of a head's outputs in shared memory, padded
   static constexpr int BYTES = WARPS * RING + SETS * QF;
   static constexpr int REC = HEADS * (HD + 3);  // floats of a piece's record of one set: O, m, M, l
-  static_assert(HEADS * HROW * 4 <= RING, "a warp's output fits its ring");
+  static_assert(SETS * HEADS * HROW * 4 <= RING, "a warp's output fits its ring");
 };
 
 struct Header {  // the item that begins in a CTA's part and ends in a later one's
@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(THREADS, Lay<HD, SETS>::CTAS) attend_kernel(co
   extern __shared__ __align__(16) uint8_t att_smem[];
   __shared__ Sums sums;
   __shared__ int32_t qmax[SLOTS];
-  __shared__ float stat[WARPS][HEADS][3];
+  __shared__ float stat[WARPS][SLOTS][3];
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const uint32_t c = blockIdx.x, bs = a.pool.block_shift, n_kv = a.pool.n_kv, G = a.group;
   const uint32_t nsub = a.subs, NI = n_kv * nsub;
@@ -570,41 +570,44 @@ __global__ void __launch_bounds__(THREADS, Lay<HD, SETS>::CTAS) attend_kernel(co
     }
     copy_wait<0>();
 
-    // ---- the warps' outputs meet in shared memory (each in its own ring), a set after the other ----
+    // ---- the warps' outputs meet in shared memory (each in its own ring) ----
     const bool whole = ua == 0 && ub == rw.units;
     const uint32_t mine = start == first ? 0 : 1;
     if (!whole && tid == 0 && ua == 0)
       headers[c] = Header{(int32_t)row, (int32_t)item, (int32_t)(((base + (uint64_t)(item + 1) * span) * C - 1) / U),
                           (int32_t)(mine + 2 * (MANY ? rw.rows : 1))};
+    __syncwarp();
 #pragma unroll
     for (int x = 0; x < SETS; ++x) {
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
       // lane (g, t): slots 2t and 2t + 1, the HD / 8 dims from HD / 8 g
-      float* mo = reinterpret_cast<float*>(att_smem + warp * L::RING) + 2 * t * L::HROW + g * (HD / 8);
-      __syncwarp();
+      float* mo = reinterpret_cast<float*>(att_smem + warp * L::RING) + (HEADS * x + 2 * t) * L::HROW + g * (HD / 8);
 #pragma unroll
       for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int j = 0; j < HD / 16; j += 2)
           *reinterpret_cast<float4*>(mo + r * L::HROW + 2 * j) =
               make_float4(o[x][j][r], o[x][j][r + 2], o[x][j + 1][r], o[x][j + 1][r + 2]);
-      if (t == 0) stat[warp][g][0] = m[x], stat[warp][g][1] = M[x], stat[warp][g][2] = l[x];
-      __syncthreads();
+      if (t == 0) stat[warp][HEADS * x + g][0] = m[x], stat[warp][HEADS * x + g][1] = M[x], stat[warp][HEADS * x + g][2] = l[x];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < SETS; ++x) {
       float* rec = records + ((size_t)(2 * c + mine) * SETS + x) * L::REC;
       constexpr int PER = HD * HEADS / THREADS;  // consecutive dims of one slot per thread
       const uint32_t h = tid / (HD / PER), d = (tid % (HD / PER)) * PER;
       float mm = -INFINITY, MM = -INFINITY, ll = 0.f;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, stat[w][h][0]), MM = fmaxf(MM, stat[w][h][1]);
+      for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, stat[w][HEADS * x + h][0]), MM = fmaxf(MM, stat[w][HEADS * x + h][1]);
       float out[PER] = {};
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
-        const float lw = stat[w][h][2];
+        const float lw = stat[w][HEADS * x + h][2];
         if (lw == 0.f) continue;  // a warp without positions
-        ll += lw * ex2(stat[w][h][0] - mm);
-        const float f = ex2(stat[w][h][1] - MM);
-        const float* src = reinterpret_cast<const float*>(att_smem + w * L::RING) + h * L::HROW + d;
+        ll += lw * ex2(stat[w][HEADS * x + h][0] - mm);
+        const float f = ex2(stat[w][HEADS * x + h][1] - MM);
+        const float* src = reinterpret_cast<const float*>(att_smem + w * L::RING) + (HEADS * x + h) * L::HROW + d;
 #pragma unroll
         for (int e = 0; e < PER; ++e) out[e] += src[e] * f;
       }
@@ -623,8 +626,8 @@ __global__ void __launch_bounds__(THREADS, Lay<HD, SETS>::CTAS) attend_kernel(co
           *reinterpret_cast<float4*>(rec + h * HD + d + e) = make_float4(out[e], out[e + 1], out[e + 2], out[e + 3]);
         if (d == 0) rec[HEADS * HD + h] = mm, rec[HEADS * (HD + 1) + h] = MM, rec[HEADS * (HD + 2) + h] = ll;
       }
-      __syncthreads();  // the rings and stat are free again
     }
+    __syncthreads();  // the rings and stat are free again
     }
     if (next_row) {
       base = s;
