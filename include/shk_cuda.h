@@ -281,8 +281,11 @@ struct shk_pages {
  * have[r], its rows -1, no block taken -- when its tokens outgrow table_stride
  * blocks, its rows outgrow n_rows, or its blocks and those asked for by the
  * requests before it outgrow the free stack; rows are counted as if every
- * request before it had been served.  lens_dev may be have_dev, and counts_dev
- * may be n_free_dev.  One launch; async on stream. */
+ * request before it had been served.  A row whose block id (of the table or the
+ * free stack) lies outside the pool gets -1 in all three arrays as well, and so
+ * does last[r] where it is the request's last one; the table gets -1 for such a
+ * new block, and lens[r] and the counts are as if the id were good.  lens_dev may
+ * be have_dev, and counts_dev may be n_free_dev.  One launch; async on stream. */
 struct shk_pages_assign {
     uint32_t n_seq;        /* request slots: 1 .. SHK_PAGES_MAX_SEQ */
     uint32_t block_tokens; /* 16 .. 256, a power of two */

@@ -147,14 +147,18 @@ __global__ void __launch_bounds__(TAB_THREADS) assign_kernel(const __grid_consta
     fresh = b >= have_blocks;
     return fresh ? a.free_ids + (base[q] - (int32_t)(b - have_blocks)) : a.table + (size_t)q * a.stride + b;
   };
-  auto slot_of = [&](int32_t id, uint32_t q, int32_t pos, bool fresh) -> int32_t {
-    if ((uint32_t)id >= a.n_blocks) {
-      set_error(a.err, DERR_BAD_POS);
-      return -1;
-    }
+  // The row's slot.  A row whose block id lies outside the pool is nobody's either;
+  // such a new block leaves -1 in the table, so that no later call takes what
+  // stood there before for the request's.
+  auto slot_of = [&](int32_t id, uint32_t r, int32_t& pos, int32_t& seq, bool fresh) -> int32_t {
+    const uint32_t at = (uint32_t)pos & (bt - 1);
+    const bool good = (uint32_t)id < a.n_blocks;
     // a new block's first token is always one of the rows
-    if (fresh && ((uint32_t)pos & (bt - 1)) == 0) a.table[(size_t)q * a.stride + ((uint32_t)pos >> bs)] = id;
-    return (int32_t)(((uint32_t)id << bs) + ((uint32_t)pos & (bt - 1)));
+    if (fresh && at == 0) a.table[(size_t)seq * a.stride + ((uint32_t)pos >> bs)] = good ? id : -1;
+    if (good) return (int32_t)(((uint32_t)id << bs) + at);
+    set_error(a.err, DERR_BAD_POS);
+    if (a.last[seq] == (int32_t)r) a.last[seq] = -1;  // (written before the barrier above)
+    return pos = seq = -1;
   };
   const uint32_t me = rank * blockDim.x + threadIdx.x, all = ctas * blockDim.x;
   if (a.n_rows <= all) {
@@ -163,9 +167,10 @@ __global__ void __launch_bounds__(TAB_THREADS) assign_kernel(const __grid_consta
     int32_t pos;
     bool fresh = false;
     const int32_t* at = look_up(me, q, pos, fresh);
-    a.slots[me] = at ? slot_of(*at, q, pos, fresh) : -1;
+    int32_t seq = at ? (int32_t)q : -1;
+    a.slots[me] = at ? slot_of(*at, me, pos, seq, fresh) : -1;
     a.pos[me] = pos;
-    a.seq[me] = at ? (int32_t)q : -1;
+    a.seq[me] = seq;
     return;
   }
   // many rows: four a thread, with one search and 16-byte stores where the arrays allow
@@ -186,7 +191,7 @@ __global__ void __launch_bounds__(TAB_THREADS) assign_kernel(const __grid_consta
 #pragma unroll
     for (int i = 0; i < 4; ++i) id[i] = at[i] ? *at[i] : 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) slot[i] = at[i] ? slot_of(id[i], (uint32_t)seq[i], pos[i], fresh[i]) : -1;
+    for (int i = 0; i < 4; ++i) slot[i] = at[i] ? slot_of(id[i], r0 + i, pos[i], seq[i], fresh[i]) : -1;
     if (wide && r0 + 3 < a.n_rows) {
       *reinterpret_cast<int4*>(a.slots + r0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
       *reinterpret_cast<int4*>(a.pos + r0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
