@@ -305,8 +305,11 @@ int shk_cuda_pages_assign(shk_ctx *ctx, const struct shk_pages_assign *a, void *
 /* Gives the blocks of the requests with done[r] != 0 back: pushed on the free
  * stack in request and table order, lens[r] = 0 (have[r] for the others), the
  * new height to n_free_out_dev.  lens_dev may be have_dev, n_free_out_dev may be
- * n_free_dev.  Where the stack would outgrow n_blocks (a block given back
- * twice) nothing is given back and shk_cuda_check returns SHK_EDEVICE. */
+ * n_free_dev.  Ids outside the pool are left out, the others close up (what
+ * free_dev holds above the new height is of no account); a request whose have[r]
+ * is negative or more than its table row holds keeps it and gives nothing back.
+ * Where the stack would outgrow n_blocks (a block given back twice) nothing is
+ * given back at all.  shk_cuda_check returns SHK_EDEVICE after each of these. */
 int shk_cuda_pages_release(shk_ctx *ctx, uint32_t n_seq, uint32_t block_tokens, uint32_t n_blocks,
                            uint32_t table_stride, const int32_t *table_dev, const int32_t *done_dev,
                            const int32_t *have_dev, int32_t *lens_dev, int32_t *free_dev,

@@ -18,8 +18,8 @@ namespace {
 // the lengths for itself (no exchange), and the rows, each of which looks up its
 // request and its block, are dealt to all.  The cluster's barrier separates the
 // last read of the inputs from the writes to arrays that may be the same.
-// Release and assign of 1024 requests with 50k rows 14.7 us together, of 64
-// requests 8.8 (five of them the two calls' own).
+// Release and assign of 1024 requests with 50k rows 15.6 us together, of 64
+// requests 9.0 (five of them the two calls' own).
 constexpr int TAB_THREADS = 1024;
 constexpr int TAB_CLUSTER = 8;
 // Rows that one CTA takes alone (1024 requests, 50k rows: 57 us on one CTA, 12 on
@@ -74,10 +74,25 @@ __device__ __forceinline__ uint32_t cluster_ctas() {
   asm volatile("mov.u32 %0, %cluster_nctarank;" : "=r"(r));
   return r;
 }
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // All CTAs of the cluster have read what this kernel may overwrite.
 __device__ __forceinline__ void cluster_barrier() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_arrive();
+  cluster_wait();
+}
+
+// One word of CTA `rank`'s shared memory.
+__device__ __forceinline__ void cluster_put(const uint32_t* word, uint32_t rank, uint32_t v) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(word)), "r"(rank));
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
 }
 
 // Rows and new blocks are two running sums over the requests, both in the
@@ -204,44 +219,73 @@ __global__ void __launch_bounds__(TAB_THREADS) assign_kernel(const __grid_consta
   }
 }
 
+// Ids outside the pool are looked for where they are copied, and closed up behind
+// that by one CTA, which has to wait for the others' word (0.8 us with 8 CTAs).
 __global__ void __launch_bounds__(TAB_THREADS) release_kernel(const __grid_constant__ ReleaseArgs a) {
   extern __shared__ int32_t tab_sm[];
   __shared__ uint64_t part[32];
+  __shared__ uint32_t odd_ids;  // CTA 0's: some CTA met an id outside the pool
   int32_t* start = tab_sm;  // first freed block of each request
   const uint32_t bs = a.block_shift, bt = 1u << bs;
   const uint32_t rank = cluster_rank(), ctas = cluster_ctas();
   pdl_trigger();
   pdl_wait();
   const int32_t n_free = *a.n_free;
+  if (threadIdx.x == 0) odd_ids = 0;
   uint64_t total = 0;
-  bool bad = false;
+  // the blocks that request r gives back; a length that its table row cannot hold: none
+  auto given = [&](uint32_t r) -> uint32_t {
+    const int32_t h = a.have[r];
+    if (a.done[r] == 0) return 0;
+    const uint64_t n = h > 0 ? ((uint64_t)h + bt - 1) >> bs : 0;
+    return n <= a.stride ? (uint32_t)n : 0;
+  };
+  auto wrong = [&](int32_t h) { return h < 0 || ((uint64_t)h + bt - 1) >> bs > a.stride; };
   for (uint32_t r0 = 0; r0 < a.n_seq; r0 += blockDim.x) {
     const uint32_t r = r0 + threadIdx.x;
-    uint64_t n = 0;
-    int32_t h = 0, done = 0;
-    if (r < a.n_seq) h = a.have[r], done = a.done[r];
-    if (done != 0) {
-      n = h > 0 ? ((uint64_t)h + bt - 1) >> bs : 0;
-      if (h < 0 || n > a.stride) bad = true, n = 0;
-    }
+    const uint64_t n = r < a.n_seq ? given(r) : 0;
     const uint64_t end = block_scan64(n, total, part);
     if (r < a.n_seq) start[r] = (int32_t)min(end - n, (uint64_t)a.n_blocks);
   }
   // a stack that would outgrow the pool means blocks given back twice
-  bad = __syncthreads_or(bad || n_free < 0 || (int64_t)n_free + (int64_t)total > (int64_t)a.n_blocks);
+  const bool bad = n_free < 0 || (int64_t)n_free + (int64_t)total > (int64_t)a.n_blocks;
+  __syncthreads();
   if (ctas > 1) cluster_barrier();
-  if (bad && threadIdx.x == 0) set_error(a.err, DERR_BAD_POS);
+  bool odd = false;
   for (uint32_t i = rank * blockDim.x + threadIdx.x; !bad && i < total; i += ctas * blockDim.x) {
     const uint32_t q = owner_of(start, a.n_seq, (int32_t)i);
     const int32_t id = a.table[(size_t)q * a.stride + (i - start[q])];
-    if ((uint32_t)id >= a.n_blocks) set_error(a.err, DERR_BAD_POS);
+    odd |= (uint32_t)id >= a.n_blocks;
     a.free_ids[n_free + i] = id;
+  }
+  odd = __syncthreads_or(odd);
+  if (ctas > 1) {  // CTA 0 alone waits for the others' ids, and writes the lengths meanwhile
+    if (odd && rank && threadIdx.x == 0) cluster_put(&odd_ids, 0, 1);
+    cluster_arrive();
   }
   if (rank) return;
   for (uint32_t r = threadIdx.x; r < a.n_seq; r += blockDim.x) {
     const int32_t h = a.have[r];
-    a.lens[r] = !bad && a.done[r] != 0 ? 0 : h;
+    const bool done = a.done[r] != 0;
+    if (done && wrong(h)) set_error(a.err, DERR_BAD_POS);
+    a.lens[r] = done && !bad && !wrong(h) ? 0 : h;
   }
+  if (ctas > 1) {
+    cluster_wait();
+    odd |= odd_ids != 0;
+  }
+  if (odd) {  // the others move up, a block's worth at a time: all of it is read before any of it is written
+    uint64_t kept = 0;
+    for (uint32_t i0 = 0; i0 < total; i0 += blockDim.x) {
+      const uint32_t i = i0 + threadIdx.x;
+      const int32_t id = i < total ? a.free_ids[n_free + i] : -1;
+      const bool good = (uint32_t)id < a.n_blocks;
+      const uint64_t end = block_scan64(good, kept, part);
+      if (good) a.free_ids[n_free + (int32_t)end - 1] = id;
+    }
+    total = kept;
+  }
+  if ((bad || odd) && threadIdx.x == 0) set_error(a.err, DERR_BAD_POS);
   if (threadIdx.x == 0) *a.n_free_out = bad ? n_free : n_free + (int32_t)total;
 }
 

@@ -60,3 +60,33 @@ def test_a_bad_block_stays_out_of_the_steps_behind_it(ctx):
         ctx.check()
         pool.same()
         assert (out == 7).all()
+
+
+@pytest.mark.parametrize("n,stride", [(3, 4), (40, 30), (1200, 9)])
+def test_release_leaves_out_bad_ids(ctx, n, stride):
+    """Every seventh id is outside the pool: the others go back in order, the height counts them alone."""
+    rng = np.random.default_rng(n)
+    n_blocks = 3 * n * stride
+    have, done = rng.integers(0, 16 * stride + 1, n), rng.integers(0, 2, n)
+    table = rng.permutation(n_blocks)[: n * stride].reshape(n, stride)
+    hurt = np.where(rng.random(table.shape) < 1 / 7, rng.choice([-1, n_blocks, -2 ** 31, 2 ** 31 - 1], table.shape), table)
+    hurt[-1, 0], have[-1], done[-1] = n_blocks, max(1, have[-1]), 1
+    free = np.full(n_blocks, -9)
+    free[:5] = [1, 2, 3, 4, 5]
+    h, d, t, f, height = dev(have), dev(done), dev(hurt), dev(free), dev([5])
+    lens = dev(np.full(n, -5))
+    ctx.pages_release(n, 16, n_blocks, stride, p(t), p(d), p(h), p(lens), p(f), p(height), p(height))
+    refused(ctx)
+    back = [i for r in range(n) if done[r] for i in hurt[r, : -(-have[r] // 16)] if 0 <= i < n_blocks]
+    assert height.item() == 5 + len(back)
+    assert f.tolist()[: 5 + len(back)] == free[:5].tolist() + back
+    assert np.array_equal(lens.cpu().numpy(), np.where(done != 0, 0, have))
+
+
+def test_release_leaves_out_bad_lengths(ctx):
+    """A negative length and one that its table row cannot hold stay as they are; the other requests' blocks go back."""
+    table, have, done = dev([[0, 1], [2, 3], [4, 5], [6, 7]]), dev([32, -3, 33, 16]), dev([1, 1, 1, 5])
+    free, height, lens = dev([8, 9] + [-9] * 8), dev([2]), dev([-5] * 4)
+    ctx.pages_release(4, 16, 10, 2, p(table), p(done), p(have), p(lens), p(free), p(height), p(height))
+    refused(ctx)
+    assert lens.tolist() == [0, -3, 33, 0] and height.item() == 5 and free.tolist()[:5] == [8, 9, 0, 1, 6]
