@@ -245,8 +245,8 @@ uint32_t shk_cuda_kv_seq_len(shk_kv *kv, uint32_t layer);
  *      struct shk_pages describes one layer's.
  *
  *      A step of a batch: shk_cuda_pages_release (blocks of the requests that
- *      ended), shk_cuda_pages_assign (blocks, slots, positions of the new
- *      tokens), per layer shk_cuda_pages_append and shk_cuda_pages_attend, then
+ *      ended) or shk_cuda_pages_truncate (of those that were cut short as well),
+ *      shk_cuda_pages_assign (blocks, slots, positions of the new tokens), per layer shk_cuda_pages_append and shk_cuda_pages_attend, then
  *      shk_cuda_sample on the logits.  All of it is stream-ordered and reads
  *      lengths on the device only, so a captured step can be replayed.
  *
@@ -272,7 +272,7 @@ struct shk_pages {
     uint32_t block_tokens;            /* 16, 32, 64, 128 or 256 */
 };
 /* Block tables and slots from lengths.  Request r holds have[r] tokens in the
- * blocks table[r][0 ..] and gets add[r] more.  Requests are served in order:
+ * blocks table[r][0 ..], have[r] / block_tokens of them rounded up, and gets add[r] more.  Requests are served in order:
  * their rows (one per new token) are laid out one request after the other, and
  * a new block of theirs is taken from the top of the free stack
  * free_dev[0 .. *n_free_dev).  Row i: slots[i] = block * block_tokens + place in
@@ -314,6 +314,17 @@ int shk_cuda_pages_release(shk_ctx *ctx, uint32_t n_seq, uint32_t block_tokens, 
                            uint32_t table_stride, const int32_t *table_dev, const int32_t *done_dev,
                            const int32_t *have_dev, int32_t *lens_dev, int32_t *free_dev,
                            const int32_t *n_free_dev, int32_t *n_free_out_dev, void *stream);
+/* Requests cut short, as after rejected draft tokens: r keeps its first keep[r]
+ * tokens (all where keep[r] >= have[r], 0: as if it had ended), lens[r] =
+ * min(keep[r], have[r]), and the blocks that hold none of them go back, like
+ * shk_cuda_pages_release's; a negative keep[r] counts as a bad length.  lens_dev
+ * may be have_dev or keep_dev.  shk_cuda_pages_assign takes a request's blocks
+ * from have[r] alone: a length lowered in any other way loses the blocks behind
+ * it.  The scales of a block that is kept stay what its dropped tokens made them. */
+int shk_cuda_pages_truncate(shk_ctx *ctx, uint32_t n_seq, uint32_t block_tokens, uint32_t n_blocks,
+                            uint32_t table_stride, const int32_t *table_dev, const int32_t *keep_dev,
+                            const int32_t *have_dev, int32_t *lens_dev, int32_t *free_dev,
+                            const int32_t *n_free_dev, int32_t *n_free_out_dev, void *stream);
 /* Quantise-and-store n_tokens rows of K and V (dtype F32, F16 or BF16; row i at
  * i * row_stride elements, 0 = n_kv_heads * head_dim) at slots_dev[i]; a
  * negative slot is a padding row and is skipped.  Per block and head the scale

@@ -219,13 +219,16 @@ __global__ void __launch_bounds__(TAB_THREADS) assign_kernel(const __grid_consta
   }
 }
 
+// A request that ended gives all its blocks back, one that is cut short those
+// behind the last token it keeps.
 // Ids outside the pool are looked for where they are copied, and closed up behind
 // that by one CTA, which has to wait for the others' word (0.8 us with 8 CTAs).
 __global__ void __launch_bounds__(TAB_THREADS) release_kernel(const __grid_constant__ ReleaseArgs a) {
   extern __shared__ int32_t tab_sm[];
   __shared__ uint64_t part[32];
   __shared__ uint32_t odd_ids;  // CTA 0's: some CTA met an id outside the pool
-  int32_t* start = tab_sm;  // first freed block of each request
+  int32_t* start = tab_sm;             // first freed block of each request
+  int32_t* skip = tab_sm + a.n_seq;    // blocks that it keeps
   const uint32_t bs = a.block_shift, bt = 1u << bs;
   const uint32_t rank = cluster_rank(), ctas = cluster_ctas();
   pdl_trigger();
@@ -233,19 +236,20 @@ __global__ void __launch_bounds__(TAB_THREADS) release_kernel(const __grid_const
   const int32_t n_free = *a.n_free;
   if (threadIdx.x == 0) odd_ids = 0;
   uint64_t total = 0;
-  // the blocks that request r gives back; a length that its table row cannot hold: none
-  auto given = [&](uint32_t r) -> uint32_t {
-    const int32_t h = a.have[r];
-    if (a.done[r] == 0) return 0;
-    const uint64_t n = h > 0 ? ((uint64_t)h + bt - 1) >> bs : 0;
-    return n <= a.stride ? (uint32_t)n : 0;
-  };
-  auto wrong = [&](int32_t h) { return h < 0 || ((uint64_t)h + bt - 1) >> bs > a.stride; };
+  const auto blocks = [&](int32_t tokens) { return (uint32_t)(((uint64_t)tokens + bt - 1) >> bs); };
+  // the tokens that request r keeps of its h
+  const auto keeps = [&](uint32_t r, int32_t h) { return a.keep ? min(a.keep[r], h) : a.done[r] != 0 ? 0 : h; };
+  // a length that is none, or that its table row cannot hold: the request stays as it is
+  const auto wrong = [&](int32_t h, int32_t kept) { return (kept < h && kept < 0) || h < kept || blocks(max(h, 0)) > a.stride; };
   for (uint32_t r0 = 0; r0 < a.n_seq; r0 += blockDim.x) {
     const uint32_t r = r0 + threadIdx.x;
-    const uint64_t n = r < a.n_seq ? given(r) : 0;
+    uint32_t n = 0, first = 0;
+    if (r < a.n_seq) {
+      const int32_t h = a.have[r], kept = keeps(r, h);
+      if (kept != h && !wrong(h, kept)) first = blocks(kept), n = blocks(h) - first;
+    }
     const uint64_t end = block_scan64(n, total, part);
-    if (r < a.n_seq) start[r] = (int32_t)min(end - n, (uint64_t)a.n_blocks);
+    if (r < a.n_seq) start[r] = (int32_t)min(end - n, (uint64_t)a.n_blocks), skip[r] = (int32_t)first;
   }
   // a stack that would outgrow the pool means blocks given back twice
   const bool bad = n_free < 0 || (int64_t)n_free + (int64_t)total > (int64_t)a.n_blocks;
@@ -254,7 +258,7 @@ __global__ void __launch_bounds__(TAB_THREADS) release_kernel(const __grid_const
   bool odd = false;
   for (uint32_t i = rank * blockDim.x + threadIdx.x; !bad && i < total; i += ctas * blockDim.x) {
     const uint32_t q = owner_of(start, a.n_seq, (int32_t)i);
-    const int32_t id = a.table[(size_t)q * a.stride + (i - start[q])];
+    const int32_t id = a.table[(size_t)q * a.stride + skip[q] + (i - start[q])];
     odd |= (uint32_t)id >= a.n_blocks;
     a.free_ids[n_free + i] = id;
   }
@@ -266,9 +270,10 @@ __global__ void __launch_bounds__(TAB_THREADS) release_kernel(const __grid_const
   if (rank) return;
   for (uint32_t r = threadIdx.x; r < a.n_seq; r += blockDim.x) {
     const int32_t h = a.have[r];
-    const bool done = a.done[r] != 0;
-    if (done && wrong(h)) set_error(a.err, DERR_BAD_POS);
-    a.lens[r] = done && !bad && !wrong(h) ? 0 : h;
+    const int32_t kept = keeps(r, h);
+    const bool no = kept != h && wrong(h, kept);
+    if (no) set_error(a.err, DERR_BAD_POS);
+    a.lens[r] = bad || no ? h : kept;
   }
   if (ctas > 1) {
     cluster_wait();
@@ -670,7 +675,7 @@ cudaError_t append_dt(const PagesPool& p, uint32_t dtype, const AppendCall& c) {
 cudaError_t pages_init() {
   cudaError_t e = cudaFuncSetAttribute(assign_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * 4 * 16384);
   if (e != cudaSuccess) return e;
-  e = cudaFuncSetAttribute(release_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * 16384);
+  e = cudaFuncSetAttribute(release_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * 4 * 16384);
   return e != cudaSuccess ? e : pages_attend_init();
 }
 
@@ -681,7 +686,7 @@ cudaError_t pages_assign_launch(const AssignArgs& a, cudaStream_t st) {
 cudaError_t pages_release_launch(const ReleaseArgs& a, cudaStream_t st) {
   // the blocks to give back are at most what the tables can hold, or the pool
   const uint64_t most = (uint64_t)a.n_seq * a.stride;
-  return tables_go(release_kernel, a, most < a.n_blocks ? (uint32_t)most : a.n_blocks, 1, st);
+  return tables_go(release_kernel, a, most < a.n_blocks ? (uint32_t)most : a.n_blocks, 2, st);
 }
 
 cudaError_t pages_append_launch(const PagesPool& p, uint32_t n, const void* k, const void* v, uint32_t dtype,

@@ -48,6 +48,7 @@ struct ReleaseArgs {
   uint32_t n_seq, block_shift, n_blocks, stride;
   const int32_t* table;
   const int32_t* done;
+  const int32_t* keep;  // not null: tokens kept, in place of done
   const int32_t* have;
   int32_t* lens;
   int32_t* free_ids;

@@ -947,12 +947,13 @@ int shk_cuda_pages_assign(shk_ctx* c, const shk_pages_assign* a, void* s) {
   return SHK_OK;
 }
 
-int shk_cuda_pages_release(shk_ctx* c, uint32_t n_seq, uint32_t block_tokens, uint32_t n_blocks, uint32_t table_stride,
-                           const int32_t* table, const int32_t* done, const int32_t* have, int32_t* lens,
-                           int32_t* free_ids, const int32_t* n_free, int32_t* n_free_out, void* s) {
+// done: requests that ended; or keep: the tokens that each one keeps.
+static int give_back(shk_ctx* c, uint32_t n_seq, uint32_t block_tokens, uint32_t n_blocks, uint32_t table_stride,
+                     const int32_t* table, const int32_t* done, const int32_t* keep, const int32_t* have, int32_t* lens,
+                     int32_t* free_ids, const int32_t* n_free, int32_t* n_free_out, void* s) {
   if (c) on_dev(c);
-  if (!c || !table || !done || !have || !lens || !free_ids || !n_free || !n_free_out) return SHK_EINVAL;
-  if (!words({table, done, have, lens, free_ids, n_free, n_free_out})) return SHK_EINVAL;
+  if (!c || !table || !(done || keep) || !have || !lens || !free_ids || !n_free || !n_free_out) return SHK_EINVAL;
+  if (!words({table, done, keep, have, lens, free_ids, n_free, n_free_out})) return SHK_EINVAL;
   ReleaseArgs g{};
   if (!pages_dims(n_blocks, block_tokens, &g.block_shift)) return SHK_EINVAL;
   if (!n_seq || n_seq > SHK_PAGES_MAX_SEQ || !table_stride) return SHK_EINVAL;
@@ -961,6 +962,7 @@ int shk_cuda_pages_release(shk_ctx* c, uint32_t n_seq, uint32_t block_tokens, ui
   g.stride = table_stride;
   g.table = table;
   g.done = done;
+  g.keep = keep;
   g.have = have;
   g.lens = lens;
   g.free_ids = free_ids;
@@ -969,6 +971,20 @@ int shk_cuda_pages_release(shk_ctx* c, uint32_t n_seq, uint32_t block_tokens, ui
   g.err = c->d_err;
   CK(pages_release_launch(g, pick(c, s)));
   return SHK_OK;
+}
+
+int shk_cuda_pages_release(shk_ctx* c, uint32_t n_seq, uint32_t block_tokens, uint32_t n_blocks, uint32_t table_stride,
+                           const int32_t* table, const int32_t* done, const int32_t* have, int32_t* lens,
+                           int32_t* free_ids, const int32_t* n_free, int32_t* n_free_out, void* s) {
+  return give_back(c, n_seq, block_tokens, n_blocks, table_stride, table, done, nullptr, have, lens, free_ids, n_free,
+                   n_free_out, s);
+}
+
+int shk_cuda_pages_truncate(shk_ctx* c, uint32_t n_seq, uint32_t block_tokens, uint32_t n_blocks, uint32_t table_stride,
+                            const int32_t* table, const int32_t* keep, const int32_t* have, int32_t* lens,
+                            int32_t* free_ids, const int32_t* n_free, int32_t* n_free_out, void* s) {
+  return give_back(c, n_seq, block_tokens, n_blocks, table_stride, table, nullptr, keep, have, lens, free_ids, n_free,
+                   n_free_out, s);
 }
 
 int shk_cuda_pages_append(shk_ctx* c, const shk_pages* p, uint32_t n_tokens, const void* k, const void* v,

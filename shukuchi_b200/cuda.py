@@ -143,6 +143,7 @@ _SIGS = {
     "shk_cuda_kv_attend_batch": (I, [P, U32, U32, P, P, P, P, U32, U32, F, P]),
     "shk_cuda_pages_assign": (I, [P, P, P]),
     "shk_cuda_pages_release": (I, [P, U32, U32, U32, U32, P, P, P, P, P, P, P, P]),
+    "shk_cuda_pages_truncate": (I, [P, U32, U32, U32, U32, P, P, P, P, P, P, P, P]),
     "shk_cuda_pages_append": (I, [P, P, U32, P, P, U32, SZ, P, P]),
     "shk_cuda_pages_read": (I, [P, P, U32, P, P, P, P]),
     "shk_cuda_pages_attend_ws": (SZ, [U32, U32, U32, U32]),
@@ -320,6 +321,14 @@ class Context:
                                                     have, lens, free, n_free, n_free_out, stream)
         if rc:
             check("shk_cuda_pages_release", rc)
+
+    def pages_truncate(self, n_seq, block_tokens, n_blocks, table_stride, table, keep, have, lens, free, n_free,
+                       n_free_out, stream=None):
+        """Requests cut to keep[r] tokens (rejected drafts, or 0: ended), the blocks behind those back on the free stack."""
+        rc = (_lib or lib()).shk_cuda_pages_truncate(self.h, n_seq, block_tokens, n_blocks, table_stride, table, keep,
+                                                     have, lens, free, n_free, n_free_out, stream)
+        if rc:
+            check("shk_cuda_pages_truncate", rc)
 
     def sample(self, logits, n_rows, n_vocab, u, out, prob=None, temperature=None, top_k=None, top_p=None,
                min_p=None, dtype=0, row_stride=0, stream=None):
