@@ -100,6 +100,13 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// 2^d / l in two factors, the second a power of two: 2^d for a V scale near the
+// smallest floats is below what ex2 gives, and what the output is not.
+__device__ __forceinline__ float2 out_factor(float d, float l) {
+  const bool low = d < -64.f;
+  return make_float2(l == 0.f ? 0.f : ex2(low ? d + 64.f : d) / l, low ? 0x1p-64f : 1.f);
+}
+
 __device__ __forceinline__ void copy(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -615,10 +622,10 @@ __global__ void __launch_bounds__(THREADS, Lay<HD, SETS>::CTAS) attend_kernel(co
         const uint32_t slot = HEADS * x + h;
         if (slot < slots) {
           // MM - mm is at most the largest exponent of a scale
-          const float f = ll == 0.f ? 0.f : ex2(MM - mm - 14.f) / ll;
+          const float2 f = out_factor(MM - mm - 14.f, ll);
           const size_t at = slot_row(slot) * a.out_stride + slot_dim(slot) + d;
 #pragma unroll
-          for (int e = 0; e < PER; ++e) store_dt(a.out, at + e, a.dtype, ll == 0.f ? 0.f : out[e] * f);
+          for (int e = 0; e < PER; ++e) store_dt(a.out, at + e, a.dtype, ll == 0.f ? 0.f : out[e] * f.x * f.y);
         }
       } else {
 #pragma unroll
@@ -652,7 +659,7 @@ __global__ void __launch_bounds__(THREADS_J) attend_join_kernel(const __grid_con
   // (8 in a small block of two groups: 64 x 4 rows 42.3 us, 4: 41.0)
   constexpr uint32_t HELD = THREADS_J == 256 ? 8 / GROUPS : 8;
   __shared__ float weight[HEADS][MAX_CTAS + 1];  // of a piece's outputs
-  __shared__ float fin[HEADS];
+  __shared__ float2 fin[HEADS];
   __shared__ float4 sum[THREADS_J];
   const uint32_t c = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
   pdl_wait();
@@ -684,7 +691,7 @@ __global__ void __launch_bounds__(THREADS_J) attend_join_kernel(const __grid_con
     M = warp_max(M);
     l = warp_sum(l == 0.f ? 0.f : l * ex2(m - mm));
     for (uint32_t i = lane; i < n; i += 32) weight[hh][i] = weight[hh][i] == -INFINITY ? 0.f : ex2(weight[hh][i] - M);
-    if (lane == 0) fin[hh] = l == 0.f ? 0.f : ex2(M - mm - 14.f) / l;
+    if (lane == 0) fin[hh] = out_factor(M - mm - 14.f, l);
   }
   __syncthreads();
   float4 o{};
@@ -706,13 +713,13 @@ __global__ void __launch_bounds__(THREADS_J) attend_join_kernel(const __grid_con
     const float4 v = sum[k * PER_GROUP + e];
     o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
   }
-  const float f = fin[h];
+  const float2 f = fin[h];
   const uint32_t in = nsub == 1 ? slot * a.inv_group >> 16 : 0, row = (uint32_t)hd.row + in, head = sub * SLOTS + slot - in * G;
   const size_t at = row * a.out_stride + (size_t)(head * n_kv + kvh) * HD + 4 * (e % (HD / 4));
-  store_dt(a.out, at, a.dtype, o.x * f);
-  store_dt(a.out, at + 1, a.dtype, o.y * f);
-  store_dt(a.out, at + 2, a.dtype, o.z * f);
-  store_dt(a.out, at + 3, a.dtype, o.w * f);
+  store_dt(a.out, at, a.dtype, o.x * f.x * f.y);
+  store_dt(a.out, at + 1, a.dtype, o.y * f.x * f.y);
+  store_dt(a.out, at + 2, a.dtype, o.z * f.x * f.y);
+  store_dt(a.out, at + 3, a.dtype, o.w * f.x * f.y);
 }
 
 template <int HD, uint32_t TYPE, int SETS, bool MANY>
