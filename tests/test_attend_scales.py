@@ -66,3 +66,29 @@ def test_ends_of_the_v_scales(ctx, kind, hd, blocks, exponent):
     ref, lim = attend_reference(q, K, V, table, [0, 1], pos, 16, H, SCALE)
     lim += parts_slack(pool, kind, K, q, table, pos)
     assert np.all(np.abs(got - ref) <= lim + 2.0 ** -150)
+
+
+@pytest.mark.parametrize("kind", [sc.PAGES_I8, sc.PAGES_E4M3])
+@pytest.mark.parametrize("first", [0, 1])
+@pytest.mark.parametrize("apart", [10, 20, 30, 45])
+def test_v_scales_far_apart(ctx, kind, first, apart):
+    """A block whose scale is 2^apart of the others', with zeros in half its dimensions: there the others' values are
+    the result, as far as the weights' parts hold them."""
+    rng = np.random.default_rng(apart)
+    n, hd = 8, 64
+    pool = Pool(ctx, rng, n, KV, 16, hd, kind)
+    pool.hs[1][:] = rng.uniform(1, 2, pool.hs[1].shape).astype(np.float32)
+    large = 0 if first else n - 1
+    pool.hs[1][large] *= np.float32(2.0 ** apart)
+    pool.h[1][large, :, :, : hd // 2] = 0
+    table, pos = np.arange(n).reshape(1, n), [16 * n - 1]
+    q = 0.1 * rng.normal(0, 1, (1, H, hd)).astype(np.float32)
+    got = attend(ctx, pool, table, pos, q)
+    K, V = pool.values()
+    ref, lim = attend_reference(q, K, V, table, [0], pos, 16, H, SCALE)
+    lim += parts_slack(pool, kind, K, q, table, pos)
+    assert np.all(np.abs(got - ref) <= lim)
+    if apart <= 20:  # within 2^-15 of the smaller blocks' own values
+        small = np.abs(ref[0, :, : hd // 2])
+        size = np.abs(V[first: n - 1 + first]).mean()
+        assert np.all(np.abs(got - ref)[0, :, : hd // 2] <= 2.0 ** -15 * size) and small.max() > 0.01 * size
