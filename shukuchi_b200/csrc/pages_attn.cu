@@ -202,6 +202,23 @@ struct Sums {
   uint32_t row;
 };
 
+// The first row from `row` on that is somebody's, n where there is none: 128 rows
+// at a time, by each warp for itself, as a request that was refused whole may leave
+// thousands of padding rows between two items (64 rows with 4000 behind the first
+// half: 1.47 ms one after the other, 52 us so).
+__device__ __forceinline__ uint32_t live_row(const int32_t* row_seq, uint32_t row, uint32_t n) {
+  const uint32_t lane = threadIdx.x & 31;
+  for (; row < n; row += 128) {
+    uint32_t live[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) live[i] = __ballot_sync(0xffffffffu, row + 32 * i + lane < n && row_seq[row + 32 * i + lane] >= 0);
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+      if (live[i]) return row + 32 * i + __ffs(live[i]) - 1;
+  }
+  return n;
+}
+
 // Row of a request's position p0 in a pool.
 __device__ __forceinline__ size_t first_row(const PagesAttnArgs& a, int32_t id, uint32_t kvh, uint32_t p0) {
   const uint32_t bs = a.pool.block_shift;
@@ -642,10 +659,10 @@ __global__ void __launch_bounds__(THREADS, Lay<HD, SETS>::CTAS) attend_kernel(co
     }
     if (next_row) {
       base = s;
-      do {
-        if (++row >= a.n_rows) return;  // (positions that were changed during the call)
-        rw = row_of<MANY>(a, row);
-      } while (rw.units == 0);
+      row += MANY ? rw.rows : 1;
+      if (row < a.n_rows && a.row_seq && a.row_seq[row] < 0) row = live_row(a.row_seq, row + 1, a.n_rows);
+      if (row >= a.n_rows) return;  // (positions that were changed during the call)
+      rw = row_of<MANY>(a, row);
     }
   }
 }
