@@ -351,9 +351,10 @@ int shk_cuda_pages_read(shk_ctx *ctx, const struct shk_pages *pages, uint32_t n_
  * (engine/src/ops.c:423).  pos < 0: the row sees nothing and becomes zeros;
  * seq < 0: no row (padding), out left as it was.  q and out are dtype F32, F16
  * or BF16 rows of n_heads * head_dim, q_stride / out_stride elements apart (0 =
- * dense); out may not overlap q.  Sums and softmax in fp32; a position's weight times
- * its V scale enters the output to 2^-22 of itself or 2^-39 of the row's largest
- * such product, whichever is more.  Rows of one request
+ * dense); out may not overlap q (rows of one stride may lie between one another,
+ * with two strides the whole ranges count).  Sums and softmax in fp32; a
+ * position's weight times its V scale enters the output to 2^-22 of itself or
+ * 2^-39 of the row's largest such product, whichever is more.  Rows of one request
  * that follow one another read its blocks together.  What no row of the call
  * sees may hold anything; between a row's last position and that of a
  * neighbour in its request, E4M3 bytes have to be numbers, as shk_cuda_pages_append

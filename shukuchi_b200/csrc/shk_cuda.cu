@@ -1021,6 +1021,16 @@ size_t shk_cuda_pages_attend_ws(uint32_t n_rows, uint32_t n_heads, uint32_t n_kv
   return pages_attend_ws_bytes(n_rows, n_heads, n_kv_heads, head_dim);
 }
 
+// Whether two arrays of n rows of `width` bytes may share a byte.  Rows of one
+// stride may lie between one another; with two strides, overlapping ranges count.
+static bool rows_overlap(const void* a, size_t a_stride, const void* b, size_t b_stride, size_t width, size_t n) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  if (x >= y + (n - 1) * b_stride + width || y >= x + (n - 1) * a_stride + width) return false;
+  if (a_stride != b_stride) return true;
+  const size_t apart = x > y ? (x - y) % a_stride : (y - x) % a_stride;
+  return apart < width || a_stride - apart < width;
+}
+
 int shk_cuda_pages_attend(shk_ctx* c, const shk_pages* p, const shk_pages_rows* r, void* s) {
   if (c) on_dev(c);
   PagesAttnArgs g{};
@@ -1039,8 +1049,7 @@ int shk_cuda_pages_attend(shk_ctx* c, const shk_pages* p, const shk_pages_rows* 
     return SHK_EINVAL;
   // a row's q may be read again after its neighbours have been written
   const size_t qs = r->q_stride ? r->q_stride : width, os = r->out_stride ? r->out_stride : width;
-  const uintptr_t q0 = reinterpret_cast<uintptr_t>(r->q_dev), o0 = reinterpret_cast<uintptr_t>(r->out_dev);
-  if (q0 < o0 + ((r->n_rows - 1) * os + width) * es && o0 < q0 + ((r->n_rows - 1) * qs + width) * es) return SHK_EINVAL;
+  if (rows_overlap(r->q_dev, qs * es, r->out_dev, os * es, width * es, r->n_rows)) return SHK_EINVAL;
   if (!r->ws_dev || !aligned(r->ws_dev, 16) ||
       r->ws_bytes < pages_attend_ws_bytes(r->n_rows, r->n_heads, g.pool.n_kv, g.pool.hd))
     return SHK_EINVAL;
