@@ -375,6 +375,7 @@ struct shk_pages_rows {
     void *ws_dev;
     size_t ws_bytes;
 };
+/* 0 for heads or a head_dim that shk_cuda_pages_attend does not take. */
 size_t shk_cuda_pages_attend_ws(uint32_t n_rows, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);
 int shk_cuda_pages_attend(shk_ctx *ctx, const struct shk_pages *pages, const struct shk_pages_rows *rows,
                           void *stream);

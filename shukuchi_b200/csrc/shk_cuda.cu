@@ -886,6 +886,8 @@ static bool pages_dims(uint32_t n_blocks, uint32_t block_tokens, uint32_t* shift
   return n_blocks > 0 && (uint64_t)n_blocks << *shift <= 0x7FFFFFFFull;
 }
 
+constexpr uint32_t PAGES_MAX_KV_HEADS = 1024, PAGES_MAX_HEADS = 4096;
+
 static bool act_dtype(uint32_t dt) { return dt == DT_F32 || dt == DT_F16 || dt == DT_BF16; }
 
 static bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
@@ -911,7 +913,7 @@ static int pages_pool(const shk_pages* p, PagesPool* out) {
   out->n_blocks = p->n_blocks;
   out->n_kv = p->n_kv_heads;
   out->hd = p->head_dim;
-  if (p->n_kv_heads > 1024) return SHK_EINVAL;
+  if (p->n_kv_heads > PAGES_MAX_KV_HEADS) return SHK_EINVAL;
   return pages_dims(p->n_blocks, p->block_tokens, &out->block_shift) ? SHK_OK : SHK_EINVAL;
 }
 
@@ -1018,6 +1020,7 @@ int shk_cuda_pages_read(shk_ctx* c, const shk_pages* p, uint32_t n_tokens, const
 
 size_t shk_cuda_pages_attend_ws(uint32_t n_rows, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim) {
   if (!n_heads || !n_kv_heads || n_heads % n_kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
+  if (n_kv_heads > PAGES_MAX_KV_HEADS || n_heads > PAGES_MAX_HEADS) return 0;
   return pages_attend_ws_bytes(n_rows, n_heads, n_kv_heads, head_dim);
 }
 
@@ -1040,7 +1043,7 @@ int shk_cuda_pages_attend(shk_ctx* c, const shk_pages* p, const shk_pages_rows* 
   if (r->n_rows == 0) return SHK_OK;
   if (!act_dtype(r->dtype)) return SHK_EUNSUPPORTED;
   const size_t width = (size_t)r->n_heads * g.pool.hd, es = r->dtype == DT_F32 ? 4 : 2;
-  if (!r->n_heads || r->n_heads % g.pool.n_kv || r->n_heads > 4096 || !r->q_dev || !r->out_dev || !r->pos_dev ||
+  if (!r->n_heads || r->n_heads % g.pool.n_kv || r->n_heads > PAGES_MAX_HEADS || !r->q_dev || !r->out_dev || !r->pos_dev ||
       !r->table_dev || !r->table_stride || !r->n_seq || !aligned(r->q_dev, es) || !aligned(r->out_dev, es) ||
       !words({r->seq_dev, r->pos_dev, r->table_dev}) ||
       (r->q_stride && r->q_stride < width) || (r->out_stride && r->out_stride < width) ||
