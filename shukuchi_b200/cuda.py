@@ -78,7 +78,8 @@ class PagesRows(C.Structure):
 
 
 # The argument structs of calls that a server makes in every step are packed by
-# struct, which takes a third of the time of filling a ctypes.Structure.
+# struct, which takes a third of the time of filling a ctypes.Structure; values
+# that it does not take (a c_void_p, say) go through the Structure.
 _ASSIGN = struct.Struct("@5I11P")
 _ROWS = struct.Struct("@3I2P2N3P2IfPN")
 assert _ASSIGN.size == C.sizeof(PagesAssign) and _ROWS.size == C.sizeof(PagesRows)
@@ -308,8 +309,12 @@ class Context:
     def pages_assign(self, n_seq, block_tokens, n_blocks, table_stride, n_rows, have, add, table, free, n_free, lens,
                      counts, slots, pos, seq, last, stream=None):
         """Block tables, slots and positions of every request's new tokens (shk_cuda_pages_assign)."""
-        a = _ASSIGN.pack(n_seq, block_tokens, n_blocks, table_stride, n_rows, have or 0, add or 0, table or 0, free or 0,
-                         n_free or 0, lens or 0, counts or 0, slots or 0, pos or 0, seq or 0, last or 0)
+        try:
+            a = _ASSIGN.pack(n_seq, block_tokens, n_blocks, table_stride, n_rows, have or 0, add or 0, table or 0,
+                             free or 0, n_free or 0, lens or 0, counts or 0, slots or 0, pos or 0, seq or 0, last or 0)
+        except struct.error:
+            a = C.byref(PagesAssign(n_seq, block_tokens, n_blocks, table_stride, n_rows, have, add, table, free, n_free,
+                                    lens, counts, slots, pos, seq, last))
         rc = (_lib or lib()).shk_cuda_pages_assign(self.h, a, stream)
         if rc:
             check("shk_cuda_pages_assign", rc)
@@ -446,8 +451,12 @@ class Pages:
     def attend(self, n_rows, q, out, n_heads, row_pos, table, table_stride, n_seq, scale, ws, ws_bytes, row_seq=None,
                dtype=DTYPE_F32, q_stride=0, out_stride=0, stream=None):
         """Rows of q over the positions 0 .. row_pos of their requests; ws_bytes >= pages_attend_ws(...)."""
-        r = _ROWS.pack(n_rows, n_heads, dtype, q or 0, out or 0, q_stride, out_stride, row_seq or 0, row_pos or 0,
-                       table or 0, n_seq, table_stride, scale, ws or 0, ws_bytes)
+        try:
+            r = _ROWS.pack(n_rows, n_heads, dtype, q or 0, out or 0, q_stride, out_stride, row_seq or 0, row_pos or 0,
+                           table or 0, n_seq, table_stride, scale, ws or 0, ws_bytes)
+        except struct.error:
+            r = C.byref(PagesRows(n_rows, n_heads, dtype, q, out, q_stride, out_stride, row_seq, row_pos, table, n_seq,
+                                  table_stride, scale, ws, ws_bytes))
         rc = (_lib or lib()).shk_cuda_pages_attend(self.ctx.h, C.byref(self.desc), r, stream)
         if rc:
             check("shk_cuda_pages_attend", rc)
