@@ -439,6 +439,7 @@ int shk_cuda_model_lm_head(shk_model *m, uint32_t *token_host, float *logits_hos
  * shk_cuda_sample draws one, in place of that call's argmax.  u in [0, 1);
  * temperature <= 0 gives the argmax, top_k <= 0, top_p >= 1 and min_p <= 0 are
  * off.  *prob_host (may be NULL): the token's share of the weights that stayed.
+ * Before the model's first output head the token is SHK_SAMPLE_NONE, its share 0.
  * Synchronous.  Single GPU (a tensor-parallel rank: SHK_EUNSUPPORTED). */
 struct shk_sampling {
     float temperature;

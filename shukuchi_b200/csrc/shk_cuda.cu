@@ -1639,6 +1639,8 @@ shk_model* shk_cuda_model_create(shk_ctx* c, const shk_model_desc* d, shk_kv* kv
   ok = ok && cudaMemset(m->d_tok, 0, 16 * sizeof(uint32_t)) == cudaSuccess;
   ok = ok && cudaMallocHost(&m->h_tok, 16 * sizeof(uint32_t)) == cudaSuccess;
   if (ok) ok = cudaMemset(m->hidden, 0, d->n_embd * sizeof(float)) == cudaSuccess;
+  // NaN until the first output head: a draw from them finds nothing
+  if (ok) ok = cudaMemset(m->logits, 0xFF, (size_t)d->n_vocab * sizeof(float)) == cudaSuccess;
   if (!ok) {
     shk_cuda_model_destroy(m);
     return nullptr;
