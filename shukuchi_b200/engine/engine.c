@@ -1342,7 +1342,7 @@ int engine_generate_ids(engine_handle_t *h, const uint32_t *prompt, uint32_t n_p
 }
 
 int engine_set_sampling(engine_handle_t *h, float temperature, int top_k, float top_p, float min_p, uint64_t seed) {
-    if (!h || !(temperature >= 0.f) || temperature > 3.0e38f || top_p != top_p || min_p != min_p) return -1;
+    if (!h || !(temperature >= 0.f) || isinf(temperature) || top_p != top_p || min_p != min_p) return -1;
     h->sampling.temperature = temperature;
     h->sampling.top_k = top_k;
     h->sampling.top_p = top_p;

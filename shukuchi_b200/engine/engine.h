@@ -94,8 +94,9 @@ uint32_t engine_vocab_size(engine_handle_t *h);
  * reference only takes the argmax): temperature 0 (the default) is greedy, top_k
  * <= 0, top_p >= 1 and min_p <= 0 are off (shk_cuda_sample says what each does).
  * Every generation's draws start from `seed`: the same seed and prompt give the
- * same tokens.  0, or -1 for a negative or NaN argument; with SHUKUCHI_TP > 1
- * a generation with a temperature above 0 returns -1. */
+ * same tokens.  0, or -1 for a temperature that is negative, infinite or NaN and
+ * for a top_p or min_p that is NaN (what was set before stays); with SHUKUCHI_TP >
+ * 1 a generation with a temperature above 0 returns -1. */
 int engine_set_sampling(engine_handle_t *h, float temperature, int top_k, float top_p, float min_p, uint64_t seed);
 /* The GPU backend's counters on stderr (matvec calls, layer forwards, token
  * steps, staged copies and bytes): the CLI's closing report, as the

@@ -64,3 +64,33 @@ def test_model_sample_before_any_logits(ctx):
         assert dec.m.sample(0.5, temperature=0.0) == (nxt, 1.0)
     finally:
         dec.close()
+
+
+def test_engine_sampling_arguments(tmp_path, monkeypatch):
+    """What is refused leaves the settings before it in place; every finite temperature, a negative top_p (one token) and
+    a negative min_p (off) are taken."""
+    monkeypatch.setenv("SHUKUCHI_HBM_RESIDENT", "1")
+    m = synth.make_model("small", seed=33)
+    path = str(tmp_path / "small.gguf")
+    gguf.write_model(path, m)
+    L, vocab, nan, inf = engine(), m.shape.n_vocab, float("nan"), float("inf")
+    h = L.engine_open(path.encode(), C.byref(Config(4, 1, 3, 32, 0, 0)))
+    assert h, "engine_open failed"
+
+    def run():
+        prompt, ids = np.array([3, 5], np.uint32), np.zeros(4, np.uint32)
+        assert L.engine_generate_ids(h, prompt.ctypes.data, 2, 4, ids.ctypes.data, None) == 4
+        return ids.tolist()
+
+    try:
+        greedy = run()
+        assert L.engine_set_sampling(h, 3.3e38, 0, 1.0, -1.0, 9) == 0
+        hot = run()
+        assert hot != greedy and max(hot) < vocab
+        for bad in ((-1.0, 0, 1.0, 0.0), (nan, 0, 1.0, 0.0), (inf, 0, 1.0, 0.0), (1.0, 0, nan, 0.0), (1.0, 0, 1.0, nan)):
+            assert L.engine_set_sampling(h, *bad, 1) == -1
+            assert run() == hot
+        assert L.engine_set_sampling(h, 3.3e38, 0, -1.0, 0.0, 9) == 0
+        assert run() == greedy
+    finally:
+        L.engine_close(h)
