@@ -215,7 +215,10 @@ __device__ __forceinline__ uint32_t live_row(const int32_t* row_seq, uint32_t ro
   for (; row < n; row += 128) {
     uint32_t live[4];
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) live[i] = __ballot_sync(0xffffffffu, row + 32 * i + lane < n && row_seq[row + 32 * i + lane] >= 0);
+    for (uint32_t i = 0; i < 4; ++i) {
+      const uint32_t r = row + 32 * i + lane;
+      live[i] = __ballot_sync(0xffffffffu, r < n && row_seq[r] >= 0);
+    }
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i)
       if (live[i]) return row + 32 * i + __ffs(live[i]) - 1;
@@ -352,321 +355,324 @@ __global__ void __launch_bounds__(THREADS, Lay<HD, SETS>::CTAS) attend_kernel(co
     s += vb - va;
     const bool next_row = s < end && s == base + (uint64_t)NI * span;
     if (ub > 0) {
-    const uint32_t kvh = item / nsub, sub = item % nsub;
-    // slot x of the item: head sub * SLOTS + x of its row, or head x % G of row x / G
-    const uint32_t slots = MANY && nsub == 1 ? rw.rows * G : min(G - sub * SLOTS, SLOTS);
-    auto slot_in = [&](uint32_t x) { return MANY && nsub == 1 ? x * a.inv_group >> 16 : 0; };
-    auto slot_row = [&](uint32_t x) { return row + slot_in(x); };
-    auto slot_dim = [&](uint32_t x) { return (size_t)((sub * SLOTS + x - slot_in(x) * G) * n_kv + kvh) * HD; };
-    const int32_t* table = a.table + (size_t)rw.z * a.stride;  // z is in range where len > 0
+      const uint32_t kvh = item / nsub, sub = item % nsub;
+      // slot x of the item: head sub * SLOTS + x of its row, or head x % G of row x / G
+      const uint32_t slots = MANY && nsub == 1 ? rw.rows * G : min(G - sub * SLOTS, SLOTS);
+      auto slot_in = [&](uint32_t x) { return MANY && nsub == 1 ? x * a.inv_group >> 16 : 0; };
+      auto slot_row = [&](uint32_t x) { return row + slot_in(x); };
+      auto slot_dim = [&](uint32_t x) { return (size_t)((sub * SLOTS + x - slot_in(x) * G) * n_kv + kvh) * HD; };
+      const int32_t* table = a.table + (size_t)rw.z * a.stride;  // z is in range where len > 0
 
-    // q of this lane's fragments: k-step st covers, for lane (g, t), the 4 dims of word st % 4 of its piece st / 4
-    float q[SETS][L::STEPS / WARPS][4];
-    uint32_t len[SETS];  // of the rows of this lane's slots
-#pragma unroll
-    for (int x = 0; x < SETS; ++x) {
-      const uint32_t slot = HEADS * x + g;
-      len[x] = rw.len;
-      if (MANY && rw.rows > 1 && slot < slots) len[x] = row_len(a, rw.z, a.row_pos[slot_row(slot)]);
-#pragma unroll
-      for (int i = 0; i < L::STEPS / WARPS; ++i) {
-        const uint32_t st = warp + WARPS * i, d = 64 * (st >> 2) + 16 * t + 4 * (st & 3);
-        const size_t at = slot < slots ? slot_row(slot) * a.q_stride + slot_dim(slot) + d : 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) q[x][i][e] = slot < slots ? load_dt(a.q, at + e, a.dtype) : 0.f;
-      }
-    }
-
-    // ---- this warp's steps: units ua .. ub - 1, positions UNIT u + STEP warp ----
-    const uint32_t steps = (rw.len + STEP - 1) / STEP;
-    const uint32_t last_u = steps > warp ? (steps - warp + WARPS - 1) / WARPS : 0;  // units with a step of this warp
-    const int32_t n = (int32_t)min(ub, last_u) - (int32_t)ua;
-    auto place = [&](int32_t i, int half) { return (ua + (uint32_t)i) * UNIT + warp * STEP + half * SUB; };
-    // a table entry is checked a step after it is read, when it has arrived
-    auto entry = [&](int32_t i, int half) -> int32_t {
-      const uint32_t p = place(i, half);
-      return i < n && p < rw.len ? table[p >> bs] : -1;
-    };
-    auto checked = [&](int32_t i, int2 id) {
-      if ((uint32_t)id.x >= a.pool.n_blocks || (uint32_t)id.y >= a.pool.n_blocks) {
-        if (i < n && ((uint32_t)id.x >= a.pool.n_blocks || place(i, 1) < rw.len)) set_error(a.err, DERR_BAD_POS);
-        if ((uint32_t)id.x >= a.pool.n_blocks) id.x = -1;
-        if ((uint32_t)id.y >= a.pool.n_blocks) id.y = -1;
-      }
-      return id;
-    };
-    auto issue_k = [&](int32_t i, int2 id) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if ((h ? id.y : id.x) >= 0)
-          fetch<HD, TYPE, false>(a.pool.k + first_row(a, h ? id.y : id.x, kvh, place(i, h)) * HD, ring + h * L::HALF, 0, lane);
-      copy_commit();
-    };
-    auto issue_v = [&](int32_t i, int2 id) {
-      const uint32_t dst = ring + L::KBUF + (i & 1) * L::KBUF;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if ((h ? id.y : id.x) >= 0)
-          fetch<HD, TYPE, true>(a.pool.v + first_row(a, h ? id.y : id.x, kvh, place(i, h)) * HD, dst + h * L::HALF,
-                                rw.len - place(i, h), lane);
-        else if (TYPE == PAGES_E4M3 && i < n)
-          fetch<HD, TYPE, true>(a.pool.v, dst + h * L::HALF, 0, lane);
-      }
-      copy_commit();
-    };
-    auto scales = [&](int32_t id) {
-      const size_t at = (size_t)(id < 0 ? 0 : id) * n_kv + kvh;
-      return make_float2(a.pool.ks[at], a.pool.vs[at]);
-    };
-    float m[SETS], M[SETS], l[SETS], o[SETS][HD / 16][4];
-#pragma unroll
-    for (int x = 0; x < SETS; ++x) {
-      m[x] = M[x] = -INFINITY, l[x] = 0.f;
-#pragma unroll
-      for (int j = 0; j < HD / 16; ++j) o[x][j][0] = o[x][j][1] = o[x][j][2] = o[x][j][3] = 0.f;
-    }
-    int2 id0{-1, -1}, id1{-1, -1};
-    float2 sx{}, sy{};
-    if (n > 0) {  // the first copies are on their way before q is needed
-      id0 = int2{entry(0, 0), entry(0, 1)};
-      id1 = int2{entry(1, 0), entry(1, 1)};
-      id0 = checked(0, id0);
-      issue_k(0, id0);
-      issue_v(0, id0);
-      sx = scales(id0.x), sy = scales(id0.y);
-    }
-
-    // q scaled by a power of two so that the largest magnitude of a head is in [2^14, 2^15)
-    if (tid < SLOTS) qmax[tid] = 0;
-    __syncthreads();
-#pragma unroll
-    for (int x = 0; x < SETS; ++x) {
-      float big = 0.f;
-#pragma unroll
-      for (int i = 0; i < L::STEPS / WARPS; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(q[x][i][e]));
-      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-      if (t == 0) atomicMax(&qmax[HEADS * x + g], __float_as_int(big));
-    }
-    __syncthreads();
-    float qscale[SETS];
-#pragma unroll
-    for (int x = 0; x < SETS; ++x) {
-      const float top = __int_as_float(qmax[HEADS * x + g]);
-      int ex = 0;
-      if (top > 0.f && top < INFINITY) ex = min(14 - ilogbf(top), 126);
-      const float up = ldexpf(1.f, ex);
-      qscale[x] = a.scale * 1.4426950408889634f * ldexpf(1.f, -ex);
-#pragma unroll
-      for (int i = 0; i < L::STEPS / WARPS; ++i) {
-        uint4 f;
-        split2(q[x][i][0] * up, q[x][i][1] * up, f.x, f.y);
-        split2(q[x][i][2] * up, q[x][i][3] * up, f.z, f.w);
-        qf[(x * L::STEPS + warp + WARPS * i) * 32 + lane] = f;
-      }
-    }
-    __syncthreads();
-
-    for (int32_t i = 0; i < n; ++i) {
-      id1 = checked(i + 1, id1);
-      issue_v(i + 1, id1);
-      const float2 nx = scales(id1.x), ny = scales(id1.y);
-      const int2 id2{entry(i + 2, 0), entry(i + 2, 1)};
-      copy_wait<1>();  // this step's K and V; the next V may be on its way
-      __syncwarp();
-      const uint8_t* here = att_smem + warp * L::RING;
-      float acc[SETS][4][4] = {};
-#pragma unroll
-      for (int pi = 0; pi < L::NP; ++pi) {
-        uint32_t kw[4][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint4 x = *reinterpret_cast<const uint4*>(here + (j >> 1) * L::HALF + k_at[pi] + (j & 1) * 8 * HD);
-          kw[j][0] = x.x, kw[j][1] = x.y, kw[j][2] = x.z, kw[j][3] = x.w;
-        }
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint4 qa[SETS];
-#pragma unroll
-          for (int x = 0; x < SETS; ++x) qa[x] = qf[(x * L::STEPS + 4 * pi + w) * 32 + lane];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t b0, b1;
-            to_f16<TYPE>(kw[j][w], b0, b1);
-#pragma unroll
-            for (int x = 0; x < SETS; ++x) mma_f16(acc[x][j], qa[x], b0, b1);
-          }
-        }
-      }
-      __syncwarp();
-      issue_k(i + 1, id1);  // this step's K has been multiplied
-      // a V scale is 2^E * vf, vf below 2 (also for a scale of 0, an infinite one or NaN)
-      float E[2], vf[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float vs = (h ? id0.y : id0.x) < 0 ? 0.f : h ? sy.y : sx.y;
-        const int e8 = max(1, min(254, (int)((__float_as_uint(vs) >> 23) & 255)));
-        E[h] = (float)(e8 - 127);
-        vf[h] = e8 == 254 ? vs * 0x1p-127f : vs * __int_as_float((254 - e8) << 23);
-      }
-      // scores in powers of two; lane (g, t) holds slot g at positions 8 j + 2t, 8 j + 2t + 1
-      float sv[SETS][4][2], m0[SETS], M0[SETS];
+      // q of this lane's fragments: k-step st covers, for lane (g, t), the 4 dims of word st % 4 of its piece st / 4
+      float q[SETS][L::STEPS / WARPS][4];
+      uint32_t len[SETS];  // of the rows of this lane's slots
 #pragma unroll
       for (int x = 0; x < SETS; ++x) {
+        const uint32_t slot = HEADS * x + g;
+        len[x] = rw.len;
+        if (MANY && rw.rows > 1 && slot < slots) len[x] = row_len(a, rw.z, a.row_pos[slot_row(slot)]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float f = (j < 2 ? sx.x : sy.x) * qscale[x];
-          sv[x][j][0] = (acc[x][j][0] + acc[x][j][2]) * f;
-          sv[x][j][1] = (acc[x][j][1] + acc[x][j][3]) * f;
+        for (int i = 0; i < L::STEPS / WARPS; ++i) {
+          const uint32_t st = warp + WARPS * i, d = 64 * (st >> 2) + 16 * t + 4 * (st & 3);
+          const size_t at = slot < slots ? slot_row(slot) * a.q_stride + slot_dim(slot) + d : 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q[x][i][e] = slot < slots ? load_dt(a.q, at + e, a.dtype) : 0.f;
         }
-        const int32_t left = (int32_t)(len[x] - place(i, 0));
-        if (left < STEP || id0.x < 0 || id0.y < 0) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              if ((int32_t)(8 * j + 2 * t + e) >= left || (j < 2 ? id0.x : id0.y) < 0) sv[x][j][e] = -INFINITY;
-        }
-        const float c0 = fmaxf(fmaxf(sv[x][0][0], sv[x][0][1]), fmaxf(sv[x][1][0], sv[x][1][1]));
-        const float c1 = fmaxf(fmaxf(sv[x][2][0], sv[x][2][1]), fmaxf(sv[x][3][0], sv[x][3][1]));
-        float mn = fmaxf(c0, c1), Mn = fmaxf(c0 + E[0], c1 + E[1]);
-#pragma unroll
-        for (int y = 1; y <= 2; y <<= 1) {
-          mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, y));
-          Mn = fmaxf(Mn, __shfl_xor_sync(0xffffffffu, Mn, y));
-        }
-        mn = fmaxf(m[x], mn), Mn = fmaxf(M[x], Mn);
-        if (__any_sync(0xffffffffu, mn > m[x] || Mn > M[x])) {
-          const float al = m[x] == mn ? 1.f : ex2(m[x] - mn), aM = M[x] == Mn ? 1.f : ex2(M[x] - Mn);
-          l[x] *= al;
-          // the outputs of lane (g, t) are slots 2t and 2t + 1
-          const float a0 = __shfl_sync(0xffffffffu, aM, 8 * t), a1 = __shfl_sync(0xffffffffu, aM, 8 * t + 4);
-#pragma unroll
-          for (int j = 0; j < HD / 16; ++j) o[x][j][0] *= a0, o[x][j][1] *= a1, o[x][j][2] *= a0, o[x][j][3] *= a1;
-          m[x] = mn;
-          M[x] = Mn;
-        }
-        // a step without positions may leave the maxima at -inf: its weights are 0
-        m0[x] = m[x] == -INFINITY ? 0.f : m[x], M0[x] = M[x] == -INFINITY ? 0.f : M[x];
       }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t hi0[SETS], lo0[SETS], hi1[SETS], lo1[SETS];
-        const float vo = E[h] + 14.f;  // weights up to 2^15: their low parts stay normal f16
-#pragma unroll
-        for (int x = 0; x < SETS; ++x) {
-          float wt[4];
-          // (an infinite scale of positions that the slot does not see)
-          const float f = (int32_t)(len[x] - place(i, h)) <= 0 ? 0.f : vf[h];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float y = sv[x][2 * h + (e >> 1)][e & 1];
-            l[x] += ex2(y - m0[x]);
-            wt[e] = ex2((y - M0[x]) + vo) * f;
-          }
-          split2(wt[0], wt[1], hi0[x], lo0[x]);
-          split2(wt[2], wt[3], hi1[x], lo1[x]);
+
+      // ---- this warp's steps: units ua .. ub - 1, positions UNIT u + STEP warp ----
+      const uint32_t steps = (rw.len + STEP - 1) / STEP;
+      const uint32_t last_u = steps > warp ? (steps - warp + WARPS - 1) / WARPS : 0;  // units with a step of this warp
+      const int32_t n = (int32_t)min(ub, last_u) - (int32_t)ua;
+      auto place = [&](int32_t i, int half) { return (ua + (uint32_t)i) * UNIT + warp * STEP + half * SUB; };
+      // a table entry is checked a step after it is read, when it has arrived
+      auto entry = [&](int32_t i, int half) -> int32_t {
+        const uint32_t p = place(i, half);
+        return i < n && p < rw.len ? table[p >> bs] : -1;
+      };
+      auto checked = [&](int32_t i, int2 id) {
+        if ((uint32_t)id.x >= a.pool.n_blocks || (uint32_t)id.y >= a.pool.n_blocks) {
+          if (i < n && ((uint32_t)id.x >= a.pool.n_blocks || place(i, 1) < rw.len)) set_error(a.err, DERR_BAD_POS);
+          if ((uint32_t)id.x >= a.pool.n_blocks) id.x = -1;
+          if ((uint32_t)id.y >= a.pool.n_blocks) id.y = -1;
         }
-        const uint8_t* vp = here + L::KBUF + (i & 1) * L::KBUF + h * L::HALF;
-        uint32_t vr[4][L::NW];
+        return id;
+      };
+      auto issue_k = [&](int32_t i, int2 id) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if constexpr (HD == 128) {
-            const uint4 x = *reinterpret_cast<const uint4*>(vp + v_at + ((r & 1) + 8 * (r >> 1)) * HD);
-            vr[r][0] = x.x, vr[r][1] = x.y, vr[r][2] = x.z, vr[r][3] = x.w;
-          } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(vp + (v_at ^ ((r & 1) * 64)) + 8 * (r >> 1) * HD);
-            vr[r][0] = x.x, vr[r][1] = x.y;
-          }
+        for (int h = 0; h < 2; ++h)
+          if ((h ? id.y : id.x) >= 0)
+            fetch<HD, TYPE, false>(a.pool.k + first_row(a, h ? id.y : id.x, kvh, place(i, h)) * HD, ring + h * L::HALF, 0,
+                                   lane);
+        copy_commit();
+      };
+      auto issue_v = [&](int32_t i, int2 id) {
+        const uint32_t dst = ring + L::KBUF + (i & 1) * L::KBUF;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if ((h ? id.y : id.x) >= 0)
+            fetch<HD, TYPE, true>(a.pool.v + first_row(a, h ? id.y : id.x, kvh, place(i, h)) * HD, dst + h * L::HALF,
+                                  rw.len - place(i, h), lane);
+          else if (TYPE == PAGES_E4M3 && i < n)
+            fetch<HD, TYPE, true>(a.pool.v, dst + h * L::HALF, 0, lane);
         }
-        // tile j: rows g and g + 8 are dims 2j and 2j + 1 of the lane's run
+        copy_commit();
+      };
+      auto scales = [&](int32_t id) {
+        const size_t at = (size_t)(id < 0 ? 0 : id) * n_kv + kvh;
+        return make_float2(a.pool.ks[at], a.pool.vs[at]);
+      };
+      float m[SETS], M[SETS], l[SETS], o[SETS][HD / 16][4];
 #pragma unroll
-        for (int w = 0; w < L::NW; ++w)
+      for (int x = 0; x < SETS; ++x) {
+        m[x] = M[x] = -INFINITY, l[x] = 0.f;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            uint4 va;
-            to_f16<TYPE>(__byte_perm(vr[0][w], vr[1][w], e ? 0x7362 : 0x5140), va.x, va.y);
-            to_f16<TYPE>(__byte_perm(vr[2][w], vr[3][w], e ? 0x7362 : 0x5140), va.z, va.w);
+        for (int j = 0; j < HD / 16; ++j) o[x][j][0] = o[x][j][1] = o[x][j][2] = o[x][j][3] = 0.f;
+      }
+      int2 id0{-1, -1}, id1{-1, -1};
+      float2 sx{}, sy{};
+      if (n > 0) {  // the first copies are on their way before q is needed
+        id0 = int2{entry(0, 0), entry(0, 1)};
+        id1 = int2{entry(1, 0), entry(1, 1)};
+        id0 = checked(0, id0);
+        issue_k(0, id0);
+        issue_v(0, id0);
+        sx = scales(id0.x), sy = scales(id0.y);
+      }
+
+      // q scaled by a power of two so that the largest magnitude of a head is in [2^14, 2^15)
+      if (tid < SLOTS) qmax[tid] = 0;
+      __syncthreads();
 #pragma unroll
-            for (int x = 0; x < SETS; ++x) {
-              float s16[4] = {};
-              mma_f16(s16, va, lo0[x], lo1[x]);
-              mma_f16(s16, va, hi0[x], hi1[x]);
-              float(&to)[4] = o[x][2 * w + e];
+      for (int x = 0; x < SETS; ++x) {
+        float big = 0.f;
 #pragma unroll
-              for (int k = 0; k < 4; k += 2) {
-                const float2 sum = __fadd2_rn(make_float2(to[k], to[k + 1]), make_float2(s16[k], s16[k + 1]));
-                to[k] = sum.x, to[k + 1] = sum.y;
-              }
+        for (int i = 0; i < L::STEPS / WARPS; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(q[x][i][e]));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        if (t == 0) atomicMax(&qmax[HEADS * x + g], __float_as_int(big));
+      }
+      __syncthreads();
+      float qscale[SETS];
+#pragma unroll
+      for (int x = 0; x < SETS; ++x) {
+        const float top = __int_as_float(qmax[HEADS * x + g]);
+        int ex = 0;
+        if (top > 0.f && top < INFINITY) ex = min(14 - ilogbf(top), 126);
+        const float up = ldexpf(1.f, ex);
+        qscale[x] = a.scale * 1.4426950408889634f * ldexpf(1.f, -ex);
+#pragma unroll
+        for (int i = 0; i < L::STEPS / WARPS; ++i) {
+          uint4 f;
+          split2(q[x][i][0] * up, q[x][i][1] * up, f.x, f.y);
+          split2(q[x][i][2] * up, q[x][i][3] * up, f.z, f.w);
+          qf[(x * L::STEPS + warp + WARPS * i) * 32 + lane] = f;
+        }
+      }
+      __syncthreads();
+
+      for (int32_t i = 0; i < n; ++i) {
+        id1 = checked(i + 1, id1);
+        issue_v(i + 1, id1);
+        const float2 nx = scales(id1.x), ny = scales(id1.y);
+        const int2 id2{entry(i + 2, 0), entry(i + 2, 1)};
+        copy_wait<1>();  // this step's K and V; the next V may be on its way
+        __syncwarp();
+        const uint8_t* here = att_smem + warp * L::RING;
+        float acc[SETS][4][4] = {};
+#pragma unroll
+        for (int pi = 0; pi < L::NP; ++pi) {
+          uint32_t kw[4][4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint4 x = *reinterpret_cast<const uint4*>(here + (j >> 1) * L::HALF + k_at[pi] + (j & 1) * 8 * HD);
+            kw[j][0] = x.x, kw[j][1] = x.y, kw[j][2] = x.z, kw[j][3] = x.w;
+          }
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            uint4 qa[SETS];
+#pragma unroll
+            for (int x = 0; x < SETS; ++x) qa[x] = qf[(x * L::STEPS + 4 * pi + w) * 32 + lane];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint32_t b0, b1;
+              to_f16<TYPE>(kw[j][w], b0, b1);
+#pragma unroll
+              for (int x = 0; x < SETS; ++x) mma_f16(acc[x][j], qa[x], b0, b1);
             }
           }
-      }
-      id0 = id1, id1 = id2;
-      sx = nx, sy = ny;
-      __syncwarp();  // the next V goes where this one was
-    }
-    copy_wait<0>();
-
-    // ---- the warps' outputs meet in shared memory (each in its own ring) ----
-    const bool whole = ua == 0 && ub == rw.units;
-    const uint32_t mine = start == first ? 0 : 1;
-    if (!whole && tid == 0 && ua == 0)
-      headers[c] = Header{(int32_t)row, (int32_t)item, (int32_t)(((base + (uint64_t)(item + 1) * span) * C - 1) / U),
-                          (int32_t)(mine + 2 * (MANY ? rw.rows : 1))};
-    __syncwarp();
-#pragma unroll
-    for (int x = 0; x < SETS; ++x) {
-      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
-      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-      // lane (g, t): slots 2t and 2t + 1, the HD / 8 dims from HD / 8 g
-      float* mo = reinterpret_cast<float*>(att_smem + warp * L::RING) + (HEADS * x + 2 * t) * L::HROW + g * (HD / 8);
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int j = 0; j < HD / 16; j += 2)
-          *reinterpret_cast<float4*>(mo + r * L::HROW + 2 * j) =
-              make_float4(o[x][j][r], o[x][j][r + 2], o[x][j + 1][r], o[x][j + 1][r + 2]);
-      if (t == 0) stat[warp][HEADS * x + g][0] = m[x], stat[warp][HEADS * x + g][1] = M[x], stat[warp][HEADS * x + g][2] = l[x];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int x = 0; x < SETS; ++x) {
-      float* rec = records + ((size_t)(2 * c + mine) * SETS + x) * L::REC;
-      constexpr int PER = HD * HEADS / THREADS;  // consecutive dims of one slot per thread
-      const uint32_t h = tid / (HD / PER), d = (tid % (HD / PER)) * PER;
-      float mm = -INFINITY, MM = -INFINITY, ll = 0.f;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, stat[w][HEADS * x + h][0]), MM = fmaxf(MM, stat[w][HEADS * x + h][1]);
-      float out[PER] = {};
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float lw = stat[w][HEADS * x + h][2];
-        if (lw == 0.f) continue;  // a warp without positions
-        ll += lw * ex2(stat[w][HEADS * x + h][0] - mm);
-        const float f = ex2(stat[w][HEADS * x + h][1] - MM);
-        const float* src = reinterpret_cast<const float*>(att_smem + w * L::RING) + (HEADS * x + h) * L::HROW + d;
-#pragma unroll
-        for (int e = 0; e < PER; ++e) out[e] += src[e] * f;
-      }
-      if (whole) {
-        const uint32_t slot = HEADS * x + h;
-        if (slot < slots) {
-          // MM - mm is at most the largest exponent of a scale
-          const float2 f = out_factor(MM - mm - 14.f, ll);
-          const size_t at = slot_row(slot) * a.out_stride + slot_dim(slot) + d;
-#pragma unroll
-          for (int e = 0; e < PER; ++e) store_dt(a.out, at + e, a.dtype, ll == 0.f ? 0.f : out[e] * f.x * f.y);
         }
-      } else {
+        __syncwarp();
+        issue_k(i + 1, id1);  // this step's K has been multiplied
+        // a V scale is 2^E * vf, vf below 2 (also for a scale of 0, an infinite one or NaN)
+        float E[2], vf[2];
 #pragma unroll
-        for (int e = 0; e < PER; e += 4)
-          *reinterpret_cast<float4*>(rec + h * HD + d + e) = make_float4(out[e], out[e + 1], out[e + 2], out[e + 3]);
-        if (d == 0) rec[HEADS * HD + h] = mm, rec[HEADS * (HD + 1) + h] = MM, rec[HEADS * (HD + 2) + h] = ll;
+        for (int h = 0; h < 2; ++h) {
+          const float vs = (h ? id0.y : id0.x) < 0 ? 0.f : h ? sy.y : sx.y;
+          const int e8 = max(1, min(254, (int)((__float_as_uint(vs) >> 23) & 255)));
+          E[h] = (float)(e8 - 127);
+          vf[h] = e8 == 254 ? vs * 0x1p-127f : vs * __int_as_float((254 - e8) << 23);
+        }
+        // scores in powers of two; lane (g, t) holds slot g at positions 8 j + 2t, 8 j + 2t + 1
+        float sv[SETS][4][2], m0[SETS], M0[SETS];
+#pragma unroll
+        for (int x = 0; x < SETS; ++x) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float f = (j < 2 ? sx.x : sy.x) * qscale[x];
+            sv[x][j][0] = (acc[x][j][0] + acc[x][j][2]) * f;
+            sv[x][j][1] = (acc[x][j][1] + acc[x][j][3]) * f;
+          }
+          const int32_t left = (int32_t)(len[x] - place(i, 0));
+          if (left < STEP || id0.x < 0 || id0.y < 0) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if ((int32_t)(8 * j + 2 * t + e) >= left || (j < 2 ? id0.x : id0.y) < 0) sv[x][j][e] = -INFINITY;
+          }
+          const float c0 = fmaxf(fmaxf(sv[x][0][0], sv[x][0][1]), fmaxf(sv[x][1][0], sv[x][1][1]));
+          const float c1 = fmaxf(fmaxf(sv[x][2][0], sv[x][2][1]), fmaxf(sv[x][3][0], sv[x][3][1]));
+          float mn = fmaxf(c0, c1), Mn = fmaxf(c0 + E[0], c1 + E[1]);
+#pragma unroll
+          for (int y = 1; y <= 2; y <<= 1) {
+            mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, y));
+            Mn = fmaxf(Mn, __shfl_xor_sync(0xffffffffu, Mn, y));
+          }
+          mn = fmaxf(m[x], mn), Mn = fmaxf(M[x], Mn);
+          if (__any_sync(0xffffffffu, mn > m[x] || Mn > M[x])) {
+            const float al = m[x] == mn ? 1.f : ex2(m[x] - mn), aM = M[x] == Mn ? 1.f : ex2(M[x] - Mn);
+            l[x] *= al;
+            // the outputs of lane (g, t) are slots 2t and 2t + 1
+            const float a0 = __shfl_sync(0xffffffffu, aM, 8 * t), a1 = __shfl_sync(0xffffffffu, aM, 8 * t + 4);
+#pragma unroll
+            for (int j = 0; j < HD / 16; ++j) o[x][j][0] *= a0, o[x][j][1] *= a1, o[x][j][2] *= a0, o[x][j][3] *= a1;
+            m[x] = mn;
+            M[x] = Mn;
+          }
+          // a step without positions may leave the maxima at -inf: its weights are 0
+          m0[x] = m[x] == -INFINITY ? 0.f : m[x], M0[x] = M[x] == -INFINITY ? 0.f : M[x];
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t hi0[SETS], lo0[SETS], hi1[SETS], lo1[SETS];
+          const float vo = E[h] + 14.f;  // weights up to 2^15: their low parts stay normal f16
+#pragma unroll
+          for (int x = 0; x < SETS; ++x) {
+            float wt[4];
+            // (an infinite scale of positions that the slot does not see)
+            const float f = (int32_t)(len[x] - place(i, h)) <= 0 ? 0.f : vf[h];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float y = sv[x][2 * h + (e >> 1)][e & 1];
+              l[x] += ex2(y - m0[x]);
+              wt[e] = ex2((y - M0[x]) + vo) * f;
+            }
+            split2(wt[0], wt[1], hi0[x], lo0[x]);
+            split2(wt[2], wt[3], hi1[x], lo1[x]);
+          }
+          const uint8_t* vp = here + L::KBUF + (i & 1) * L::KBUF + h * L::HALF;
+          uint32_t vr[4][L::NW];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if constexpr (HD == 128) {
+              const uint4 x = *reinterpret_cast<const uint4*>(vp + v_at + ((r & 1) + 8 * (r >> 1)) * HD);
+              vr[r][0] = x.x, vr[r][1] = x.y, vr[r][2] = x.z, vr[r][3] = x.w;
+            } else {
+              const uint2 x = *reinterpret_cast<const uint2*>(vp + (v_at ^ ((r & 1) * 64)) + 8 * (r >> 1) * HD);
+              vr[r][0] = x.x, vr[r][1] = x.y;
+            }
+          }
+          // tile j: rows g and g + 8 are dims 2j and 2j + 1 of the lane's run
+#pragma unroll
+          for (int w = 0; w < L::NW; ++w)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              uint4 va;
+              to_f16<TYPE>(__byte_perm(vr[0][w], vr[1][w], e ? 0x7362 : 0x5140), va.x, va.y);
+              to_f16<TYPE>(__byte_perm(vr[2][w], vr[3][w], e ? 0x7362 : 0x5140), va.z, va.w);
+#pragma unroll
+              for (int x = 0; x < SETS; ++x) {
+                float s16[4] = {};
+                mma_f16(s16, va, lo0[x], lo1[x]);
+                mma_f16(s16, va, hi0[x], hi1[x]);
+                float(&to)[4] = o[x][2 * w + e];
+#pragma unroll
+                for (int k = 0; k < 4; k += 2) {
+                  const float2 sum = __fadd2_rn(make_float2(to[k], to[k + 1]), make_float2(s16[k], s16[k + 1]));
+                  to[k] = sum.x, to[k + 1] = sum.y;
+                }
+              }
+            }
+        }
+        id0 = id1, id1 = id2;
+        sx = nx, sy = ny;
+        __syncwarp();  // the next V goes where this one was
       }
-    }
-    __syncthreads();  // the rings and stat are free again
+      copy_wait<0>();
+
+      // ---- the warps' outputs meet in shared memory (each in its own ring) ----
+      const bool whole = ua == 0 && ub == rw.units;
+      const uint32_t mine = start == first ? 0 : 1;
+      if (!whole && tid == 0 && ua == 0)
+        headers[c] = Header{(int32_t)row, (int32_t)item, (int32_t)(((base + (uint64_t)(item + 1) * span) * C - 1) / U),
+                            (int32_t)(mine + 2 * (MANY ? rw.rows : 1))};
+      __syncwarp();
+#pragma unroll
+      for (int x = 0; x < SETS; ++x) {
+        l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+        l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+        // lane (g, t): slots 2t and 2t + 1, the HD / 8 dims from HD / 8 g
+        float* mo = reinterpret_cast<float*>(att_smem + warp * L::RING) + (HEADS * x + 2 * t) * L::HROW + g * (HD / 8);
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int j = 0; j < HD / 16; j += 2)
+            *reinterpret_cast<float4*>(mo + r * L::HROW + 2 * j) =
+                make_float4(o[x][j][r], o[x][j][r + 2], o[x][j + 1][r], o[x][j + 1][r + 2]);
+        float* st = stat[warp][HEADS * x + g];
+        if (t == 0) st[0] = m[x], st[1] = M[x], st[2] = l[x];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int x = 0; x < SETS; ++x) {
+        float* rec = records + ((size_t)(2 * c + mine) * SETS + x) * L::REC;
+        constexpr int PER = HD * HEADS / THREADS;  // consecutive dims of one slot per thread
+        const uint32_t h = tid / (HD / PER), d = (tid % (HD / PER)) * PER;
+        float mm = -INFINITY, MM = -INFINITY, ll = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w)
+          mm = fmaxf(mm, stat[w][HEADS * x + h][0]), MM = fmaxf(MM, stat[w][HEADS * x + h][1]);
+        float out[PER] = {};
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          const float lw = stat[w][HEADS * x + h][2];
+          if (lw == 0.f) continue;  // a warp without positions
+          ll += lw * ex2(stat[w][HEADS * x + h][0] - mm);
+          const float f = ex2(stat[w][HEADS * x + h][1] - MM);
+          const float* src = reinterpret_cast<const float*>(att_smem + w * L::RING) + (HEADS * x + h) * L::HROW + d;
+#pragma unroll
+          for (int e = 0; e < PER; ++e) out[e] += src[e] * f;
+        }
+        if (whole) {
+          const uint32_t slot = HEADS * x + h;
+          if (slot < slots) {
+            // MM - mm is at most the largest exponent of a scale
+            const float2 f = out_factor(MM - mm - 14.f, ll);
+            const size_t at = slot_row(slot) * a.out_stride + slot_dim(slot) + d;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) store_dt(a.out, at + e, a.dtype, ll == 0.f ? 0.f : out[e] * f.x * f.y);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < PER; e += 4)
+            *reinterpret_cast<float4*>(rec + h * HD + d + e) = make_float4(out[e], out[e + 1], out[e + 2], out[e + 3]);
+          if (d == 0) rec[HEADS * HD + h] = mm, rec[HEADS * (HD + 1) + h] = MM, rec[HEADS * (HD + 2) + h] = ll;
+        }
+      }
+      __syncthreads();  // the rings and stat are free again
     }
     if (next_row) {
       base = s;
