@@ -335,8 +335,9 @@ int shk_cuda_pages_truncate(shk_ctx *ctx, uint32_t n_seq, uint32_t block_tokens,
  * makes the scale infinite (the block then reads as NaN).  The rows of one
  * block must be consecutive in the call and rising by one, as
  * shk_cuda_pages_assign lays them out: a block's second run in one call is not
- * stored, and shk_cuda_check returns SHK_EDEVICE.  Calls that append to one
- * block must be ordered (one stream).  Async on stream. */
+ * stored, and shk_cuda_check returns SHK_EDEVICE.  (The search for such runs grows
+ * with the square of n_tokens: better several calls above 100000.)  Calls that
+ * append to one block must be ordered (one stream).  Async on stream. */
 int shk_cuda_pages_append(shk_ctx *ctx, const struct shk_pages *pages, uint32_t n_tokens, const void *k_dev,
                           const void *v_dev, uint32_t dtype, size_t row_stride, const int32_t *slots_dev,
                           void *stream);
@@ -355,7 +356,9 @@ int shk_cuda_pages_read(shk_ctx *ctx, const struct shk_pages *pages, uint32_t n_
  * with two strides the whole ranges count).  Sums and softmax in fp32; a
  * position's weight times its V scale enters the output to 2^-22 of itself or
  * 2^-39 of the row's largest such product, whichever is more.  Rows of one request
- * that follow one another read its blocks together.  What no row of the call
+ * that follow one another read its blocks together; how many may is chosen from
+ * n_rows and n_seq, so padding rows and idle request slots far beyond the live
+ * ones make the call slower (up to 1.7 times).  What no row of the call
  * sees may hold anything; between a row's last position and that of a
  * neighbour in its request, E4M3 bytes have to be numbers, as shk_cuda_pages_append
  * writes them.  ws_dev:

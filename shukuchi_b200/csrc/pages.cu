@@ -454,10 +454,12 @@ __device__ __noinline__ void refuse_runs(const uint32_t* run_block, const uint32
 // its rows in their registers.
 // A block whose rows come in two runs of one call would be written by two CTAs at
 // once: the later run is refused, so each CTA looks through the earlier tokens for
-// the blocks of its own runs (a bit per hashed block first).
+// the blocks of its own runs (a bit per hashed block first).  That is a number of
+// reads that grows with the square of the call's tokens: nothing to be seen of it
+// at 20000 (62 us), a sixth of the time at 65536 (242 us), two fifths at 131072 (694).
 //
-// 6300 tokens of bf16 (8 heads of 128) into e4m3 blocks of 64: 21 us (1.8 TB/s) in
-// a row of calls, bound by instructions (22 an element, most of them the two
+// 6300 tokens of bf16 (8 heads of 128) into e4m3 blocks of 64: 20 to 22 us (1.8 TB/s)
+// in a row of calls, bound by instructions (22 an element, most of them the two
 // roundings of round4) at 0.5 a cycle and by 3 or 4 CTAs on an SM; 32 tokens 5 us.
 template <int HD, uint32_t TYPE, uint32_t DT>
 __global__ void __launch_bounds__(APP_THREADS, 4) append_kernel(PagesPool p, uint32_t n, const void* k, const void* v,
@@ -693,8 +695,11 @@ cudaError_t pages_append_launch(const PagesPool& p, uint32_t n, const void* k, c
                                 size_t row_stride, const int32_t* slots, int* err, int num_sms, cudaStream_t st) {
   // Few tokens, or blocks of 16: short runs, a warp per item, so 8 (head, K or V)
   // pairs to a CTA.  Else one pair to a CTA and whole blocks of tokens to it.
-  // (4000 requests' single tokens, with the read: 130 us with 8 pairs, 144 with
-  // one; 6300 tokens of prompts in blocks of 64: 52 and 36.)
+  // (8 heads of 128, bf16 to e4m3: 6300 tokens of prompts in blocks of 64 34 us with
+  // 8 pairs, 22 with one; in blocks of 16 18.6 and 20.5.  Runs are known on the
+  // device alone, so the rule goes by n and loses where they are unlike that: 4000
+  // single tokens in blocks of 64 take 59 us with one pair where 8 would take 35,
+  // two prompts of 150 take 22 with 8 where one would take 11.)
   const uint32_t all = 2 * p.n_kv, full = 4 * (uint32_t)num_sms, bt = 1u << p.block_shift;
   const bool by_warp = bt <= 16 || (uint64_t)n * all <= (uint64_t)APP_WARPS * full;
   const uint32_t pairs = by_warp ? APP_WARPS : 1, ny = (all + pairs - 1) / pairs;

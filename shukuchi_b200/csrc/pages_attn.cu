@@ -37,11 +37,13 @@
 // calls, for scales that K/V of one model and head do not have.
 //
 // Measured (64 heads over 8 of 128): 16 requests of 30k to 65k positions, e4m3,
-// 270 to 290 us, 5.6 to 6.0 TB/s; 32 of 1 to 8192, i8, 65 us, 4.3 TB/s, of which
-// the join is 9; one of 8192 16.4 us, one of 777 (32 heads) 11 us, both chains of
-// loads that wait on one another.  64 x 4 rows of 100 to 2000 positions (32 heads
-// over 4 of 64) 40 us: instructions, 770 a warp's step of 32 positions for 16
-// slots at 0.54 a cycle.  Five and six CTAs an SM there: 47 and 52 us.
+// 313 to 316 us, 5.2 TB/s; 32 of 1 to 8192, i8, 71 us, 3.9 TB/s, of which the join
+// is 9; one of 8192 16.9 us, one of 777 (32 heads) 11.5 us, both chains of loads
+// that wait on one another.  64 x 4 rows of 100 to 2000 positions (32 heads over 4
+// of 64) 41 us: instructions, 800 a warp's step of 32 positions for 16 slots at
+// 0.54 a cycle.  Five and six CTAs an SM there: 47 and 52 us.  A prompt's rows have
+// no tile of their own, K/V are read and converted again for every 16 / G of them:
+// 2048 rows of 32 heads over 8 of 128 on their own causal positions 366 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -790,6 +792,10 @@ cudaError_t attend_go(const PagesAttnArgs& a, int num_sms, cudaStream_t st) {
   // Rows of one request share an item of one set as well: 5 rows of 16 heads over 16:
   // 111 us apart, 51 together.  The search for such rows costs other calls 0.5 us
   // of instruction fetches, so they go without.
+  // Which rows are live only the device knows, so the rule goes by the arrays' sizes
+  // and picks the other variant where padding changes those (32 heads over 8 of 128,
+  // lengths to 2000): 64 single rows in 64 rows 44 us, in 256 rows of 64 requests
+  // 64; 4 rows each of 32 requests in 128 rows of 32 request slots 39, of 256 slots 67.
   const uint64_t G = a.n_heads / a.pool.n_kv;
   if (a.n_rows * G > (uint64_t)HEADS * min(a.n_seq, a.n_rows)) return attend_sets<HD, TYPE, 2, true>(a, num_sms, st);
   return a.row_seq && a.n_rows > a.n_seq ? attend_sets<HD, TYPE, 1, true>(a, num_sms, st)
