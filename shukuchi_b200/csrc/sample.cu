@@ -26,8 +26,8 @@
 //
 // Bound by instructions: about 100 a token with top-p (two exponentials of libm
 // quality, exact integer sums, the bin), IPC 0.58 of 1 with two CTAs an SM, the
-// rest barriers.  128256 logits: 11.5 us a row alone, 42 us for 64 rows of mixed
-// settings (0.79 TB/s); 333 rows of 32000 51 us with top-p, 31 with temperature alone.
+// rest barriers.  128256 logits: 11.5 us a row alone, 40 us for 64 rows of mixed
+// settings (0.82 TB/s); 333 rows of 32000 51 us with top-p, 31 with temperature alone.
 // Slices of 8192 logits (three or four CTAs an SM) 71 to 80 us for the 333 rows,
 // of 32768 60 (and 50 against 53 for 64 rows with top-p, 29 against 36 with top-k).
 #include <cuda_bf16.h>

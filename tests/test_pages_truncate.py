@@ -2,9 +2,11 @@
 server that rejects drafts step after step keeps every block of its pool."""
 import numpy as np
 import pytest
+import torch
 
+import test_request_batch as batch
 from shukuchi_b200 import cuda as sc
-from test_pages import assign_reference, dev, p, tables_case
+from test_pages import append_reference, assign_reference, attend_reference, dev, p, tables_case
 
 gpu = pytest.mark.gpu
 
@@ -95,3 +97,52 @@ def test_truncate_arguments(ctx):
             with pytest.raises(sc.ShkError):
                 ctx.pages_truncate(1, 16, 4, 1, *[bad if i == at else p(x) for i in range(7)])
     ctx.check()
+
+
+class Drafts(batch.Server):
+    """A step that begins with the lengths to keep (in `done`), as after a check of drafts."""
+
+    def step(self, stream=None):
+        c, n = self.ctx, self.n
+        c.pages_truncate(n, self.block, self.n_blocks, self.stride, p(self.table), p(self.done), p(self.lens), p(self.lens),
+                         p(self.free), p(self.counts), p(self.counts), stream=stream)
+        c.pages_assign(n, self.block, self.n_blocks, self.stride, self.rows, p(self.lens), p(self.add), p(self.table),
+                       p(self.free), p(self.counts), p(self.lens), p(self.counts), p(self.slot), p(self.pos), p(self.seq),
+                       p(self.last), stream=stream)
+        self.pool.pages.append(self.rows, p(self.k), p(self.v), p(self.slot), stream=stream)
+        self.pool.pages.attend(self.rows, p(self.q), p(self.out), self.H, p(self.pos), p(self.table), self.stride, n, 0.125,
+                               p(self.ws), self.ws.numel(), row_seq=p(self.seq), stream=stream)
+
+
+@gpu
+def test_draft_steps(ctx):
+    """Steps of drafts whose rejected rows are cut off again: pools and outputs against the references, and a captured
+    step replayed against the calls, bit for bit."""
+    eager, graph = (Drafts(ctx, np.random.default_rng(5), 12, 60, 16, 96) for _ in range(2))
+    g, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=side):
+        graph.step(stream=side.cuda_stream)
+    rng, lens = np.random.default_rng(9), np.zeros(12, int)
+    for step in range(9):
+        # of the four or more tokens that the last step added one to all stay; long requests end
+        keep = np.where(lens > 90, 0, np.maximum(lens - rng.integers(0, 4, 12), 0))
+        add = np.where(rng.random(12) < 0.2, 0, np.where(keep == 0, rng.integers(1, 40, 12) if step % 3 == 0 else 4, 4))
+        for s in (eager, graph):
+            s.fill(np.random.default_rng(100 + step), add, keep)
+        eager.step()
+        g.replay()
+        torch.cuda.synchronize()
+        ctx.check()
+        for a, b in zip(eager.state(), graph.state()):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        lens, counts = eager.lens.cpu().numpy(), eager.counts.tolist()
+        assert counts[0] + (-(-lens // 16)).sum() == 60
+        slot, pos, seq = (x.cpu().numpy() for x in (eager.slot, eager.pos, eager.seq))
+        for i, x in enumerate((eager.k, eager.v)):
+            assert not append_reference(eager.pool.h[i], eager.pool.hs[i], x.cpu().numpy(), slot, 16, sc.PAGES_I8)
+        eager.pool.same()
+        ref, lim = attend_reference(eager.q.cpu().numpy().reshape(96, 8, 64), *eager.pool.values(), eager.table.cpu().numpy(),
+                                    seq, pos, 16, 8, 0.125)
+        out, live = eager.out.double().cpu().numpy().reshape(96, 8, 64), seq >= 0
+        assert np.all(np.abs(out - ref)[live] <= lim[live]) and (out[~live] == 7).all() and live.sum() == counts[1] > 0
